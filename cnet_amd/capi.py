@@ -116,6 +116,11 @@ SIGNATURES = {
     "cnet_adam_update": [c_fp] * 6 + [_l, C.c_float, C.c_float, _i, _i],
     "cnet_embedding_fwd": [c_fp, c_fp, _i, _i, c_fp, c_fp, c_fp, _l, _i, _i],
     "cnet_embedding_bwd": [c_fp, c_fp, c_fp, _l, c_fp, c_fp, _i, _i, _i, _i, _i],
+    "cnet_norm_gate_fwd": [c_fp, c_fp, _l, c_fp, c_fp, _l, c_fp, c_fp, _l, c_fp, _i, _i, C.c_float],
+    "cnet_norm_join_fwd": [c_fp, c_fp, _l] * 3 + [C.c_float, c_fp, c_fp, _l, c_fp, c_fp, c_fp, c_fp, c_fp, _l, c_fp, _i, _i, C.c_float],
+    "cnet_norm_gate_bwd_sym": [c_fp, c_fp, _l, c_fp, c_fp, c_fp, _l, c_fp, c_fp, _l] + ([c_fp] * 4 + [_l]) * 2 + [_i, _i, _i, _i],
+    "cnet_norm_join_bwd_sym": [c_fp, c_fp, _l, c_fp, c_fp, c_fp, _l, C.c_float, c_fp, c_fp, _l, c_fp, c_fp, c_fp] + [c_fp, c_fp, _l] * 2 +
+                              ([c_fp] * 4 + [_l]) * 3 + [c_fp] * 4 + [_i, _i, _i, _i],
     "cnet_last_error": [],
 }
 

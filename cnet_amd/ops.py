@@ -361,3 +361,38 @@ def linear_cross_entropy_fwd_bwd_sym(x, w, y, labels, s, loss, argmax, dz, out=N
     o = out.p() if out is not None else (None, None)
     call("cnet_clinear_cross_entropy_fwd_bwd_sym", *x.p(), x.ld, *w.p(), w.ld, *y.p(), y.ld, labels.ptr, o[0], o[1],
          out.ld if out is not None else 0, s.ptr, loss.ptr, argmax.ptr, *_pair(dz, mirror), dz.ld, x.rows, x.cols, w.rows)
+
+
+# ------------------------------------------------------------------------------------------------- norms around a block
+# Gradients may be Grads or, where only the dz planes are kept (operands, and results with mirror=False), CMats of those planes.
+def _opt(m):
+    """planes and leading dimension of an operand that may be left out"""
+    return (*m.p()[:2], m.ld) if m is not None else (None, None, 0)
+
+
+def _ptr(v):
+    return v.ptr if v is not None else None
+
+
+def norm_gate_fwd(x, v, y, s, eps, shared=True):
+    """y = v .* x / rms(x); s (or None) receives 1 / rms per row."""
+    call("cnet_norm_gate_fwd", *x.p(), x.ld, *v.p(), 0 if shared else v.ld, *y.p(), y.ld, _ptr(s), x.rows, x.cols, eps)
+
+
+def norm_gate_bwd_sym(x, s, v, g, dx, dv, shared=True, accumulate=0, accumulate_w=0, mirror=True, mirror_w=True):
+    call("cnet_norm_gate_bwd_sym", *x.p(), x.ld, s.ptr, *v.p(), 0 if shared else v.ld, *g.p()[:2], g.ld, *_pair(dx, mirror), dx.ld,
+         *_pair(dv, mirror_w), dv.ld, x.rows, x.cols, accumulate, accumulate_w)
+
+
+def norm_join_fwd(u, f, v, scale, h, s, w, y, s2, eps, shared=True):
+    """h = u + scale v .* f / rms(f) and y = w .* h / rms(h); w, y and s2 None behind the last block."""
+    assert (w is None) == (y is None)
+    call("cnet_norm_join_fwd", *u.p(), u.ld, *f.p(), f.ld, *v.p(), 0 if shared else v.ld, scale, *h.p(), h.ld, _ptr(s), *_opt(w)[:2], *_opt(y),
+         _ptr(s2), u.rows, u.cols, eps)
+
+
+def norm_join_bwd_sym(f, s, v, scale, h, s2, w, gh, gy, du, df, dv, dw, shared=True, accumulate=0, accumulate_w=0, mirror=True, mirror_w=True):
+    """gh: the gradient that reaches h along the residual path, gy: the one at y; either may be None (with gy None also h, s2, w, dw)."""
+    call("cnet_norm_join_bwd_sym", *f.p(), f.ld, s.ptr, *v.p(), 0 if shared else v.ld, scale, *_opt(h), _ptr(s2), *_opt(w)[:2], *_opt(gh), *_opt(gy),
+         *_pair(du, mirror), du.ld, *_pair(df, mirror), df.ld, *_pair(dv, mirror_w), dv.ld, *(_pair(dw, mirror_w) if dw is not None else (None,) * 4),
+         f.rows, f.cols, accumulate, accumulate_w)

@@ -519,6 +519,41 @@ int cnet_embedding_fwd(const float *table_re, const float *table_im, int dim, in
 int cnet_embedding_bwd(const int32_t *tokens, const float *g_dzs_re, const float *g_dzs_im, int64_t ldg,
                        float *table_dzs_re, float *table_dzs_im, int dim, int vocab, int rows, int slots, int accumulate);
 
+/* ---- Norms around a block of layers.  Upstream has the L2 normalisation of SoftMax only (impl/softmax.h:33-73) and no norm
+ *      with weights; these are what a deep stack of blocks needs next to Hadamard, Residual and SoftMax.
+ * cnet_norm_gate_fwd, in front of a block: y = v .* x s with s = 1 / max(sqrt(mean_k |x_k|^2 + eps), 1e-15), one s per row.
+ *      v: the gate, one shared row of weights (ldv == 0) or a row of its own for every row of x, as in cnet_hadamard_fwd.
+ *      s[rows] is what the backward pass reads; NULL when there will be none.
+ * cnet_norm_join_fwd, behind a block and in front of the next: h = u + scale v .* f s1 (u: the residual path, f: what the block
+ *      computed, s1 as above from f) and y = w .* h s2 (s2 from h; w one shared row).  w and y NULL: the last block, h alone.
+ *      s, s2: as above.
+ * All sums in fp32 over a fixed tree; an infinity or NaN of a row stays in that row.  Results must not overlap operands. */
+int cnet_norm_gate_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *v_re, const float *v_im, int64_t ldv,
+                       float *y_re, float *y_im, int64_t ldy, float *s, int rows, int cols, float eps);
+int cnet_norm_join_fwd(const float *u_re, const float *u_im, int64_t ldu, const float *f_re, const float *f_im, int64_t ldf,
+                       const float *v_re, const float *v_im, int64_t ldv, float scale,
+                       float *h_re, float *h_im, int64_t ldh, float *s, const float *w_re, const float *w_im,
+                       float *y_re, float *y_im, int64_t ldy, float *s2, int rows, int cols, float eps);
+/* Their backward passes for a conjugate gradient pair (see cnet_clinear_bwd_input_sym; every dz* half may be NULL), with the s
+ * and s2 of the forward pass.  g: the pair's dz planes at y.  dv, dw: summed over the rows in an order that depends on the sizes
+ * alone, or a row each with a gate of its own for every row.  accumulate != 0 adds into dx, du and df; accumulate_w into dv and
+ * dw.  With no rows the weights' gradients are those of an empty batch: zero, unless accumulate_w.
+ * The join: gh (the gradient that reaches h along the residual path) or gy (the one at y) may be NULL, not both; without gy
+ * neither h, s2, w nor dw is touched.  du receives the whole gradient at h = gh + what the norm hands back from gy. */
+int cnet_norm_gate_bwd_sym(const float *x_re, const float *x_im, int64_t ldx, const float *s, const float *v_re, const float *v_im, int64_t ldv,
+                           const float *g_dz_re, const float *g_dz_im, int64_t ldg,
+                           float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx,
+                           float *dv_dz_re, float *dv_dz_im, float *dv_dzs_re, float *dv_dzs_im, int64_t lddv,
+                           int rows, int cols, int accumulate, int accumulate_w);
+int cnet_norm_join_bwd_sym(const float *f_re, const float *f_im, int64_t ldf, const float *s, const float *v_re, const float *v_im, int64_t ldv,
+                           float scale, const float *h_re, const float *h_im, int64_t ldh, const float *s2, const float *w_re, const float *w_im,
+                           const float *gh_dz_re, const float *gh_dz_im, int64_t ldgh, const float *gy_dz_re, const float *gy_dz_im, int64_t ldgy,
+                           float *du_dz_re, float *du_dz_im, float *du_dzs_re, float *du_dzs_im, int64_t lddu,
+                           float *df_dz_re, float *df_dz_im, float *df_dzs_re, float *df_dzs_im, int64_t lddf,
+                           float *dv_dz_re, float *dv_dz_im, float *dv_dzs_re, float *dv_dzs_im, int64_t lddv,
+                           float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im,
+                           int rows, int cols, int accumulate, int accumulate_w);
+
 /* ---- Tuning overrides (environment variables).  None is needed for correct results or for the figures this library is
  *      measured with; they exist so that tests and sweeps can send a shape to every kernel that could take it.  Each is
  *      read ONCE per process, when the first launch that consults it is queued; results do not depend on them beyond
