@@ -121,6 +121,11 @@ SIGNATURES = {
     "cnet_norm_gate_bwd_sym": [c_fp, c_fp, _l, c_fp, c_fp, c_fp, _l, c_fp, c_fp, _l] + ([c_fp] * 4 + [_l]) * 2 + [_i, _i, _i, _i],
     "cnet_norm_join_bwd_sym": [c_fp, c_fp, _l, c_fp, c_fp, c_fp, _l, C.c_float, c_fp, c_fp, _l, c_fp, c_fp, c_fp] + [c_fp, c_fp, _l] * 2 +
                               ([c_fp] * 4 + [_l]) * 3 + [c_fp] * 4 + [_i, _i, _i, _i],
+    "cnet_distill_fwd": [c_fp, c_fp, _l, c_fp, c_fp, _i, c_fp, c_fp, _i, _i],
+    "cnet_distill_bwd_sym": [c_fp, c_fp, _l, c_fp, c_fp, c_fp, _i] + [c_fp] * 4 + [_l, _i, _i],
+    "cnet_distill_fwd_bwd_sym": [c_fp, c_fp, _l, c_fp, c_fp, _i, c_fp, c_fp] + [c_fp] * 4 + [_l, _i, _i],
+    "cnet_vocab_head_fwd": [c_fp, c_fp, _l, c_fp, c_fp, _l, c_fp, c_fp, c_fp, c_fp, _i, _i, _i],
+    "cnet_vocab_head_fwd_bwd_sym": [c_fp, c_fp, _l, c_fp, c_fp, _l, c_fp, c_fp, c_fp, c_fp] + ([c_fp] * 4 + [_l, _i]) * 2 + [_i, _i, _i],
     "cnet_last_error": [],
 }
 

@@ -41,6 +41,10 @@ struct Runtime {
 	// sums (the folded samples of the transform of real input)
 	void *operand_workspace = nullptr;
 	size_t operand_workspace_bytes = 0;
+	// a third, for what an entry point keeps between the matrix products it runs (the vocabulary head: a piece of logits and
+	// per-row sums), which use the other two themselves
+	void *vocab_workspace = nullptr;
+	size_t vocab_workspace_bytes = 0;
 	// A recorded graph holds the workspace address it was recorded with: while any recording exists, a workspace that
 	// has to grow is retired (kept until shutdown) instead of freed.
 	// Each live recording is kept as (executable, the graph it was instantiated from): the template graph lives as long
@@ -61,6 +65,7 @@ int hip_fail(hipError_t e, const char *what);
 // returns nullptr (and records the error) when the allocation fails
 void *workspace(size_t bytes);
 void *operand_workspace(size_t bytes);  // the second buffer (Runtime::operand_workspace); same rules
+void *vocab_workspace(size_t bytes);    // the third (Runtime::vocab_workspace); same rules
 // every hipFuncSetAttribute the matrix kernels need, made once, outside any stream capture (cgemm.hip)
 int cgemm_prime_attributes();
 

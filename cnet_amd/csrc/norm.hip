@@ -48,7 +48,11 @@ struct BwdArgs {
 	int rows, cols, accumulate, accumulate_w;
 };
 
-__device__ __forceinline__ float inv_rms(float sum, int cols, float eps) { return 1.0f / fmaxf(sqrtf(sum / (float) cols + eps), 1.0e-15f); }
+// (the clamp lets a NaN through, which fmaxf would not: the whole row is then NaN)
+__device__ __forceinline__ float inv_rms(float sum, int cols, float eps) {
+	const float rms = sqrtf(sum / (float) cols + eps);
+	return 1.0f / (rms <= 1.0e-15f ? 1.0e-15f : rms);
+}
 
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
 

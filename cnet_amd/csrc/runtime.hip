@@ -63,6 +63,8 @@ void *workspace(size_t bytes) { return grown(rt().workspace, rt().workspace_byte
 
 void *operand_workspace(size_t bytes) { return grown(rt().operand_workspace, rt().operand_workspace_bytes, bytes); }
 
+void *vocab_workspace(size_t bytes) { return grown(rt().vocab_workspace, rt().vocab_workspace_bytes, bytes); }
+
 void release_twiddles();  // cdft.hip
 int init_static_scratch(int device);  // reduce.hip
 
@@ -167,6 +169,9 @@ int cnet_shutdown(void) {
 	if (r.operand_workspace) hipFree(r.operand_workspace);
 	r.operand_workspace = nullptr;
 	r.operand_workspace_bytes = 0;
+	if (r.vocab_workspace) hipFree(r.vocab_workspace);
+	r.vocab_workspace = nullptr;
+	r.vocab_workspace_bytes = 0;
 	for (int k = 0; k < r.retired_count; ++k) hipFree(r.retired[k]);
 	r.retired_count = 0;
 	r.graphs_alive = 0;

@@ -396,3 +396,28 @@ def norm_join_bwd_sym(f, s, v, scale, h, s2, w, gh, gy, du, df, dv, dw, shared=T
     call("cnet_norm_join_bwd_sym", *f.p(), f.ld, s.ptr, *v.p(), 0 if shared else v.ld, scale, *_opt(h), _ptr(s2), *_opt(w)[:2], *_opt(gh), *_opt(gy),
          *_pair(du, mirror), du.ld, *_pair(df, mirror), df.ld, *_pair(dv, mirror_w), dv.ld, *(_pair(dw, mirror_w) if dw is not None else (None,) * 4),
          f.rows, f.cols, accumulate, accumulate_w)
+
+
+# ------------------------------------------------------------------------------------------------- losses of a vocabulary
+def distill_fwd(z, ids, probs, top, s, loss):
+    """loss of every row against `top` teacher entries (ids, probs: [rows][top])"""
+    call("cnet_distill_fwd", *z.p(), z.ld, ids.ptr, probs.ptr, top, s.ptr, loss.ptr, z.rows, z.cols)
+
+
+def distill_bwd_sym(z, s, ids, probs, top, dz, mirror=True):
+    call("cnet_distill_bwd_sym", *z.p(), z.ld, s.ptr, ids.ptr, probs.ptr, top, *_pair(dz, mirror), dz.ld, z.rows, z.cols)
+
+
+def distill_fwd_bwd_sym(z, ids, probs, top, s, loss, dz, mirror=True):
+    call("cnet_distill_fwd_bwd_sym", *z.p(), z.ld, ids.ptr, probs.ptr, top, s.ptr, loss.ptr, *_pair(dz, mirror), dz.ld, z.rows, z.cols)
+
+
+def vocab_head_fwd(x, w, labels, s, loss, argmax):
+    """Loss and most likely entry of x w^T without the logits; labels None: the loss of the most likely entry."""
+    call("cnet_vocab_head_fwd", *x.p(), x.ld, *w.p(), w.ld, _ptr(labels), s.ptr, _ptr(loss), _ptr(argmax), x.rows, x.cols, w.rows)
+
+
+def vocab_head_fwd_bwd_sym(x, w, labels, s, loss, argmax, dx, dw, accumulate_dx=0, accumulate_dw=0, mirror_dx=True, mirror_dw=True):
+    """vocab_head_fwd with the gradients at x and w; argmax may be None."""
+    call("cnet_vocab_head_fwd_bwd_sym", *x.p(), x.ld, *w.p(), w.ld, labels.ptr, s.ptr, loss.ptr, _ptr(argmax), *_pair(dx, mirror_dx), dx.ld,
+         accumulate_dx, *_pair(dw, mirror_dw), dw.ld, accumulate_dw, x.rows, x.cols, w.rows)

@@ -554,6 +554,43 @@ int cnet_norm_join_bwd_sym(const float *f_re, const float *f_im, int64_t ldf, co
                            float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im,
                            int rows, int cols, int accumulate, int accumulate_w);
 
+/* ---- The loss against a teacher's top entries, next to CrossEntropy and with its probabilities p_k = |z_k|^2 / s, s = clamped
+ *      sum |z|^2 (no counterpart upstream):
+ *        loss = sum_j q_j (log q_j - log max(p[id_j], 1e-15))        dz_k = conj(z_k) (Q / s - q(k) / max(|z_k|^2, 1e-15))
+ * with Q the sum of a row's weights q_j and q(k) the sum of those whose id is k (the same id may come more than once).
+ * ids[rows][top] int32, probs[rows][top] >= 0, 1 <= top <= CNET_DISTILL_MAX_TOP; they need not add up to 1.  An entry with a
+ * negative id is padding and left out of everything; a row of padding has loss 0 and gradient 0.  An id >= cols gives its row
+ * a NaN loss and counts in Q alone, as a label outside the row does in CrossEntropy.  One entry of weight 1 is CrossEntropy.
+ * The gradient is assigned; its dz* half may be NULL.  cnet_distill_fwd_bwd_sym gives the results of the other two in one
+ * call.  `loss` may point into memory from cnet_host_alloc. */
+#define CNET_DISTILL_MAX_TOP 1024
+int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top,
+                     float *s, float *loss, int rows, int cols);
+int cnet_distill_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, const float *s, const int32_t *ids, const float *probs, int top,
+                         float *dz_dz_re, float *dz_dz_im, float *dz_dzs_re, float *dz_dzs_im, int64_t lddz, int rows, int cols);
+int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top,
+                             float *s, float *loss, float *dz_dz_re, float *dz_dz_im, float *dz_dzs_re, float *dz_dzs_im, int64_t lddz,
+                             int rows, int cols);
+
+/* ---- A Linear to a large vocabulary with its CrossEntropy, without the logits: what cnet_clinear_fwd, cnet_cross_entropy_fwd,
+ *      cnet_cross_entropy_bwd_sym and cnet_clinear_bwd_sym compute together, where the [B x N] planes of the logits and of their
+ *      gradient (six of them in a training step) would be the largest thing in memory.  The library works on pieces of the
+ *      vocabulary in a buffer of its own.
+ * x[B][K], w[N][K]; z = x w^T; s = clamped sum |z|^2, loss = -log max(|z_label|^2 / s, 1e-15), argmax = first index of the largest
+ * |z_k|^2.
+ * labels[B]: a negative label leaves its row out (loss 0, no gradient); one >= N gives a NaN loss and acts as in
+ * cnet_cross_entropy_bwd (no entry is the label).  cnet_vocab_head_fwd: labels NULL takes each row's argmax for its label
+ * (scoring: loss is then -log of the largest probability); loss or argmax may be NULL, not both.
+ * cnet_vocab_head_fwd_bwd_sym: argmax may be NULL; dx and dw are the conjugate pairs of the gradients at x and w, summed over
+ * the rows in a fixed order, their dz* halves optional, each with its accumulate flag.  With B == 0 dw is zero (or left). */
+int cnet_vocab_head_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw,
+                        const int32_t *labels, float *s, float *loss, int32_t *argmax, int B, int K, int N);
+int cnet_vocab_head_fwd_bwd_sym(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw,
+                                const int32_t *labels, float *s, float *loss, int32_t *argmax,
+                                float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx, int accumulate_dx,
+                                float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw,
+                                int B, int K, int N);
+
 /* ---- Tuning overrides (environment variables).  None is needed for correct results or for the figures this library is
  *      measured with; they exist so that tests and sweeps can send a shape to every kernel that could take it.  Each is
  *      read ONCE per process, when the first launch that consults it is queued; results do not depend on them beyond
