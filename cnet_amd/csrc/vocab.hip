@@ -115,8 +115,9 @@ __global__ __launch_bounds__(TPB) void distill_kernel(const DistillArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ vocabulary head
-struct RowState {   // one entry per row of x, carried from piece to piece
-	double *sum;    // sum |z|^2 so far
+struct RowState {   // one entry per row of x, carried from launch to launch
+	double *sum;    // sum |z|^2 so far; below zero: still to be added up from `part`
+	double *part;   // [row][HEAD_SLABS]
 	float *best;    // largest |z|^2 so far, and its first index
 	int *index;
 	float *c_re, *c_im;  // conj(z_label) / m, the label's share of the gradient
@@ -156,6 +157,99 @@ __global__ __launch_bounds__(TPB) void head_piece_kernel(const float *__restrict
 	}
 }
 
+// ---- The loss through the Gram matrix of w.  The loss knows the logits z = x w^T through sum |z|^2 alone, a quadratic form of x:
+// with T = w^H w (K x K), y = conj(x) T is what the logits' gradient hands back to x (before its division by S and without the
+// label's term) and S = sum_j y_j x_j.  So neither S nor either gradient needs the logits: N K^2 + B K^2 products stand for
+// B N K.  What it costs is accuracy where x lies in directions that w hardly has: the terms of S cancel.  With D = sum |x_i|^2 T_ii
+// (the sum's size if the columns of w were orthogonal), a row with S < D / 64 is computed again from w itself, so that at most
+// six of the 24 bits are lost to the cancellation.
+constexpr float GRAM_LEAST = 1.0f / 64;
+constexpr int HEAD_SLABS = 32;      // parts of the vocabulary that such a row's logits are dealt out in
+constexpr int HEAD_ROWS = 64;       // rows whose marks one workgroup looks at
+constexpr double TO_DO = -1.0;
+
+// One wavefront per row: S, or the mark that asks for the direct sum (also for a NaN or an overflow on the way)
+__global__ __launch_bounds__(TPB) void head_gram_norm_kernel(const float *__restrict__ xr, const float *__restrict__ xi, long ldx,
+		const float *__restrict__ yr, const float *__restrict__ yi, long ldy, const float *__restrict__ t_re, long ldt, int B, int K, RowState st) {
+	const int lane = threadIdx.x & 63;
+	const long row = (long) blockIdx.x * WAVES + (threadIdx.x >> 6);
+	if (row >= B) return;
+	double sum = 0.0;
+	float diag = 0.f;
+	for (int c = lane; c < K; c += 64) {
+		const float a = xr[row * ldx + c], b = xi[row * ldx + c];
+		sum += (double) a * yr[row * ldy + c] - (double) b * yi[row * ldy + c];
+		diag += (a * a + b * b) * t_re[c * ldt + c];
+	}
+	sum = wave_reduce(sum, SumD());
+	diag = wave_reduce(diag, SumF());
+	if (lane == 0) st.sum[row] = sum >= (double) (GRAM_LEAST * diag) && diag < 3.0e38f ? sum : TO_DO;
+}
+
+// The rows that head_gram_norm_kernel has marked, from w: part[row][slab] = sum |z|^2 over the slab of the vocabulary blockIdx.y.
+// The workgroup lists the marked ones of its HEAD_ROWS rows (in order; usually there are none) and takes them four at a time;
+// a wavefront forms four logits of four rows together, its lanes sharing K.
+__global__ __launch_bounds__(TPB) void head_direct_norm_kernel(const float *__restrict__ xr, const float *__restrict__ xi, long ldx,
+		const float *__restrict__ wr, const float *__restrict__ wi, long ldw, int B, int K, int N, RowState st) {
+	__shared__ int list[HEAD_ROWS];
+	__shared__ double lds_d[WAVES];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+	const int mine = blockIdx.x * HEAD_ROWS + lane;
+	const bool marked = mine < B && st.sum[mine] < 0.0;
+	const unsigned long long set = __ballot(marked);
+	const int count = __popcll(set);
+	if (!count) return;
+	if (wave == 0 && marked) list[__popcll(set & ((1ull << lane) - 1))] = mine;
+	__syncthreads();
+	const int per = (N + HEAD_SLABS - 1) / HEAD_SLABS, k0 = min(N, (int) blockIdx.y * per), k1 = min(N, k0 + per);
+	for (int first = 0; first < count; first += 4) {
+		long xo[4];
+#pragma unroll
+		for (int r = 0; r < 4; ++r) xo[r] = (long) list[min(first + r, count - 1)] * ldx;
+		double sum[4] = {0.0, 0.0, 0.0, 0.0};
+		for (int k = k0 + 4 * wave; k < k1; k += 4 * WAVES) {
+			float re[4][4] = {}, im[4][4] = {};
+			for (int c = lane; c < K; c += 64) {
+				float a[4], b[4];
+#pragma unroll
+				for (int r = 0; r < 4; ++r) {
+					a[r] = xr[xo[r] + c];
+					b[r] = xi[xo[r] + c];
+				}
+#pragma unroll
+				for (int q = 0; q < 4; ++q) {
+					const long o = (long) min(k + q, N - 1) * ldw + c;
+					const float d = wr[o], e = wi[o];
+#pragma unroll
+					for (int r = 0; r < 4; ++r) {
+						re[r][q] = fmaf(a[r], d, fmaf(-b[r], e, re[r][q]));
+						im[r][q] = fmaf(a[r], e, fmaf(b[r], d, im[r][q]));
+					}
+				}
+			}
+#pragma unroll
+			for (int r = 0; r < 4; ++r)
+#pragma unroll
+				for (int q = 0; q < 4; ++q) {
+					const float u = wave_reduce(re[r][q], SumF()), v = wave_reduce(im[r][q], SumF());
+					if (k + q < k1) sum[r] += (double) u * u + (double) v * v;
+				}
+		}
+#pragma unroll
+		for (int r = 0; r < 4; ++r) {
+			// (every lane of a wavefront holds the same sum: one lane of each speaks for it)
+			if (lane == 0) lds_d[wave] = sum[r];
+			__syncthreads();
+			if (t == 0 && first + r < count) {
+				double total = lds_d[0];
+				for (int w = 1; w < WAVES; ++w) total += lds_d[w];
+				st.part[(long) list[first + r] * HEAD_SLABS + blockIdx.y] = total;
+			}
+			__syncthreads();
+		}
+	}
+}
+
 struct HeadArgs {
 	const float *x_re, *x_im, *w_re, *w_im;
 	long ldx, ldw;
@@ -178,8 +272,13 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 	__shared__ double lds_d[WAVES];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.x;
-	const float S = clamped((float) st.sum[row]);
-	int best = st.index[row];
+	double sum = st.sum[row];
+	if (sum < 0.0) {
+		sum = 0.0;
+		for (int k = 0; k < HEAD_SLABS; ++k) sum += st.part[row * HEAD_SLABS + k];
+	}
+	const float S = clamped((float) sum);
+	int best = a.labels && !a.argmax ? 0 : st.index[row];
 	if (best < 0 || best >= a.N) best = 0;  // a row of NaN has no largest entry
 	const int label = a.labels ? a.labels[row] : best;
 	const bool known = label >= 0 && label < a.N;
@@ -222,52 +321,160 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 }
 
 struct ScatterArgs {
-	const int *labels;
+	const int *row_of, *label_of;  // the rows in order of their labels
 	const float *c_re, *c_im, *x_re, *x_im;
 	long ldx;
 	float *dw_re, *dw_im, *dws_re, *dws_im;
 	long lddw;
+	float *part;  // [chunk][began before, begins here][re, im][ldk]
+	long ldk;
 	int B, K, N;
 };
 
-// dw[label[r]] -= c_r x_r for every row r, rows of the same label in order.  A workgroup owns SPAN rows of the vocabulary: it
-// walks the labels in steps of TPB, and each of its threads owns columns.
-constexpr int SPAN = 64;
-__global__ __launch_bounds__(TPB) void head_scatter_kernel(const ScatterArgs a) {
-	__shared__ int found[TPB], count[WAVES];
-	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-	const int lo = blockIdx.x * SPAN, hi = min(a.N, lo + SPAN);
-	for (int r0 = 0; r0 < a.B; r0 += TPB) {
-		const int r = r0 + t;
-		const int label = r < a.B ? a.labels[r] : -1;
-		const bool mine = label >= lo && label < hi;
-		const unsigned long long set = __ballot(mine);
-		if (lane == 0) count[wave] = __popcll(set);
-		__syncthreads();
-		int at = __popcll(set & ((1ull << lane) - 1)), total = 0;
-		for (int w = 0; w < WAVES; ++w) {
-			if (w < wave) at += count[w];
-			total += count[w];
-		}
-		if (mine) found[at] = r;
-		__syncthreads();
-		for (int k = 0; k < total; ++k) {
-			const long row = found[k];
-			const long dst = (long) a.labels[row] * a.lddw;
-			const float c_re = a.c_re[row], c_im = a.c_im[row];
-			for (int c = t; c < a.K; c += TPB) {
-				const float x_r = a.x_re[row * a.ldx + c], x_i = a.x_im[row * a.ldx + c];
-				const float d_r = c_re * x_r - c_im * x_i, d_i = c_re * x_i + c_im * x_r;
-				a.dw_re[dst + c] -= d_r;
-				a.dw_im[dst + c] -= d_i;
-				if (a.dws_re) {
-					a.dws_re[dst + c] -= d_r;
-					a.dws_im[dst + c] += d_i;
+// ---- The label's term of the weights' gradient: dw[label[r]] -= c_r x_r for every row r.  Labels of a text repeat (the most
+// frequent token of a batch of 8192 names hundreds of rows), so the rows are put in order of their labels first and then worked
+// off in chunks of equal length, whatever the labels.  The order is the stable one, so a label's rows are added in order.
+constexpr int ORDER_ROWS = 8192;  // rows ordered together (their keys fill 64 KB of LDS); longer batches go block by block
+constexpr int CHUNK = 16;         // ordered rows of one workgroup
+
+// Workgroup b sorts rows [b ORDER_ROWS, ..) by (label, row), rows without a label of the vocabulary last (a bitonic network in
+// LDS: 8192 rows take 91 exchanges of four pairs a thread).  row_of = -1 and label_of = N where there is no label.
+__global__ __launch_bounds__(1024) void head_order_kernel(const int *__restrict__ labels, int B, int N, int n2, int *__restrict__ row_of,
+		int *__restrict__ label_of) {
+	extern __shared__ unsigned long long keys[];
+	const int first = blockIdx.x * ORDER_ROWS, n = min(ORDER_ROWS, B - first);
+	for (int i = threadIdx.x; i < n2; i += 1024) {
+		const int label = i < n ? labels[first + i] : -1;
+		keys[i] = ((unsigned long long) (unsigned) (label >= 0 && label < N ? label : N) << 32) | (unsigned) i;
+	}
+	for (int k = 2; k <= n2; k *= 2)
+		for (int j = k / 2; j > 0; j /= 2) {
+			__syncthreads();
+			for (int h = threadIdx.x; h < n2 / 2; h += 1024) {
+				const int lo = 2 * h - (h & (j - 1)), hi = lo + j;
+				const unsigned long long u = keys[lo], v = keys[hi];
+				if ((u > v) == ((lo & k) == 0)) {
+					keys[lo] = v;
+					keys[hi] = u;
 				}
 			}
 		}
-		__syncthreads();
+	__syncthreads();
+	for (int i = threadIdx.x; i < n; i += 1024) {
+		const int label = (int) (keys[i] >> 32);
+		label_of[first + i] = label;
+		row_of[first + i] = label < N ? first + (int) (unsigned) keys[i] : -1;
 	}
+}
+
+template <int V>
+__device__ __forceinline__ void load_v(float *v, const float *p) {
+	if (V == 4) {
+		const float4 t = *reinterpret_cast<const float4 *>(p);
+		v[0] = t.x;
+		v[1 % V] = t.y;
+		v[2 % V] = t.z;
+		v[3 % V] = t.w;
+	} else {
+		v[0] = p[0];
+	}
+}
+template <int V>
+__device__ __forceinline__ void store_v(float *p, const float *v) {
+	if (V == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
+	else p[0] = v[0];
+}
+
+// subtracts V columns of one label's sum from its row of the gradient
+template <int V>
+__device__ __forceinline__ void subtract_label(const ScatterArgs &a, int label, int c, const float *re, const float *im) {
+	const long o = (long) label * a.lddw + c;
+	float v[V];
+	auto apply = [&](float *p, const float *d, float sign) {
+		load_v<V>(v, p + o);
+#pragma unroll
+		for (int k = 0; k < V; ++k) v[k] -= sign * d[k];
+		store_v<V>(p + o, v);
+	};
+	apply(a.dw_re, re, 1.f);
+	apply(a.dw_im, im, 1.f);
+	if (a.dws_re) {
+		apply(a.dws_re, re, 1.f);
+		apply(a.dws_im, im, -1.f);
+	}
+}
+
+// Workgroup (x, y): the ordered rows [CHUNK x, CHUNK x + CHUNK) of the block that starts at `first`, V columns per thread.  A run of
+// one label that lies inside the chunk is subtracted at once; the part of a run that reaches over the chunk's ends goes to
+// part[x][0] (it began before) or part[x][1] (it begins here).
+template <int V>
+__global__ __launch_bounds__(TPB) void head_label_kernel(const ScatterArgs a, int first) {
+	const int c = (blockIdx.y * TPB + threadIdx.x) * V;
+	const int p0 = first + blockIdx.x * CHUNK, block_end = min(a.B, first + ORDER_ROWS), p1 = min(block_end, p0 + CHUNK);
+	const int before = p0 > first ? a.label_of[p0 - 1] : -1, after = p1 < block_end ? a.label_of[p1] : -1;
+	if (c >= a.K) return;
+	float re[V], im[V];
+	int label = -1, begin = p0;
+	for (int p = p0; p < p1; ++p) {
+		const int l = a.label_of[p];
+		if (l >= a.N) break;  // rows without a label are last
+		const int r = a.row_of[p];
+		if (l != label) {
+			label = l;
+			begin = p;
+#pragma unroll
+			for (int k = 0; k < V; ++k) re[k] = im[k] = 0.f;
+		}
+		const float c_re = a.c_re[r], c_im = a.c_im[r];
+		float x_r[V], x_i[V];
+		load_v<V>(x_r, a.x_re + (long) r * a.ldx + c);
+		load_v<V>(x_i, a.x_im + (long) r * a.ldx + c);
+#pragma unroll
+		for (int k = 0; k < V; ++k) {
+			re[k] += c_re * x_r[k] - c_im * x_i[k];
+			im[k] += c_re * x_i[k] + c_im * x_r[k];
+		}
+		const int next = p + 1 < p1 ? a.label_of[p + 1] : after;
+		if (next == label && p + 1 < p1) continue;
+		const bool began = begin == p0 && before == label, goes_on = next == label;
+		if (!began && !goes_on) {
+			subtract_label<V>(a, label, c, re, im);
+		} else {
+			float *part = a.part + ((long) blockIdx.x * 2 + (began ? 0 : 1)) * 2 * a.ldk + c;
+			store_v<V>(part, re);
+			store_v<V>(part + a.ldk, im);
+		}
+	}
+}
+
+// The runs that reach over chunks: the chunk that such a run begins in adds up its parts in order
+template <int V>
+__global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs a, int first) {
+	const int c = (blockIdx.y * TPB + threadIdx.x) * V;
+	const int p0 = first + blockIdx.x * CHUNK, block_end = min(a.B, first + ORDER_ROWS), p1 = p0 + CHUNK;
+	if (p1 >= block_end || c >= a.K) return;
+	const int label = a.label_of[p1 - 1];
+	if (label >= a.N || a.label_of[p1] != label) return;            // nothing reaches over this chunk's end
+	if (p0 > first && a.label_of[p0 - 1] == label) return;         // it began earlier
+	int chunks = 1;                                                 // further chunks that hold a part of it
+	while (p1 + chunks * CHUNK < block_end && a.label_of[p1 + chunks * CHUNK] == label) ++chunks;
+	const float *part = a.part + ((long) blockIdx.x * 2 + 1) * 2 * a.ldk + c;
+	float re[V], im[V];
+	load_v<V>(re, part);
+	load_v<V>(im, part + a.ldk);
+#pragma unroll 4
+	for (int k = 1; k <= chunks; ++k) {
+		float x[V], y[V];
+		const float *more = part + (k * 2 - 1) * 2 * a.ldk;
+		load_v<V>(x, more);
+		load_v<V>(y, more + a.ldk);
+#pragma unroll
+		for (int q = 0; q < V; ++q) {
+			re[q] += x[q];
+			im[q] += y[q];
+		}
+	}
+	subtract_label<V>(a, label, c, re, im);
 }
 
 // the gradient of no rows at all
@@ -289,88 +496,189 @@ static int distill(const DistillArgs &a) {
 // what the calls of the head keep between their launches, carved out of one buffer of the library
 struct HeadBuffers {
 	RowState st;
-	float *piece, *y, *xs;  // planes re, im
-	int piece_cols;         // columns of one piece, also its leading dimension
-	long ldk;               // leading dimension of y and xs
+	float *piece, *y, *xs, *gram;  // planes re, im
+	int *row_of, *label_of;
+	float *label_part;
+	int piece_cols;                // columns of one piece, also its leading dimension
+	long ldk;                      // leading dimension of y, xs and gram
+};
+
+struct HeadPlan {
+	bool bwd, gram, pieces;
+	int piece_cols;
 };
 
 // A piece of logits (two planes of B rows) is as wide as the memory-side cache holds: the pass over it, and the product that
 // reads it, then find it there.
-constexpr size_t PIECE_BYTES = (size_t) 192 << 20;
+static long piece_bytes() {
+	static const long mb = [] {
+		const char *e = getenv("CNET_HEAD_PIECE_MB");  // tuning override
+		return e && atol(e) > 0 ? atol(e) : 192L;
+	}();
+	return mb << 20;
+}
 
-static int head_buffers(int B, int K, int N, bool bwd, HeadBuffers &b) {
+// Which way the call goes, by the matrix products it then runs (complex multiplications; they are nearly all of its time).
+//   through the Gram matrix: T over N, y over K, and for the weights P = x^H (x / S) over B and w P over K
+//   through the logits: they, y, and for the weights x^T conj(z), with the logits formed again when one piece does not hold them
+// The argmax needs the logits either way.
+static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
+	static const int forced = [] {
+		const char *e = getenv("CNET_HEAD_GRAM");  // tuning override: 0 / 1 never / always through the Gram matrix
+		return e ? atoi(e) : -1;
+	}();
+	HeadPlan p;
+	p.bwd = bwd;
 	const long whole = ((long) N + 63) / 64 * 64;
-	b.piece_cols = (int) std::min(whole, std::max(64L, (long) (PIECE_BYTES / (8 * (size_t) B)) / 64 * 64));
+	p.piece_cols = (int) std::min(whole, std::max(64L, piece_bytes() / (8 * (long) B) / 64 * 64));
+	const double b = B, k = K, n = N;
+	const double logits = b * n * k * (bwd ? (N <= p.piece_cols ? 3 : 4) : 1);
+	const double gram = (bwd ? 2 : 1) * (n + b) * k * k + (argmax ? b * n * k : 0);
+	p.gram = (bwd || !argmax) && (forced >= 0 ? forced != 0 : gram < logits);
+	p.pieces = argmax || !p.gram;
+	return p;
+}
+
+static int head_buffers(int B, int K, const HeadPlan &plan, HeadBuffers &b) {
+	b.piece_cols = plan.piece_cols;
 	b.ldk = ((long) K + 3) / 4 * 4;
 	const size_t rows = ((size_t) B + 63) / 64 * 64;
-	const size_t piece = 2 * (size_t) B * b.piece_cols, wide = bwd ? 2 * (size_t) B * b.ldk : 0;
-	float *p = (float *) vocab_workspace((7 * rows + piece + 2 * wide) * sizeof(float));
+	const size_t piece = plan.pieces ? 2 * (size_t) B * b.piece_cols : 0;
+	const size_t wide = plan.bwd || plan.gram ? 2 * (size_t) B * b.ldk : 0, square = plan.gram ? 2 * (size_t) K * b.ldk : 0;
+	const size_t part = plan.gram && !plan.pieces ? 2 * HEAD_SLABS * rows : 0;
+	const size_t order = plan.bwd ? rows : 0, label_part = plan.bwd ? (size_t) (std::min(B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
+	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part) * sizeof(float));
 	if (!p) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
-	b.st.sum = (double *) p;
-	b.st.best = p + 2 * rows;
-	b.st.index = (int *) (p + 3 * rows);
-	b.st.c_re = p + 4 * rows;
-	b.st.c_im = p + 5 * rows;
-	b.piece = p + 7 * rows;
-	b.y = b.piece + piece;
-	b.xs = b.y + wide;
+	auto take = [&](size_t floats) {
+		float *q = p;
+		p += floats;
+		return q;
+	};
+	b.st.sum = (double *) take(2 * rows);
+	b.st.part = (double *) take(part);
+	b.st.best = take(rows);
+	b.st.index = (int *) take(rows);
+	b.st.c_re = take(rows);
+	b.st.c_im = take(rows);
+	b.piece = take(piece);
+	b.y = take(wide);
+	b.xs = take(wide);
+	b.gram = take(square);
+	b.label_part = take(label_part);
+	b.row_of = (int *) take(order);
+	b.label_of = (int *) take(order);
+	return CNET_OK;
+}
+
+// C = conj(A) B, A row-major or k-major, B k-major
+static int conj_product(int a_kmajor, int M, int N, int K, const float *a_re, const float *a_im, long lda, const float *b_re, const float *b_im, long ldb,
+		float *c_re, float *c_im, long ldc, int accumulate) {
+	return cnet_cgemm_batched(a_kmajor, 1, 1, 0, M, N, K, a_re, a_im, lda, 0, b_re, b_im, ldb, 0, c_re, c_im, ldc, 0, 1, accumulate);
+}
+
+// a gradient's pair of planes from C = conj(A) B: with the dz* half wanted, A conj(B) is formed for that half and mirrored into
+// the other
+static int conj_product_pair(bool a_kmajor, int M, int N, int K, const float *a_re, const float *a_im, long lda, const float *b_re, const float *b_im,
+		long ldb, float *c_re, float *c_im, float *cs_re, float *cs_im, long ldc, int accumulate) {
+	if (!cs_re) return conj_product(a_kmajor, M, N, K, a_re, a_im, lda, b_re, b_im, ldb, c_re, c_im, ldc, accumulate);
+	const float *ar[2] = {a_re, a_re}, *ai[2] = {a_im, a_im}, *br[2] = {b_re, b_re}, *bi[2] = {b_im, b_im};
+	float *cr[2] = {cs_re, c_re}, *ci[2] = {cs_im, c_im};
+	const bool cj[2] = {true, true};
+	return cgemm_pair(a_kmajor, true, 1, M, N, K, ar, ai, lda, br, bi, ldb, cj, cr, ci, ldc, accumulate, 0, 1);
+}
+
+static int head_labels(const HeadArgs &a, const HeadBuffers &b, int B, float *dw_re, float *dw_im, float *dws_re, float *dws_im, long lddw) {
+	int n2 = 2;
+	while (n2 < std::min(B, ORDER_ROWS)) n2 *= 2;
+	hipLaunchKernelGGL(head_order_kernel, dim3((unsigned) ((B + ORDER_ROWS - 1) / ORDER_ROWS)), dim3(1024), n2 * sizeof(unsigned long long), rt().stream,
+			a.labels, B, a.N, n2, b.row_of, b.label_of);
+	CNET_LAUNCH_CHECK();
+	const ScatterArgs sc = {b.row_of, b.label_of, b.st.c_re, b.st.c_im, a.x_re, a.x_im, a.ldx, dw_re, dw_im, dws_re, dws_im, lddw, b.label_part, b.ldk,
+			B, a.K, a.N};
+	const bool vec = a.K % 4 == 0 && a.ldx % 4 == 0 && lddw % 4 == 0 && aligned16(a.x_re) && aligned16(a.x_im) && aligned16(dw_re) && aligned16(dw_im) &&
+			aligned16(dws_re) && aligned16(dws_im);
+	const int per_group = TPB * (vec ? 4 : 1);
+	for (int first = 0; first < B; first += ORDER_ROWS) {
+		const dim3 grid((unsigned) ((std::min(B - first, ORDER_ROWS) + CHUNK - 1) / CHUNK), (unsigned) ((a.K + per_group - 1) / per_group));
+		if (vec) {
+			hipLaunchKernelGGL(head_label_kernel<4>, grid, dim3(TPB), 0, rt().stream, sc, first);
+			hipLaunchKernelGGL(head_label_join_kernel<4>, grid, dim3(TPB), 0, rt().stream, sc, first);
+		} else {
+			hipLaunchKernelGGL(head_label_kernel<1>, grid, dim3(TPB), 0, rt().stream, sc, first);
+			hipLaunchKernelGGL(head_label_join_kernel<1>, grid, dim3(TPB), 0, rt().stream, sc, first);
+		}
+		CNET_LAUNCH_CHECK();
+	}
 	return CNET_OK;
 }
 
 static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float *dws_re, float *dws_im, long lddw, int accumulate_dw, bool bwd) {
 	HeadArgs a = proto;
 	const int K = a.K, N = a.N;
+	const HeadPlan plan = head_plan(B, K, N, bwd, a.argmax || !a.labels);
 	HeadBuffers b;
-	int rc = head_buffers(B, K, N, bwd, b);
+	int rc = head_buffers(B, K, plan, b);
 	if (rc) return rc;
-	float *z_re = b.piece, *z_im = b.piece + (size_t) B * b.piece_cols;
-	float *y_re = b.y, *y_im = b.y + (size_t) B * b.ldk;
+	const int np = b.piece_cols;
+	const long ldk = b.ldk;
+	float *z_re = b.piece, *z_im = b.piece + (size_t) B * np;
+	float *y_re = b.y, *y_im = b.y + (size_t) B * ldk;
+	float *g_re = b.gram, *g_im = b.gram + (size_t) K * ldk;
 	a.y_re = y_re;
 	a.y_im = y_im;
 	a.xs_re = b.xs;
-	a.xs_im = b.xs + (size_t) B * b.ldk;
-	a.ldy = b.ldk;
-	const int np = b.piece_cols;
+	a.xs_im = b.xs + (size_t) B * ldk;
+	a.ldy = ldk;
 	auto logits = [&](int n0, int n) {
 		return cnet_clinear_fwd(a.x_re, a.x_im, a.ldx, a.w_re + (size_t) n0 * a.ldw, a.w_im + (size_t) n0 * a.ldw, a.ldw, z_re, z_im, np, B, K, n, 0);
 	};
-	for (int n0 = 0; n0 < N; n0 += np) {
+	for (int n0 = 0; plan.pieces && n0 < N; n0 += np) {
 		const int n = std::min(np, N - n0);
 		rc = logits(n0, n);
 		if (rc) return rc;
 		hipLaunchKernelGGL(head_piece_kernel, dim3((unsigned) B), dim3(TPB), 0, rt().stream, z_re, z_im, (long) np, n, n0, b.st);
 		CNET_LAUNCH_CHECK();
-		if (bwd) {  // y += conj(z) w: linear in z, so the division by S can wait until S is whole
-			rc = cnet_cgemm_batched(0, 1, 1, 0, B, K, n, z_re, z_im, np, 0, a.w_re + (size_t) n0 * a.ldw, a.w_im + (size_t) n0 * a.ldw, a.ldw, 0, y_re,
-					y_im, b.ldk, 0, 1, n0 > 0);
+		if (bwd && !plan.gram) {  // y += conj(z) w: linear in z, so the division by S can wait until S is whole
+			rc = conj_product(0, B, K, n, z_re, z_im, np, a.w_re + (size_t) n0 * a.ldw, a.w_im + (size_t) n0 * a.ldw, a.ldw, y_re, y_im, ldk, n0 > 0);
 			if (rc) return rc;
+		}
+	}
+	if (plan.gram) {
+		rc = conj_product(1, K, K, N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, 0);
+		if (rc) return rc;
+		rc = conj_product(0, B, K, K, a.x_re, a.x_im, a.ldx, g_re, g_im, ldk, y_re, y_im, ldk, 0);
+		if (rc) return rc;
+		if (!plan.pieces) {
+			hipLaunchKernelGGL(head_gram_norm_kernel, dim3((unsigned) ((B + WAVES - 1) / WAVES)), dim3(TPB), 0, rt().stream, a.x_re, a.x_im, a.ldx, y_re,
+					y_im, ldk, g_re, ldk, B, K, b.st);
+			CNET_LAUNCH_CHECK();
+			hipLaunchKernelGGL(head_direct_norm_kernel, dim3((unsigned) ((B + HEAD_ROWS - 1) / HEAD_ROWS), HEAD_SLABS), dim3(TPB), 0, rt().stream,
+					a.x_re, a.x_im, a.ldx, a.w_re, a.w_im, a.ldw, B, K, N, b.st);
+			CNET_LAUNCH_CHECK();
 		}
 	}
 	if (bwd) hipLaunchKernelGGL(head_finish_kernel<true>, dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, b.st);
 	else hipLaunchKernelGGL(head_finish_kernel<false>, dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, b.st);
 	CNET_LAUNCH_CHECK();
 	if (!bwd) return CNET_OK;
-	for (int n0 = 0; n0 < N; n0 += np) {
+	if (plan.gram) {
+		rc = conj_product(1, K, K, B, a.x_re, a.x_im, a.ldx, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk, 0);
+		if (rc) return rc;
+		rc = conj_product_pair(false, N, K, K, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw);
+		if (rc) return rc;
+	}
+	for (int n0 = 0; !plan.gram && n0 < N; n0 += np) {
 		const int n = std::min(np, N - n0);
 		if (N > np) {
 			rc = logits(n0, n);
 			if (rc) return rc;
 		}
 		const size_t o = (size_t) n0 * lddw;
-		if (dws_re) {  // dz* = z^T conj(x / S) is computed, dz written as its conjugate
-			const float *ar[2] = {z_re, z_re}, *ai[2] = {z_im, z_im}, *br[2] = {a.xs_re, a.xs_re}, *bi[2] = {a.xs_im, a.xs_im};
-			float *cr[2] = {dws_re + o, dw_re + o}, *ci[2] = {dws_im + o, dw_im + o};
-			const bool cj[2] = {true, true};
-			rc = cgemm_pair(true, true, 1, n, K, B, ar, ai, np, br, bi, b.ldk, cj, cr, ci, lddw, accumulate_dw, 0, 1);
-		} else {
-			rc = cnet_cgemm_batched(1, 1, 1, 0, n, K, B, z_re, z_im, np, 0, a.xs_re, a.xs_im, b.ldk, 0, dw_re + o, dw_im + o, lddw, 0, 1, accumulate_dw);
-		}
+		rc = conj_product_pair(true, n, K, B, z_re, z_im, np, a.xs_re, a.xs_im, ldk, dw_re + o, dw_im + o, dws_re ? dws_re + o : nullptr,
+				dws_re ? dws_im + o : nullptr, lddw, accumulate_dw);
 		if (rc) return rc;
 	}
-	const ScatterArgs sc = {a.labels, b.st.c_re, b.st.c_im, a.x_re, a.x_im, a.ldx, dw_re, dw_im, dws_re, dws_im, lddw, B, K, N};
-	hipLaunchKernelGGL(head_scatter_kernel, dim3((unsigned) ((N + SPAN - 1) / SPAN)), dim3(TPB), 0, rt().stream, sc);
-	CNET_LAUNCH_CHECK();
-	return CNET_OK;
+	return head_labels(a, b, B, dw_re, dw_im, dws_re, dws_im, lddw);
 }
 
 extern "C" {

@@ -247,7 +247,7 @@ def head_check(B, K, N, pad=0, off=0, argmax=True, data=None):
 # B, K, N, padding of the leading dimensions, offset of the first element
 HEAD = [(1, 1, 1, 0, 0), (3, 5, 7, 0, 0), (1, 64, 512, 0, 0), (2, 1024, 300, 0, 0), (16, 128, 1001, 0, 0), (17, 33, 130, 2, 1), (48, 256, 2000, 4, 0),
         (65, 100, 1000, 0, 0), (96, 64, 512, 0, 0), (513, 40, 300, 0, 0), (300, 96, 700, 0, 4), (700, 333, 1100, 3, 0), (1500, 64, 1024, 0, 0),
-        (130, 512, 4099, 0, 0), (2100, 17, 19, 0, 0)]
+        (130, 512, 4099, 0, 0), (2100, 17, 19, 0, 0), (9000, 8, 40, 0, 0), (8200, 20, 3, 1, 0), (40, 1300, 64, 0, 0)]
 
 
 @pytest.mark.parametrize("B,K,N,pad,off", HEAD)
