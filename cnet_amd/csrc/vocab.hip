@@ -31,6 +31,24 @@ __device__ __forceinline__ double clamped(double v) { return v <= (double) LEAST
 
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
 
+template <int V>
+__device__ __forceinline__ void load_v(float *v, const float *p) {
+	if (V == 4) {
+		const float4 t = *reinterpret_cast<const float4 *>(p);
+		v[0] = t.x;
+		v[1 % V] = t.y;
+		v[2 % V] = t.z;
+		v[3 % V] = t.w;
+	} else {
+		v[0] = p[0];
+	}
+}
+template <int V>
+__device__ __forceinline__ void store_v(float *p, const float *v) {
+	if (V == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
+	else p[0] = v[0];
+}
+
 // ------------------------------------------------------------------------------------------------ distillation
 struct DistillArgs {
 	const float *z_re, *z_im;
@@ -265,8 +283,40 @@ struct HeadArgs {
 	int K, N;
 };
 
-// One workgroup per row: S, the label's logit (its products summed in double: the gradient goes with its inverse), loss, and the
-// gradient at x: y / S minus the label's row of w times conj(z_label) / m.
+// what a row's label makes of it
+struct LabelTerm {
+	int label;          // -1: none in the vocabulary
+	float loss, inv;    // inv: 1 / S, 0 for a row that is left out
+	float c_re, c_im;   // conj(z_label) / m
+};
+
+// The label's logit is formed from x and w with its products summed in double: the gradient goes with its inverse, and an unlikely
+// label has one near zero, of which a sum in single precision leaves few digits.  W wavefronts.
+template <int W>
+__device__ __forceinline__ LabelTerm label_term(const HeadArgs &a, long row, int label, float S, double *lds, int t, int lane, int wave) {
+	const bool known = label >= 0 && label < a.N;
+	double re = 0.0, im = 0.0;
+	if (known) {
+		const float *xr = a.x_re + row * a.ldx, *xi = a.x_im + row * a.ldx;
+		const float *wr = a.w_re + label * a.ldw, *wi = a.w_im + label * a.ldw;
+		for (int c = t; c < a.K; c += 64 * W) {
+			re += (double) xr[c] * wr[c] - (double) xi[c] * wi[c];
+			im += (double) xr[c] * wi[c] + (double) xi[c] * wr[c];
+		}
+	}
+	re = group_reduce<double, W>(re, SumD(), lds, 0, wave, lane);
+	im = group_reduce<double, W>(im, SumD(), lds, 0, wave, lane);
+	const double power = re * re + im * im, m = clamped(power);
+	LabelTerm l;
+	l.label = known ? label : -1;
+	l.loss = label < 0 ? 0.f : known ? -logf((float) clamped(power / (double) S)) : __builtin_nanf("");
+	l.inv = label < 0 ? 0.f : 1.0f / S;
+	l.c_re = known ? (float) (re / m) : 0.f;
+	l.c_im = known ? (float) (-im / m) : 0.f;
+	return l;
+}
+
+// One workgroup per row: S, the label's logit, loss, and the gradient at x: y / S minus the label's row of w times conj(z_label) / m.
 template <bool BWD>
 __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st) {
 	__shared__ double lds_d[WAVES];
@@ -280,43 +330,84 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 	const float S = clamped((float) sum);
 	int best = a.labels && !a.argmax ? 0 : st.index[row];
 	if (best < 0 || best >= a.N) best = 0;  // a row of NaN has no largest entry
-	const int label = a.labels ? a.labels[row] : best;
-	const bool known = label >= 0 && label < a.N;
-	const float *xr = a.x_re + row * a.ldx, *xi = a.x_im + row * a.ldx;
-	const float *wr = a.w_re + (known ? label : 0) * a.ldw, *wi = a.w_im + (known ? label : 0) * a.ldw;
-	double re = 0.0, im = 0.0;
-	if (known) {
-		for (int c = t; c < a.K; c += TPB) {
-			re += (double) xr[c] * wr[c] - (double) xi[c] * wi[c];
-			im += (double) xr[c] * wi[c] + (double) xi[c] * wr[c];
-		}
-	}
-	re = group_reduce<double, WAVES>(re, SumD(), lds_d, 0, wave, lane);
-	im = group_reduce<double, WAVES>(im, SumD(), lds_d, 0, wave, lane);
-	const double power = re * re + im * im, m = clamped(power);
+	const LabelTerm l = label_term<WAVES>(a, row, a.labels ? a.labels[row] : best, S, lds_d, t, lane, wave);
 	if (t == 0) {
 		a.s[row] = S;
-		if (a.loss) a.loss[row] = label < 0 ? 0.f : known ? -logf((float) clamped(power / (double) S)) : __builtin_nanf("");
+		if (a.loss) a.loss[row] = l.loss;
 		if (a.argmax) a.argmax[row] = best;
 	}
 	if (!BWD) return;
-	const float inv = label < 0 ? 0.f : 1.0f / S;
-	const float c_re = known ? (float) (re / m) : 0.f, c_im = known ? (float) (-im / m) : 0.f;
 	if (t == 0) {
-		st.c_re[row] = c_re;
-		st.c_im[row] = c_im;
+		st.c_re[row] = l.c_re;
+		st.c_im[row] = l.c_im;
 	}
+	const float *xr = a.x_re + row * a.ldx, *xi = a.x_im + row * a.ldx;
+	const long label_row = (l.label < 0 ? 0 : l.label) * a.ldw;
 	for (int c = t; c < a.K; c += TPB) {
 		const long o = row * a.ldy + c, d = row * a.lddx + c;
-		const float g_r = a.y_re[o] * inv - (c_re * wr[c] - c_im * wi[c]), g_i = a.y_im[o] * inv - (c_re * wi[c] + c_im * wr[c]);
+		const float w_r = a.w_re[label_row + c], w_i = a.w_im[label_row + c];
+		const float g_r = a.y_re[o] * l.inv - (l.c_re * w_r - l.c_im * w_i), g_i = a.y_im[o] * l.inv - (l.c_re * w_i + l.c_im * w_r);
 		put(a.dx_re + d, g_r, a.accumulate_dx);
 		put(a.dx_im + d, g_i, a.accumulate_dx);
 		if (a.dxs_re) {
 			put(a.dxs_re + d, g_r, a.accumulate_dx);
 			put(a.dxs_im + d, -g_i, a.accumulate_dx);
 		}
-		a.xs_re[o] = xr[c] * inv;
-		a.xs_im[o] = xi[c] * inv;
+		a.xs_re[o] = xr[c] * l.inv;
+		a.xs_im[o] = xi[c] * l.inv;
+	}
+}
+
+// The logits of one row as a whole (two planes of leading dimension ldz, a multiple of four): S, the largest, the label's logit,
+// loss; and, BWD, the logits overwritten with their gradient.  T threads per row.
+template <int T, bool BWD>
+__global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__restrict__ z_re, float *__restrict__ z_im, long ldz) {
+	constexpr int W = T / 64;
+	__shared__ double lds_d[W];
+	__shared__ ArgMax lds_a[W];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+	const long row = blockIdx.x;
+	float *zr = z_re + row * ldz, *zi = z_im + row * ldz;
+	double sum = 0.0;
+	ArgMax top = {-1.0f, 0x7fffffff};
+	for (int c = 4 * t; c < a.N; c += 4 * T) {
+		float u[4], v[4];
+		load_v<4>(u, zr + c);
+		load_v<4>(v, zi + c);
+#pragma unroll
+		for (int k = 0; k < 4; ++k)
+			if (c + k < a.N) {
+				sum = fma((double) v[k], (double) v[k], fma((double) u[k], (double) u[k], sum));
+				const float q = fmaf(u[k], u[k], v[k] * v[k]);
+				if (q > top.v) top = ArgMax{q, c + k};
+			}
+	}
+	sum = group_reduce<double, W>(sum, SumD(), lds_d, 0, wave, lane);
+	top = group_reduce<ArgMax, W>(top, ArgMaxOp(), lds_a, 0, wave, lane);
+	const float S = clamped((float) sum);
+	const int best = top.i < 0 || top.i >= a.N ? 0 : top.i;  // a row of NaN has no largest entry
+	const LabelTerm l = label_term<W>(a, row, a.labels ? a.labels[row] : best, S, lds_d, t, lane, wave);
+	if (t == 0) {
+		a.s[row] = S;
+		if (a.loss) a.loss[row] = l.loss;
+		if (a.argmax) a.argmax[row] = best;
+	}
+	if (!BWD) return;
+	for (int c = 4 * t; c < a.N; c += 4 * T) {
+		float u[4], v[4];
+		load_v<4>(u, zr + c);
+		load_v<4>(v, zi + c);
+#pragma unroll
+		for (int k = 0; k < 4; ++k) {
+			u[k] *= l.inv;
+			v[k] *= -l.inv;
+			if (c + k == l.label) {
+				u[k] -= l.c_re;
+				v[k] -= l.c_im;
+			}
+		}
+		store_v<4>(zr + c, u);
+		store_v<4>(zi + c, v);
 	}
 }
 
@@ -367,24 +458,6 @@ __global__ __launch_bounds__(1024) void head_order_kernel(const int *__restrict_
 	}
 }
 
-template <int V>
-__device__ __forceinline__ void load_v(float *v, const float *p) {
-	if (V == 4) {
-		const float4 t = *reinterpret_cast<const float4 *>(p);
-		v[0] = t.x;
-		v[1 % V] = t.y;
-		v[2 % V] = t.z;
-		v[3 % V] = t.w;
-	} else {
-		v[0] = p[0];
-	}
-}
-template <int V>
-__device__ __forceinline__ void store_v(float *p, const float *v) {
-	if (V == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
-	else p[0] = v[0];
-}
-
 // subtracts V columns of one label's sum from its row of the gradient
 template <int V>
 __device__ __forceinline__ void subtract_label(const ScatterArgs &a, int label, int c, const float *re, const float *im) {
@@ -409,40 +482,59 @@ __device__ __forceinline__ void subtract_label(const ScatterArgs &a, int label, 
 // part[x][0] (it began before) or part[x][1] (it begins here).
 template <int V>
 __global__ __launch_bounds__(TPB) void head_label_kernel(const ScatterArgs a, int first) {
-	const int c = (blockIdx.y * TPB + threadIdx.x) * V;
-	const int p0 = first + blockIdx.x * CHUNK, block_end = min(a.B, first + ORDER_ROWS), p1 = min(block_end, p0 + CHUNK);
-	const int before = p0 > first ? a.label_of[p0 - 1] : -1, after = p1 < block_end ? a.label_of[p1] : -1;
+	__shared__ int label_at[CHUNK + 2], row_at[CHUNK];  // label_at[k + 1]: ordered row k of the chunk, and its neighbours
+	__shared__ float c_at[2][CHUNK];
+	const int t = threadIdx.x, c = (blockIdx.y * TPB + t) * V;
+	const int p0 = first + blockIdx.x * CHUNK, block_end = min(a.B, first + ORDER_ROWS);
+	if (t < CHUNK + 2) {
+		const int p = p0 + t - 1;
+		const int l = p >= first && p < block_end ? a.label_of[p] : -1;
+		label_at[t] = l >= a.N ? -1 : l;
+		if (t > 0 && t <= CHUNK) {
+			const int r = l >= 0 && l < a.N ? a.row_of[p] : 0;
+			row_at[t - 1] = r;
+			c_at[0][t - 1] = a.c_re[r];
+			c_at[1][t - 1] = a.c_im[r];
+		}
+	}
+	__syncthreads();
 	if (c >= a.K) return;
 	float re[V], im[V];
-	int label = -1, begin = p0;
-	for (int p = p0; p < p1; ++p) {
-		const int l = a.label_of[p];
-		if (l >= a.N) break;  // rows without a label are last
-		const int r = a.row_of[p];
-		if (l != label) {
-			label = l;
-			begin = p;
+	int begin = 0;
+	constexpr int AHEAD = 8;  // rows of x in flight
 #pragma unroll
-			for (int k = 0; k < V; ++k) re[k] = im[k] = 0.f;
-		}
-		const float c_re = a.c_re[r], c_im = a.c_im[r];
-		float x_r[V], x_i[V];
-		load_v<V>(x_r, a.x_re + (long) r * a.ldx + c);
-		load_v<V>(x_i, a.x_im + (long) r * a.ldx + c);
+	for (int k0 = 0; k0 < CHUNK; k0 += AHEAD) {
+		float x_r[AHEAD][V], x_i[AHEAD][V];
 #pragma unroll
-		for (int k = 0; k < V; ++k) {
-			re[k] += c_re * x_r[k] - c_im * x_i[k];
-			im[k] += c_re * x_i[k] + c_im * x_r[k];
+		for (int u = 0; u < AHEAD; ++u) {  // (a place without a label reads row 0 and is not used)
+			load_v<V>(x_r[u], a.x_re + (long) row_at[k0 + u] * a.ldx + c);
+			load_v<V>(x_i[u], a.x_im + (long) row_at[k0 + u] * a.ldx + c);
 		}
-		const int next = p + 1 < p1 ? a.label_of[p + 1] : after;
-		if (next == label && p + 1 < p1) continue;
-		const bool began = begin == p0 && before == label, goes_on = next == label;
-		if (!began && !goes_on) {
-			subtract_label<V>(a, label, c, re, im);
-		} else {
-			float *part = a.part + ((long) blockIdx.x * 2 + (began ? 0 : 1)) * 2 * a.ldk + c;
-			store_v<V>(part, re);
-			store_v<V>(part + a.ldk, im);
+#pragma unroll
+		for (int u = 0; u < AHEAD; ++u) {
+			const int k = k0 + u, label = label_at[k + 1];
+			if (label < 0) return;  // rows without a label are last
+			if (k == 0 || label_at[k] != label) {
+				begin = k;
+#pragma unroll
+				for (int q = 0; q < V; ++q) re[q] = im[q] = 0.f;
+			}
+			const float c_re = c_at[0][k], c_im = c_at[1][k];
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				re[q] += c_re * x_r[u][q] - c_im * x_i[u][q];
+				im[q] += c_re * x_i[u][q] + c_im * x_r[u][q];
+			}
+			const bool same = label_at[k + 2] == label;
+			if (same && k + 1 < CHUNK) continue;
+			const bool began = begin == 0 && label_at[0] == label;
+			if (!began && !same) {
+				subtract_label<V>(a, label, c, re, im);
+			} else {
+				float *part = a.part + ((long) blockIdx.x * 2 + (began ? 0 : 1)) * 2 * a.ldk + c;
+				store_v<V>(part, re);
+				store_v<V>(part + a.ldk, im);
+			}
 		}
 	}
 }
@@ -477,6 +569,26 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 	subtract_label<V>(a, label, c, re, im);
 }
 
+// Fills the rows behind `panel` wide diagonal blocks of a Hermitian matrix from the columns above them: C[j][i] = conj(C[i][j]).
+// Tiles of 32 x 32 turned over in LDS; blockIdx (x, y) = tile (column, row) of the part that is there.
+__global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K, int panel) {
+	__shared__ float tile[2][32][33];
+	const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
+	if (c0 / panel <= r0 / panel) return;  // (panel is a multiple of 32)
+	const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+	for (int k = ty; k < 32; k += 8)
+		if (r0 + k < K && c0 + tx < K) {
+			tile[0][k][tx] = c_re[(long) (r0 + k) * ldc + c0 + tx];
+			tile[1][k][tx] = c_im[(long) (r0 + k) * ldc + c0 + tx];
+		}
+	__syncthreads();
+	for (int k = ty; k < 32; k += 8)
+		if (c0 + k < K && r0 + tx < K) {
+			c_re[(long) (c0 + k) * ldc + r0 + tx] = tile[0][tx][k];
+			c_im[(long) (c0 + k) * ldc + r0 + tx] = -tile[1][tx][k];
+		}
+}
+
 // the gradient of no rows at all
 __global__ __launch_bounds__(TPB) void head_clear_kernel(float *p, long ld, int cols) {
 	for (int c = threadIdx.x; c < cols; c += TPB) p[blockIdx.x * ld + c] = 0.f;
@@ -504,7 +616,7 @@ struct HeadBuffers {
 };
 
 struct HeadPlan {
-	bool bwd, gram, pieces;
+	bool bwd, whole, gram, pieces;
 	int piece_cols;
 };
 
@@ -518,10 +630,18 @@ static long piece_bytes() {
 	return mb << 20;
 }
 
-// Which way the call goes, by the matrix products it then runs (complex multiplications; they are nearly all of its time).
-//   through the Gram matrix: T over N, y over K, and for the weights P = x^H (x / S) over B and w P over K
-//   through the logits: they, y, and for the weights x^T conj(z), with the logits formed again when one piece does not hold them
-// The argmax needs the logits either way.
+// A Hermitian product C = conj(A)^T B (K x K, both operands k-major, L long) in panels of rows that leave out what lies below the
+// diagonal blocks: 1024 x 1024 over 32768 takes 1.24 ms in four panels and 2.09 ms whole, over 8192 0.35 against 0.47 ms; a shorter
+// product would not fill the device with its panels.
+constexpr int PANEL = 256;
+static bool in_panels(int K, int L) { return K >= 2 * PANEL && (double) K * K * L >= (double) (1L << 31); }
+
+// Which way the call goes, by what its launches take: a product of m complex multiplications about 4 us + 8 m flop at 130 TFLOP/s,
+// any other kernel about 3 us, plus its bytes.
+//   whole   the logits in one piece, turned into their gradient where they lie; y and dw from it: three products, one kernel
+//   pieces  the logits piece by piece, and a second time for dw; the label's term by itself
+//   gram    T over N, y over K, P = x^H (x / S) over B, dw from it over K; the label's term by itself.  The argmax needs the logits
+//           all the same.
 static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	static const int forced = [] {
 		const char *e = getenv("CNET_HEAD_GRAM");  // tuning override: 0 / 1 never / always through the Gram matrix
@@ -529,13 +649,21 @@ static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	}();
 	HeadPlan p;
 	p.bwd = bwd;
-	const long whole = ((long) N + 63) / 64 * 64;
-	p.piece_cols = (int) std::min(whole, std::max(64L, piece_bytes() / (8 * (long) B) / 64 * 64));
+	const long all = ((long) N + 63) / 64 * 64;
+	p.piece_cols = (int) std::min(all, std::max(64L, piece_bytes() / (8 * (long) B) / 64 * 64));
+	const int pieces = (N + p.piece_cols - 1) / p.piece_cols;
 	const double b = B, k = K, n = N;
-	const double logits = b * n * k * (bwd ? (N <= p.piece_cols ? 3 : 4) : 1);
-	const double gram = (bwd ? 2 : 1) * (n + b) * k * k + (argmax ? b * n * k : 0);
-	p.gram = (bwd || !argmax) && (forced >= 0 ? forced != 0 : gram < logits);
-	p.pieces = argmax || !p.gram;
+	auto product = [](double m) { return 4.0 + m * 8 / 130e6; };
+	auto bytes = [](double v) { return 3.0 + v / 4e6; };
+	const double label = bwd ? 20 + bytes(60 * b * k) : 0;
+	const double scan = pieces * (product(b * n * k / pieces) + bytes(8 * b * n / pieces));
+	double direct, gram = (in_panels(K, N) ? 0.6 : 1.0) * product(n * k * k) + product(b * k * k) + (argmax ? scan : bytes(16 * b * k) + 3) + bytes(24 * b * k);
+	if (pieces == 1) direct = scan + (bwd ? bytes(16 * b * n) + 2 * product(b * n * k) : 0);
+	else direct = scan + bytes(24 * b * k) + (bwd ? pieces * 3 * product(b * n * k / pieces) + label : 0);
+	if (bwd) gram += (in_panels(K, B) ? 0.6 : 1.0) * product(b * k * k) + product(n * k * k) + label;
+	p.gram = (bwd || !argmax) && (forced >= 0 ? forced != 0 : gram < direct);
+	p.whole = !p.gram && pieces == 1;
+	p.pieces = !p.whole && (argmax || !p.gram);
 	return p;
 }
 
@@ -543,10 +671,11 @@ static int head_buffers(int B, int K, const HeadPlan &plan, HeadBuffers &b) {
 	b.piece_cols = plan.piece_cols;
 	b.ldk = ((long) K + 3) / 4 * 4;
 	const size_t rows = ((size_t) B + 63) / 64 * 64;
-	const size_t piece = plan.pieces ? 2 * (size_t) B * b.piece_cols : 0;
-	const size_t wide = plan.bwd || plan.gram ? 2 * (size_t) B * b.ldk : 0, square = plan.gram ? 2 * (size_t) K * b.ldk : 0;
+	const size_t piece = plan.pieces || plan.whole ? 2 * (size_t) B * b.piece_cols : 0;
+	const size_t wide = (plan.bwd && !plan.whole) || plan.gram ? 2 * (size_t) B * b.ldk : 0, square = plan.gram ? 2 * (size_t) K * b.ldk : 0;
 	const size_t part = plan.gram && !plan.pieces ? 2 * HEAD_SLABS * rows : 0;
-	const size_t order = plan.bwd ? rows : 0, label_part = plan.bwd ? (size_t) (std::min(B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
+	const bool label = plan.bwd && !plan.whole;
+	const size_t order = label ? rows : 0, label_part = label ? (size_t) (std::min(B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
 	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part) * sizeof(float));
 	if (!p) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
 	auto take = [&](size_t floats) {
@@ -585,6 +714,21 @@ static int conj_product_pair(bool a_kmajor, int M, int N, int K, const float *a_
 	float *cr[2] = {cs_re, c_re}, *ci[2] = {cs_im, c_im};
 	const bool cj[2] = {true, true};
 	return cgemm_pair(a_kmajor, true, 1, M, N, K, ar, ai, lda, br, bi, ldb, cj, cr, ci, ldc, accumulate, 0, 1);
+}
+
+// C = conj(A)^T B, Hermitian
+static int gram_product(int K, int L, const float *a_re, const float *a_im, long lda, const float *b_re, const float *b_im, long ldb, float *c_re, float *c_im,
+		long ldc) {
+	if (!in_panels(K, L)) return conj_product(1, K, K, L, a_re, a_im, lda, b_re, b_im, ldb, c_re, c_im, ldc, 0);
+	for (int k0 = 0; k0 < K; k0 += PANEL) {
+		const long o = (long) k0 * ldc + k0;
+		const int rc = conj_product(1, std::min(PANEL, K - k0), K - k0, L, a_re + k0, a_im + k0, lda, b_re + k0, b_im + k0, ldb, c_re + o, c_im + o, ldc, 0);
+		if (rc) return rc;
+	}
+	const unsigned tiles = (unsigned) ((K + 31) / 32);
+	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, PANEL);
+	CNET_LAUNCH_CHECK();
+	return CNET_OK;
 }
 
 static int head_labels(const HeadArgs &a, const HeadBuffers &b, int B, float *dw_re, float *dw_im, float *dws_re, float *dws_im, long lddw) {
@@ -632,6 +776,22 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 	auto logits = [&](int n0, int n) {
 		return cnet_clinear_fwd(a.x_re, a.x_im, a.ldx, a.w_re + (size_t) n0 * a.ldw, a.w_im + (size_t) n0 * a.ldw, a.ldw, z_re, z_im, np, B, K, n, 0);
 	};
+	if (plan.whole) {
+		rc = logits(0, N);
+		if (rc) return rc;
+		// a row of its own workgroup: many threads where the rows are long
+		if (N > 4096) {
+			if (bwd) hipLaunchKernelGGL((head_row_kernel<1024, true>), dim3((unsigned) B), dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
+			else hipLaunchKernelGGL((head_row_kernel<1024, false>), dim3((unsigned) B), dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
+		} else {
+			if (bwd) hipLaunchKernelGGL((head_row_kernel<TPB, true>), dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
+			else hipLaunchKernelGGL((head_row_kernel<TPB, false>), dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
+		}
+		CNET_LAUNCH_CHECK();
+		if (!bwd) return CNET_OK;
+		return cnet_clinear_bwd_sym(z_re, z_im, np, a.x_re, a.x_im, a.ldx, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx,
+				a.accumulate_dx, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw, B, K, N);
+	}
 	for (int n0 = 0; plan.pieces && n0 < N; n0 += np) {
 		const int n = std::min(np, N - n0);
 		rc = logits(n0, n);
@@ -644,7 +804,7 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 		}
 	}
 	if (plan.gram) {
-		rc = conj_product(1, K, K, N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, 0);
+		rc = gram_product(K, N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk);
 		if (rc) return rc;
 		rc = conj_product(0, B, K, K, a.x_re, a.x_im, a.ldx, g_re, g_im, ldk, y_re, y_im, ldk, 0);
 		if (rc) return rc;
@@ -662,7 +822,7 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 	CNET_LAUNCH_CHECK();
 	if (!bwd) return CNET_OK;
 	if (plan.gram) {
-		rc = conj_product(1, K, K, B, a.x_re, a.x_im, a.ldx, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk, 0);
+		rc = gram_product(K, B, a.x_re, a.x_im, a.ldx, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk);
 		if (rc) return rc;
 		rc = conj_product_pair(false, N, K, K, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw);
 		if (rc) return rc;

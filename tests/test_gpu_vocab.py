@@ -202,11 +202,15 @@ def head_check(B, K, N, pad=0, off=0, argmax=True, data=None):
     n = 2 * (K + N) + 64                                   # roundings on the longest path of a sum over both
     ok = np.isfinite(ref["loss"])
 
+    def close_loss(loss, want, rows):
+        # the label's logit has its products summed in double; what s is off by (its longest path, above) is off in the logarithm
+        bad = np.abs(loss - want) > (2 * (2 * K + 32) * HALF * ref["size_s"] / ref["s"])[rows] + 8 * HALF * (1 + np.abs(want))
+        assert not bad.any(), (loss[bad][:5], want[bad][:5])
+
     def check(s, loss, am):
         near(s, ref["s"], ref["size_s"], 2 * K + 32, "s")
-        s_rel = (3 * np.sqrt(2 * (2 * K + 32)) * HALF * ref["size_s"] / ref["s"]).max()
         assert np.array_equal(np.isnan(loss), ~ok)
-        assert np.all(np.abs(loss[ok] - ref["loss"][ok]) <= 2 * s_rel + 8 * HALF * (1 + np.abs(ref["loss"][ok])))
+        close_loss(loss[ok], ref["loss"][ok], ok)
         if am is not None:
             check_argmax(am, ref)
         assert np.all(loss[labels < 0] == 0)
@@ -218,7 +222,7 @@ def head_check(B, K, N, pad=0, off=0, argmax=True, data=None):
     ops.vocab_head_fwd(X, W, None, s1, loss1, am1)
     assert np.array_equal(am1.download(), am.download()) and np.array_equal(s1.download(), s.download())
     p = ref["power"][np.arange(B), am.download()] / ref["s"]
-    assert np.allclose(loss1.download(), -np.log(np.maximum(p, LEAST)), rtol=1e-5, atol=1e-5)
+    close_loss(loss1.download(), -np.log(np.maximum(p, LEAST)), np.arange(B))
     # a training step
     s2, loss2, am2 = capi.empty(B), capi.empty(B), capi.empty(B, np.int32)
     dX, dW = grad(x.shape, ld, off), grad(w.shape, ld, off)
@@ -237,7 +241,9 @@ def head_check(B, K, N, pad=0, off=0, argmax=True, data=None):
     assert np.all(dzs_of(dX2) == 5 + 5j) and np.all(dzs_of(dW2) == 5 + 5j)
     first = dz_of(dX), dz_of(dW)
     ops.vocab_head_fwd_bwd_sym(X, W, L, s2, loss2, am2 if argmax else None, dX, dW, accumulate_dx=1, accumulate_dw=1)
-    assert np.array_equal(dz_of(dX), 2 * first[0])
+    # (a product that goes out in two launches adds its parts to what is there one after the other: (a + b) + c in place of
+    # a + (b + c), so the doubled sum may be rounded differently)
+    near(dz_of(dX), 2 * first[0], 4 * (ref["size_dx"] + label_n / n * ref["label_dx"]), n, "dx twice")
     near(dz_of(dW), 2 * first[1], 4 * (ref["size_dw"] + label_n / n * ref["label_dw"]), n + 2 * B, "dw twice")
     assert np.array_equal(dzs_of(dW), dz_of(dW).conj())
     for pl in [X.re, X.im, W.re, W.im] + dX.planes + dW.planes + dX2.planes + dW2.planes:
@@ -254,6 +260,30 @@ HEAD = [(1, 1, 1, 0, 0), (3, 5, 7, 0, 0), (1, 64, 512, 0, 0), (2, 1024, 300, 0, 
 @pytest.mark.parametrize("argmax", [True, False])
 def test_vocab_head(gpu, B, K, N, pad, off, argmax):
     head_check(B, K, N, pad, off, argmax)
+
+
+@pytest.mark.parametrize("env", [{"CNET_HEAD_GRAM": "0", "CNET_HEAD_PIECE_MB": "1"}, {"CNET_HEAD_GRAM": "1", "CNET_HEAD_PIECE_MB": "1"},
+                                 {"CNET_HEAD_GRAM": "0"}])
+def test_vocab_head_every_way(gpu, env):
+    """through pieces of the logits, through the Gram matrix, and through whole logits, whatever the sizes"""
+    script = os.path.join(os.path.dirname(os.path.abspath(__file__)), "gpu_vocab_head_check.py")
+    res = subprocess.run([sys.executable, script], env={**os.environ, **env}, capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0 and res.stdout.strip().endswith("ok"), res.stdout[-500:] + res.stderr[-2000:]
+
+
+@pytest.mark.parametrize("weak", [1e-1, 1e-3, 1e-6])
+def test_vocab_head_rows_in_directions_that_the_weights_hardly_have(gpu, weak):
+    """Every row of w is one strong direction plus a little noise, and a third of the rows of x is orthogonal to it: there the Gram
+    matrix gives sum |z|^2 as a difference of large terms, and the rows are computed again from w."""
+    rng = np.random.default_rng(15)
+    B, K, N = 600, 64, 1000
+    x, w, labels = head_data(rng, B, K, N)
+    axis = np.ones(K) / np.sqrt(K)
+    w = rnd(rng, N, 1) * axis + weak * w
+    x[::3] -= (x[::3] @ axis)[:, None] * axis
+    x, w = (z.real.astype(np.float32).astype(np.float64) + 1j * z.imag.astype(np.float32) for z in (x, w))
+    labels[7] = 1
+    head_check(B, K, N, argmax=False, data=(x, w, labels))
 
 
 def test_vocab_head_gives_what_the_separate_calls_give(gpu):
