@@ -39,7 +39,7 @@ struct FwdArgs {
 };
 
 struct BwdArgs {
-	Planes x, v, h, w, g, gh;  // x the operand of the (first) norm; h, w, gh belong to the join; g = dL/dy
+	Planes x, v, h, w, g, gh;  // x: the operand of the (first) norm; gh: dL/d its result along the residual path; h, w, g = dL/dy: the next norm's
 	const float *s, *s2;
 	Out4 du, dx, dv;   // dv: only with a gate of its own for every row (the shared one goes through `partial`)
 	float *partial;    // [slab][planes][cols]: dv re, im (unless every row has a gate of its own), dw re, im
@@ -56,9 +56,277 @@ __device__ __forceinline__ float inv_rms(float sum, int cols, float eps) {
 
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
 
-// One workgroup per row, any width: the row is walked once per stage.
+// V consecutive columns from c on; what lies behind the row's end reads as zero and is not written
+template <int V>
+__device__ __forceinline__ void load_cols(float *v, const float *p, int c, int cols, int policy = 0) {
+	if (V == 4 && c + V <= cols) {
+		const float4 x = ld4(p + c, policy);
+		v[0] = x.x;
+		v[1 % V] = x.y;
+		v[2 % V] = x.z;
+		v[3 % V] = x.w;
+	} else {
+#pragma unroll
+		for (int k = 0; k < V; ++k) v[k] = c + k < cols ? p[c + k] : 0.f;
+	}
+}
+template <int V>
+__device__ __forceinline__ void store_cols(float *p, const float *v, int c, int cols, int accumulate, int policy) {
+	if (V == 4 && c + V <= cols) {
+		float4 x = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
+		if (accumulate) {
+			const float4 o = *reinterpret_cast<const float4 *>(p + c);
+			x.x += o.x, x.y += o.y, x.z += o.z, x.w += o.w;
+		}
+		st4(p + c, x, policy);
+	} else {
+#pragma unroll
+		for (int k = 0; k < V; ++k)
+			if (c + k < cols) put(p + c + k, v[k], accumulate);
+	}
+}
+// a gradient (dz) into its planes, and its conjugate where the dz* half is wanted
+template <int V>
+__device__ __forceinline__ void store_grad(const Out4 &o, long row, float *re, float *im, int c, int cols, int accumulate, int policy) {
+	const long at = row * o.ld;
+	store_cols<V>(o.re + at, re, c, cols, accumulate, policy);
+	store_cols<V>(o.im + at, im, c, cols, accumulate, policy);
+	if (o.sre) {
+#pragma unroll
+		for (int k = 0; k < V; ++k) im[k] = -im[k];
+		store_cols<V>(o.sre + at, re, c, cols, accumulate, policy);
+		store_cols<V>(o.sim + at, im, c, cols, accumulate, policy);
+	}
+}
+
+// T threads hold a row in registers, V x NIT columns each: every operand is read once and every result written once.  T = 64: four
+// rows to a workgroup of 256.
+template <int T, int NIT, int V, bool JOIN>
+__global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdArgs a, const int policy) {
+	constexpr int G = T / 64, ROWS = T < TPB ? TPB / T : 1;
+	__shared__ float lds[ROWS * G];
+	const int slot = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
+	const bool live = (long) blockIdx.x * ROWS + slot < a.rows;
+	const long row = live ? (long) blockIdx.x * ROWS + slot : a.rows - 1;
+	float x_r[NIT][V], x_i[NIT][V], u_r[NIT][V], u_i[NIT][V];
+#pragma unroll
+	for (int k = 0; k < NIT; ++k) {
+		const int c = (k * T + t) * V;
+		load_cols<V>(x_r[k], a.x.re + row * a.x.ld, c, a.cols, policy);
+		load_cols<V>(x_i[k], a.x.im + row * a.x.ld, c, a.cols, policy);
+	}
+	if (JOIN) {
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			const int c = (k * T + t) * V;
+			load_cols<V>(u_r[k], a.u.re + row * a.u.ld, c, a.cols, policy);
+			load_cols<V>(u_i[k], a.u.im + row * a.u.ld, c, a.cols, policy);
+		}
+	}
+	float sum = 0.f;
+#pragma unroll
+	for (int k = 0; k < NIT; ++k)
+#pragma unroll
+		for (int q = 0; q < V; ++q) sum += x_r[k][q] * x_r[k][q] + x_i[k][q] * x_i[k][q];
+	sum = group_reduce<float, G>(sum, SumF(), lds, slot, wave, lane);
+	const float s = inv_rms(sum, a.cols, a.eps);
+	if (t == 0 && live && a.s) a.s[row] = s;
+	float sum2 = 0.f;
+#pragma unroll
+	for (int k = 0; k < NIT; ++k) {
+		const int c = (k * T + t) * V;
+		float v_r[V], v_i[V];
+		load_cols<V>(v_r, a.v.re + row * a.v.ld, c, a.cols);
+		load_cols<V>(v_i, a.v.im + row * a.v.ld, c, a.cols);
+#pragma unroll
+		for (int q = 0; q < V; ++q) {
+			const float n_r = x_r[k][q] * s, n_i = x_i[k][q] * s;
+			float y_r = v_r[q] * n_r - v_i[q] * n_i, y_i = v_r[q] * n_i + v_i[q] * n_r;
+			if (JOIN) {
+				y_r = u_r[k][q] + a.scale * y_r;
+				y_i = u_i[k][q] + a.scale * y_i;
+				sum2 += y_r * y_r + y_i * y_i;
+			}
+			x_r[k][q] = y_r;
+			x_i[k][q] = y_i;
+		}
+		if (live) {
+			store_cols<V>((JOIN ? a.h_re + row * a.ldh : a.y_re + row * a.ldy), x_r[k], c, a.cols, 0, policy);
+			store_cols<V>((JOIN ? a.h_im + row * a.ldh : a.y_im + row * a.ldy), x_i[k], c, a.cols, 0, policy);
+		}
+	}
+	if (!JOIN || !a.y_re) return;
+	sum2 = group_reduce<float, G>(sum2, SumF(), lds, slot, wave, lane);
+	const float s2 = inv_rms(sum2, a.cols, a.eps);
+	if (!live) return;
+	if (t == 0 && a.s2) a.s2[row] = s2;
+#pragma unroll
+	for (int k = 0; k < NIT; ++k) {
+		const int c = (k * T + t) * V;
+		float w_r[V], w_i[V], y_r[V], y_i[V];
+		load_cols<V>(w_r, a.w.re, c, a.cols);
+		load_cols<V>(w_i, a.w.im, c, a.cols);
+#pragma unroll
+		for (int q = 0; q < V; ++q) {
+			const float n_r = x_r[k][q] * s2, n_i = x_i[k][q] * s2;
+			y_r[q] = w_r[q] * n_r - w_i[q] * n_i;
+			y_i[q] = w_r[q] * n_i + w_i[q] * n_r;
+		}
+		store_cols<V>(a.y_re + row * a.ldy, y_r, c, a.cols, 0, policy);
+		store_cols<V>(a.y_im + row * a.ldy, y_i, c, a.cols, 0, policy);
+	}
+}
+
+struct Sum3 {
+	float a, b, c;
+};
+struct Sum3Op {
+	__device__ Sum3 operator()(Sum3 x, Sum3 y) const { return Sum3{x.a + y.a, x.b + y.b, x.c + y.c}; }
+};
+
+// T threads hold one row at a time, V x NIT columns each; R groups of T threads walk the workgroup's rows in turn (group r takes row
+// r, r + R, ..) and keep their columns' sums of dv and dw in registers, which meet in LDS in group order at the end.
+// One exchange per row: with e = gh + s2 p (p = g w) and z = v n1, t2 = mean Re(p n2) and the mean of Re(dh z), which is
+// Re(e z) - s2 t2 Re(conj(n2) z), come from three sums that do not wait for each other.
+// SECOND: the next block's norm takes part (the join with a gradient at y).
+template <int T, int NIT, int V, bool SECOND>
+__global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdArgs a, const int policy) {
+	constexpr int G = T / 64, R = T < TPB ? TPB / T : 1, NP = SECOND ? 4 : 2;
+	__shared__ Sum3 lds[R * G];
+	extern __shared__ float sums[];  // [R - 1][NP][cols]
+	const int group = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
+	const int r0 = blockIdx.x * a.rows_per_slab, r1 = min(a.rows, r0 + a.rows_per_slab);
+	const bool shared = a.v.ld == 0;
+	const float inv_n = 1.0f / (float) a.cols;
+	float acc[NP][NIT][V];
+#pragma unroll
+	for (int p = 0; p < NP; ++p)
+#pragma unroll
+		for (int k = 0; k < NIT; ++k)
+#pragma unroll
+			for (int q = 0; q < V; ++q) acc[p][k][q] = 0.f;
+	// (every group makes the same number of rounds: the exchange is the whole workgroup's; a round beyond the rows stores nothing)
+	for (int base = r0; base < r1; base += R) {
+		const bool live = base + group < r1;
+		const long row = live ? base + group : r1 - 1;
+		const float s = a.s[row], s2 = SECOND ? a.s2[row] : 0.f;
+		float x_r[NIT][V], x_i[NIT][V], e_r[NIT][V], e_i[NIT][V], h_r[NIT][V], h_i[NIT][V], g_r[NIT][V], g_i[NIT][V], v_r[NIT][V], v_i[NIT][V];
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			const int c = (k * T + t) * V;
+			load_cols<V>(x_r[k], a.x.re + row * a.x.ld, c, a.cols, policy);
+			load_cols<V>(x_i[k], a.x.im + row * a.x.ld, c, a.cols, policy);
+			if (a.gh.re) {
+				load_cols<V>(e_r[k], a.gh.re + row * a.gh.ld, c, a.cols, policy);
+				load_cols<V>(e_i[k], a.gh.im + row * a.gh.ld, c, a.cols, policy);
+			} else {
+#pragma unroll
+				for (int q = 0; q < V; ++q) e_r[k][q] = e_i[k][q] = 0.f;
+			}
+			if (SECOND) {
+				load_cols<V>(h_r[k], a.h.re + row * a.h.ld, c, a.cols, policy);
+				load_cols<V>(h_i[k], a.h.im + row * a.h.ld, c, a.cols, policy);
+				load_cols<V>(g_r[k], a.g.re + row * a.g.ld, c, a.cols, policy);
+				load_cols<V>(g_i[k], a.g.im + row * a.g.ld, c, a.cols, policy);
+			}
+			load_cols<V>(v_r[k], a.v.re + row * a.v.ld, c, a.cols);
+			load_cols<V>(v_i[k], a.v.im + row * a.v.ld, c, a.cols);
+		}
+		Sum3 m = {0.f, 0.f, 0.f};
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			const int c = (k * T + t) * V;
+			float w_r[V], w_i[V];
+			if (SECOND) {
+				load_cols<V>(w_r, a.w.re, c, a.cols);
+				load_cols<V>(w_i, a.w.im, c, a.cols);
+			}
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				const float n_r = x_r[k][q] * s, n_i = x_i[k][q] * s;
+				x_r[k][q] = n_r;
+				x_i[k][q] = n_i;
+				const float z_r = v_r[k][q] * n_r - v_i[k][q] * n_i, z_i = v_r[k][q] * n_i + v_i[k][q] * n_r;
+				if (SECOND) {
+					const float p_r = g_r[k][q] * w_r[q] - g_i[k][q] * w_i[q], p_i = g_r[k][q] * w_i[q] + g_i[k][q] * w_r[q];
+					const float k_r = h_r[k][q] * s2, k_i = h_i[k][q] * s2;
+					h_r[k][q] = k_r;
+					h_i[k][q] = k_i;
+					m.b += p_r * k_r - p_i * k_i;
+					m.c += k_r * z_r + k_i * z_i;
+					e_r[k][q] += s2 * p_r;
+					e_i[k][q] += s2 * p_i;
+				}
+				m.a += e_r[k][q] * z_r - e_i[k][q] * z_i;
+			}
+		}
+		m = group_reduce<Sum3, G>(m, Sum3Op(), lds, group, wave, lane);
+		const float t2 = m.b * inv_n * s2, t1 = a.scale * (m.a - t2 * m.c) * inv_n;
+		if (!live) continue;
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			const int c = (k * T + t) * V;
+			float o_r[V], o_i[V], d_r[V], d_i[V];
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				d_r[q] = e_r[k][q];
+				d_i[q] = e_i[k][q];
+				if (SECOND) {
+					d_r[q] -= h_r[k][q] * t2;
+					d_i[q] += h_i[k][q] * t2;
+					acc[2 % NP][k][q] += g_r[k][q] * h_r[k][q] - g_i[k][q] * h_i[k][q];
+					acc[3 % NP][k][q] += g_r[k][q] * h_i[k][q] + g_i[k][q] * h_r[k][q];
+				}
+				e_r[k][q] = a.scale * d_r[q];
+				e_i[k][q] = a.scale * d_i[q];
+				o_r[q] = s * (e_r[k][q] * v_r[k][q] - e_i[k][q] * v_i[k][q] - x_r[k][q] * t1);
+				o_i[q] = s * (e_r[k][q] * v_i[k][q] + e_i[k][q] * v_r[k][q] + x_i[k][q] * t1);
+			}
+			if (a.du.re) store_grad<V>(a.du, row, d_r, d_i, c, a.cols, a.accumulate, policy);
+			store_grad<V>(a.dx, row, o_r, o_i, c, a.cols, a.accumulate, policy);
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				d_r[q] = e_r[k][q] * x_r[k][q] - e_i[k][q] * x_i[k][q];
+				d_i[q] = e_r[k][q] * x_i[k][q] + e_i[k][q] * x_r[k][q];
+				acc[0][k][q] += d_r[q];
+				acc[1][k][q] += d_i[q];
+			}
+			if (!shared) store_grad<V>(a.dv, row, d_r, d_i, c, a.cols, a.accumulate_w, policy);
+		}
+	}
+	if (!a.planes) return;
+	if (R > 1 && group > 0) {
+#pragma unroll
+		for (int p = 0; p < NP; ++p)
+#pragma unroll
+			for (int k = 0; k < NIT; ++k) store_cols<V>(sums + ((group - 1) * NP + p) * (T * NIT * V), acc[p][k], (k * T + t) * V, T * NIT * V, 0, 0);
+	}
+	if (R > 1) __syncthreads();
+	if (group > 0) return;
+	float *part = a.partial + (long) blockIdx.x * a.planes * a.cols;
+#pragma unroll
+	for (int p = 0; p < NP; ++p) {
+		if (p < 2 && !shared) continue;
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			const int c = (k * T + t) * V;
+			for (int r = 1; r < R; ++r) {
+				float more[V];
+				load_cols<V>(more, sums + ((r - 1) * NP + p) * (T * NIT * V), c, T * NIT * V);
+#pragma unroll
+				for (int q = 0; q < V; ++q) acc[p][k][q] += more[q];
+			}
+			float *dst = part + (long) (shared ? p : p - 2) * a.cols;
+#pragma unroll
+			for (int q = 0; q < V; ++q)
+				if (c + q < a.cols) dst[c + q] = acc[p][k][q];
+		}
+	}
+}
+
+// Rows wider than the kernels above hold in registers: one workgroup per row, which walks it once per stage.
 template <bool JOIN>
-__global__ __launch_bounds__(TPB) void norm_fwd_kernel(const FwdArgs a) {
+__global__ __launch_bounds__(TPB) void norm_fwd_wide_kernel(const FwdArgs a) {
 	__shared__ float lds[TPB / 64];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.x;
@@ -98,10 +366,10 @@ __global__ __launch_bounds__(TPB) void norm_fwd_kernel(const FwdArgs a) {
 	}
 }
 
-// A workgroup takes `rows_per_slab` rows one after the other; its columns' sums of dv and dw stay in its own rows of `partial`
+// The same for rows too wide for registers.  A workgroup takes `rows_per_slab` rows one after the other; its columns' sums of dv and dw stay in its own rows of `partial`
 // (each thread always meets the same columns: no atomics, one order), which norm_sum_kernel adds in slab order.
-template <bool JOIN>
-__global__ __launch_bounds__(TPB) void norm_bwd_kernel(const BwdArgs a) {
+template <bool SECOND>
+__global__ __launch_bounds__(TPB) void norm_bwd_wide_kernel(const BwdArgs a) {
 	__shared__ float lds[TPB / 64];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const int r0 = blockIdx.x * a.rows_per_slab, r1 = min(a.rows, r0 + a.rows_per_slab);
@@ -109,7 +377,7 @@ __global__ __launch_bounds__(TPB) void norm_bwd_kernel(const BwdArgs a) {
 	const float inv_n = 1.0f / (float) a.cols;
 	float *part = a.partial + (long) blockIdx.x * a.planes * a.cols;
 	for (long row = r0; row < r1; ++row) {
-		const float s = a.s[row], s2 = JOIN && a.g.re ? a.s2[row] : 0.f;
+		const float s = a.s[row], s2 = SECOND ? a.s2[row] : 0.f;
 		// the gradient that the next norm hands back to h at one column, before its share of t2
 		auto next = [&](int c, float &p_r, float &p_i, float &n_r, float &n_i) {
 			const float g_r = a.g.re[row * a.g.ld + c], g_i = a.g.im[row * a.g.ld + c];
@@ -120,7 +388,7 @@ __global__ __launch_bounds__(TPB) void norm_bwd_kernel(const BwdArgs a) {
 			n_i = a.h.im[row * a.h.ld + c] * s2;
 		};
 		float t2 = 0.f;
-		if (JOIN && a.g.re) {
+		if (SECOND) {
 			for (int c = t; c < a.cols; c += TPB) {
 				float p_r, p_i, n_r, n_i;
 				next(c, p_r, p_i, n_r, n_i);
@@ -130,21 +398,16 @@ __global__ __launch_bounds__(TPB) void norm_bwd_kernel(const BwdArgs a) {
 		}
 		// the gradient at the result of the (first) norm and its weights: scale dh, or g
 		auto at = [&](int c, float &d_r, float &d_i) {
-			if (!JOIN) {
-				d_r = a.g.re[row * a.g.ld + c];
-				d_i = a.g.im[row * a.g.ld + c];
-				return;
-			}
 			d_r = a.gh.re ? a.gh.re[row * a.gh.ld + c] : 0.f;
 			d_i = a.gh.re ? a.gh.im[row * a.gh.ld + c] : 0.f;
-			if (a.g.re) {
+			if (SECOND) {
 				float p_r, p_i, n_r, n_i;
 				next(c, p_r, p_i, n_r, n_i);
 				d_r += s2 * (p_r - n_r * t2);
 				d_i += s2 * (p_i + n_i * t2);
 			}
 		};
-		const float k = JOIN ? a.scale : 1.0f;
+		const float k = a.scale;
 		float t1 = 0.f;
 		for (int c = t; c < a.cols; c += TPB) {
 			float d_r, d_i;
@@ -159,7 +422,7 @@ __global__ __launch_bounds__(TPB) void norm_bwd_kernel(const BwdArgs a) {
 		for (int c = t; c < a.cols; c += TPB) {
 			float d_r, d_i;
 			at(c, d_r, d_i);
-			if (JOIN) {
+			if (a.du.re) {
 				const long o = row * a.du.ld + c;
 				put(a.du.re + o, d_r, a.accumulate);
 				put(a.du.im + o, d_i, a.accumulate);
@@ -195,7 +458,7 @@ __global__ __launch_bounds__(TPB) void norm_bwd_kernel(const BwdArgs a) {
 					put(a.dv.sim + ov, -e_i, a.accumulate_w);
 				}
 			}
-			if (JOIN && a.g.re) {
+			if (SECOND) {
 				float p_r, p_i, m_r, m_i;
 				next(c, p_r, p_i, m_r, m_i);
 				const float g_r = a.g.re[row * a.g.ld + c], g_i = a.g.im[row * a.g.ld + c];
@@ -206,13 +469,23 @@ __global__ __launch_bounds__(TPB) void norm_bwd_kernel(const BwdArgs a) {
 	}
 }
 
-// dst[plane][c] (+)= sum over slabs, in slab order; plane 0, 1: `first`, 2, 3: `second`
-__global__ __launch_bounds__(TPB) void norm_sum_kernel(const float *__restrict__ partial, int nslabs, int planes, int cols, Out4 first, Out4 second,
-		int accumulate) {
-	const long idx = (long) blockIdx.x * TPB + threadIdx.x;
-	if (idx >= (long) planes * cols) return;
+// dst[plane][c] (+)= sum over slabs; plane 0, 1: `first`, 2, 3: `second`.  COLS (plane, column) pairs per workgroup x LANES lanes that
+// each add one contiguous part of the slabs in order; the lanes' sums are added in lane order.
+template <int LANES, int COLS>
+__global__ __launch_bounds__(LANES * COLS) void norm_sum_kernel(const float *__restrict__ partial, int nslabs, int planes, int cols, Out4 first,
+		Out4 second, int accumulate) {
+	__shared__ float red[LANES][COLS];
+	const int tx = threadIdx.x % COLS, ty = threadIdx.x / COLS;
+	const long idx = (long) blockIdx.x * COLS + tx;
+	const bool live = idx < (long) planes * cols;
+	const int per = (nslabs + LANES - 1) / LANES, k0 = min(nslabs, ty * per), k1 = min(nslabs, k0 + per);
+	red[ty][tx] = live ? cnet::ordered_sum(partial + (long) k0 * planes * cols + idx, (long) planes * cols, k1 - k0) : 0.f;
+	__syncthreads();
+	if (ty || !live) return;
 	const int p = (int) (idx / cols), c = (int) (idx - (long) p * cols);
-	const float sum = cnet::ordered_sum(partial + idx, (long) planes * cols, nslabs);
+	float sum = red[0][tx];
+#pragma unroll 8
+	for (int l = 1; l < LANES; ++l) sum += red[l][tx];
 	const Out4 &o = p < 2 ? first : second;
 	put((p & 1 ? o.im : o.re) + c, sum, accumulate);
 	if (o.sre) put((p & 1 ? o.sim : o.sre) + c, p & 1 ? -sum : sum, accumulate);
@@ -222,43 +495,89 @@ __global__ __launch_bounds__(TPB) void norm_sum_kernel(const float *__restrict__
 
 using namespace cnet;
 
-static int norm_fwd(const FwdArgs &a, bool join) {
-	dim3 grid((unsigned) a.rows);
-	if (join) hipLaunchKernelGGL(norm_fwd_kernel<true>, grid, dim3(TPB), 0, rt().stream, a);
-	else hipLaunchKernelGGL(norm_fwd_kernel<false>, grid, dim3(TPB), 0, rt().stream, a);
+// (no slabs: the sum over no rows, zero)
+static int norm_sum(const float *partial, int nslabs, int planes, int cols, const Out4 &first, const Out4 &second, int accumulate) {
+	const long n = (long) planes * cols;
+	if (nslabs > 32)
+		hipLaunchKernelGGL((norm_sum_kernel<64, 16>), dim3((unsigned) ((n + 15) / 16)), dim3(1024), 0, rt().stream, partial, nslabs, planes, cols, first,
+				second, accumulate);
+	else
+		hipLaunchKernelGGL((norm_sum_kernel<4, 64>), dim3((unsigned) ((n + 63) / 64)), dim3(256), 0, rt().stream, partial, nslabs, planes, cols, first,
+				second, accumulate);
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
 
-static int norm_bwd(BwdArgs &a, bool join, const Out4 &dv, const Out4 &dw) {
-	const bool shared = a.v.ld == 0, second = join && a.g.re;
+template <int T, int E>
+static void launch_fwd(const FwdArgs &a, bool join, bool vec, int policy) {
+	constexpr int ROWS = T < TPB ? TPB / T : 1;
+	const dim3 grid((unsigned) ((a.rows + ROWS - 1) / ROWS)), block(T < TPB ? TPB : T);
+	if (join && vec) hipLaunchKernelGGL((norm_fwd_kernel<T, E / 4, 4, true>), grid, block, 0, rt().stream, a, policy);
+	else if (join) hipLaunchKernelGGL((norm_fwd_kernel<T, E, 1, true>), grid, block, 0, rt().stream, a, policy);
+	else if (vec) hipLaunchKernelGGL((norm_fwd_kernel<T, E / 4, 4, false>), grid, block, 0, rt().stream, a, policy);
+	else hipLaunchKernelGGL((norm_fwd_kernel<T, E, 1, false>), grid, block, 0, rt().stream, a, policy);
+}
+
+// 128-bit accesses: every row of every plane starts on 16 bytes
+static bool vec_ok(const Planes &p) { return p.ld % 4 == 0 && aligned16(p.re) && aligned16(p.im); }
+static bool vec_ok(const Out4 &o) { return o.ld % 4 == 0 && aligned16(o.re) && aligned16(o.im) && aligned16(o.sre) && aligned16(o.sim); }
+
+static int norm_fwd(const FwdArgs &a, bool join) {
+	const bool vec = vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.u) && vec_ok(a.w) && vec_ok(Planes{a.y_re, a.y_im, a.ldy}) &&
+			vec_ok(Planes{a.h_re, a.h_im, a.ldh});
+	const int policy = stream_policy(ST_STORES, join ? 8 : 4, (long) a.rows * a.cols);
+	if (a.cols <= 256) launch_fwd<64, 4>(a, join, vec, policy);
+	else if (a.cols <= 512) launch_fwd<64, 8>(a, join, vec, policy);
+	else if (a.cols <= 1024) launch_fwd<64, 16>(a, join, vec, policy);
+	else if (a.cols <= 2048) launch_fwd<256, 8>(a, join, vec, policy);
+	else if (a.cols <= 4096) launch_fwd<256, 16>(a, join, vec, policy);
+	else if (a.cols <= 8192) launch_fwd<1024, 8>(a, join, vec, policy);
+	else if (a.cols <= 16384) launch_fwd<1024, 16>(a, join, vec, policy);
+	else if (join) hipLaunchKernelGGL(norm_fwd_wide_kernel<true>, dim3((unsigned) a.rows), dim3(TPB), 0, rt().stream, a);
+	else hipLaunchKernelGGL(norm_fwd_wide_kernel<false>, dim3((unsigned) a.rows), dim3(TPB), 0, rt().stream, a);
+	CNET_LAUNCH_CHECK();
+	return CNET_OK;
+}
+
+template <int T, int E>
+static void launch_bwd(const BwdArgs &a, bool second, bool vec, int nslabs, int policy) {
+	constexpr int R = T < TPB ? TPB / T : 1;
+	const dim3 grid((unsigned) nslabs), block(T < TPB ? TPB : T);
+	const size_t lds = (size_t) (R - 1) * (second ? 4 : 2) * T * E * sizeof(float);
+	if (second && vec) hipLaunchKernelGGL((norm_bwd_kernel<T, E / 4, 4, true>), grid, block, lds, rt().stream, a, policy);
+	else if (second) hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, true>), grid, block, lds, rt().stream, a, policy);
+	else if (vec) hipLaunchKernelGGL((norm_bwd_kernel<T, E / 4, 4, false>), grid, block, lds, rt().stream, a, policy);
+	else hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, false>), grid, block, lds, rt().stream, a, policy);
+}
+
+// The gate alone is the join without a second norm, without a residual path to hand its gradient to, and with scale 1: its gradient
+// at y arrives in a.gh then.
+static int norm_bwd(BwdArgs &a, const Out4 &dv, const Out4 &dw) {
+	const bool shared = a.v.ld == 0, second = a.g.re != nullptr;
 	a.planes = (shared ? 2 : 0) + (second ? 2 : 0);
-	const int want = std::min(a.rows, 4 * rt().prop.multiProcessorCount);
+	const bool vec = vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.h) && vec_ok(a.w) && vec_ok(a.g) && vec_ok(a.gh) && vec_ok(a.du) && vec_ok(a.dx) && vec_ok(a.dv);
+	// Two or three workgroups to a compute unit, each with as many rows: a workgroup's sums are written and read again, which more of
+	// them would do more often.
+	const int groups = a.cols <= 512 ? 4 : a.cols <= 1024 ? 2 : 1;  // rows that a workgroup works on at a time
+	const int want = std::max(1, std::min((a.rows + groups - 1) / groups, 3 * rt().prop.multiProcessorCount));
 	a.rows_per_slab = (a.rows + want - 1) / want;
 	const int nslabs = (a.rows + a.rows_per_slab - 1) / a.rows_per_slab;
 	if (a.planes) {
 		a.partial = (float *) workspace((size_t) nslabs * a.planes * a.cols * sizeof(float));
 		if (!a.partial) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
 	}
-	if (join) hipLaunchKernelGGL(norm_bwd_kernel<true>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
-	else hipLaunchKernelGGL(norm_bwd_kernel<false>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
+	const int policy = stream_policy(ST_LOADS, second ? 12 : 6, (long) a.rows * a.cols);
+	if (a.cols <= 512) launch_bwd<64, 8>(a, second, vec, nslabs, policy);
+	else if (a.cols <= 1024) launch_bwd<128, 8>(a, second, vec, nslabs, policy);
+	else if (a.cols <= 2048) launch_bwd<256, 8>(a, second, vec, nslabs, policy);
+	else if (a.cols <= 4096) launch_bwd<512, 8>(a, second, vec, nslabs, policy);
+	else if (second) hipLaunchKernelGGL(norm_bwd_wide_kernel<true>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
+	else hipLaunchKernelGGL(norm_bwd_wide_kernel<false>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
 	CNET_LAUNCH_CHECK();
-	if (a.planes) {
-		const long n = (long) a.planes * a.cols;
-		hipLaunchKernelGGL(norm_sum_kernel, dim3((unsigned) ((n + TPB - 1) / TPB)), dim3(TPB), 0, rt().stream, a.partial, nslabs, a.planes, a.cols,
-				shared ? dv : dw, dw, a.accumulate_w);
-		CNET_LAUNCH_CHECK();
-	}
-	return CNET_OK;
+	return a.planes ? norm_sum(a.partial, nslabs, a.planes, a.cols, shared ? dv : dw, dw, a.accumulate_w) : CNET_OK;
 }
 
-// no rows: the sum over them is zero
-static int norm_no_rows(int planes, int cols, const Out4 &first, const Out4 &second) {
-	const long n = (long) planes * cols;
-	hipLaunchKernelGGL(norm_sum_kernel, dim3((unsigned) ((n + TPB - 1) / TPB)), dim3(TPB), 0, rt().stream, nullptr, 0, planes, cols, first, second, 0);
-	CNET_LAUNCH_CHECK();
-	return CNET_OK;
-}
+static int norm_no_rows(int planes, int cols, const Out4 &first, const Out4 &second) { return norm_sum(nullptr, 0, planes, cols, first, second, 0); }
 
 extern "C" {
 
@@ -301,14 +620,14 @@ int cnet_norm_gate_bwd_sym(const float *x_re, const float *x_im, int64_t ldx, co
 	CNET_CHECK_ARG(ldx >= cols && (ldv == 0 || ldv >= cols) && ldg >= cols && lddx >= cols);
 	a.x = Planes{x_re, x_im, (long) ldx};
 	a.v = Planes{v_re, v_im, (long) ldv};
-	a.g = Planes{g_dz_re, g_dz_im, (long) ldg};
+	a.gh = Planes{g_dz_re, g_dz_im, (long) ldg};
 	a.s = s;
 	a.dx = Out4{dx_dz_re, dx_dz_im, dx_dzs_re, dx_dzs_im, (long) lddx};
 	a.dv = dv;
 	a.scale = 1.0f;
 	a.accumulate = accumulate;
 	a.accumulate_w = accumulate_w;
-	return norm_bwd(a, false, dv, dv);
+	return norm_bwd(a, dv, dv);
 }
 
 int cnet_norm_join_fwd(const float *u_re, const float *u_im, int64_t ldu, const float *f_re, const float *f_im, int64_t ldf, const float *v_re,
@@ -383,7 +702,7 @@ int cnet_norm_join_bwd_sym(const float *f_re, const float *f_im, int64_t ldf, co
 	a.cols = cols;
 	a.accumulate = accumulate;
 	a.accumulate_w = accumulate_w;
-	return norm_bwd(a, true, dv, dw);
+	return norm_bwd(a, dv, dw);
 }
 
 }  // extern "C"

@@ -49,6 +49,10 @@ __device__ __forceinline__ void store_v(float *p, const float *v) {
 	else p[0] = v[0];
 }
 
+struct SumF2 {
+	__device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, a.y + b.y); }
+};
+
 // ------------------------------------------------------------------------------------------------ distillation
 struct DistillArgs {
 	const float *z_re, *z_im;
@@ -62,74 +66,205 @@ struct DistillArgs {
 	int rows, cols;
 };
 
-// One workgroup per row.  FWD: S and the loss; BWD: the gradient, with the S just formed or the one given.  The gradient is
-// written for every column as if no entry named it, and the named ones are written again behind a barrier: the first entry of
-// an index writes it, with the weights of all entries of that index.
-template <bool FWD, bool BWD>
-__global__ __launch_bounds__(TPB) void distill_kernel(const DistillArgs a) {
-	__shared__ double lds_d[WAVES];
-	__shared__ float lds_f[WAVES];
-	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-	const long row = blockIdx.x;
+// A row's entries in LDS, `top` of each (floats): index, weight, and the row's values there
+struct Entries {
+	int *id;
+	float *q, *re, *im;
+};
+__device__ __forceinline__ Entries entries_at(float *lds, int top) { return Entries{(int *) lds, lds + top, lds + 2 * top, lds + 3 * top}; }
+
+// T threads fetch the entries of their row
+template <int T>
+__device__ __forceinline__ void fetch_entries(const DistillArgs &a, const Entries &e, long row, int t) {
+	for (int j = t; j < a.top; j += T) {
+		const int id = a.ids[row * a.top + j];
+		const bool there = id >= 0 && id < a.cols;
+		e.id[j] = id;
+		e.q[j] = id < 0 ? 0.f : a.probs[row * a.top + j];
+		e.re[j] = there ? a.z_re[row * a.ldz + id] : 0.f;
+		e.im[j] = there ? a.z_im[row * a.ldz + id] : 0.f;
+	}
+}
+
+// one thread's part of the loss, and of the entries' total weight
+template <int T>
+__device__ __forceinline__ void entry_sums(const DistillArgs &a, const Entries &e, float S, int t, float &terms, float &total) {
+	terms = total = 0.f;
+	for (int j = t; j < a.top; j += T) {
+		const float q = e.q[j];
+		total += q;
+		if (q == 0.f) continue;
+		double p = (double) __builtin_nanf("");
+		if (e.id[j] < a.cols) p = clamped(((double) e.re[j] * e.re[j] + (double) e.im[j] * e.im[j]) / (double) S);
+		terms += q * logf((float) (q / p));
+	}
+}
+
+__device__ __forceinline__ void distill_store(const DistillArgs &a, long row, int c, float re, float im) {
+	const long o = row * a.lddz + c;
+	a.dz_re[o] = re;
+	a.dz_im[o] = im;
+	if (a.dzs_re) {
+		a.dzs_re[o] = re;
+		a.dzs_im[o] = -im;
+	}
+}
+
+// The gradient at the entries' own columns among [c0, c1), over what the pass over the whole row has left there: the first entry
+// of an index writes it, with the weights of all entries of that index.
+template <int T>
+__device__ __forceinline__ void entry_gradients(const DistillArgs &a, const Entries &e, long row, float S, float total, int t, int c0, int c1) {
+	for (int j = t; j < a.top; j += T) {
+		const int id = e.id[j];
+		if (id < c0 || id >= c1) continue;
+		float q = 0.f;
+		int first = j;
+		for (int i = a.top - 1; i >= 0; --i)
+			if (e.id[i] == id) {
+				first = i;
+				q += e.q[i];
+			}
+		if (first != j) continue;
+		const double m = clamped((double) e.re[j] * e.re[j] + (double) e.im[j] * e.im[j]);
+		const float k = (float) ((double) total / S - q / m);
+		distill_store(a, row, id, e.re[j] * k, -(e.im[j] * k));
+	}
+}
+
+// The row in registers: T threads hold V x NIT columns each, so z is read once and the gradient written once, 16 bytes per element
+// each way (24 with dz*).  The entries and their values are fetched while the row is on its way.  T = 64: four rows to a workgroup.
+// 
+template <int T, int NIT, int V>
+__global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const DistillArgs a, const int policy) {
+	constexpr int G = T / 64, ROWS = T < TPB ? TPB / T : 1;
+	extern __shared__ float lds[];
+	__shared__ double lds_d[G];
+	__shared__ float2 lds_f[G];
+	const int slot = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
+	const bool live = (long) blockIdx.x * ROWS + slot < a.rows;
+	const long row = live ? (long) blockIdx.x * ROWS + slot : a.rows - 1;
+	const Entries e = entries_at(lds + slot * 4 * a.top, a.top);
 	const float *zr = a.z_re + row * a.ldz, *zi = a.z_im + row * a.ldz;
-	const int *ids = a.ids + row * a.top;
-	const float *probs = a.probs + row * a.top;
+	float re[NIT][V], im[NIT][V];
+#pragma unroll
+	for (int k = 0; k < NIT; ++k) {
+		const int c = (k * T + t) * V;
+#pragma unroll
+		for (int q = 0; q < V; ++q) re[k][q] = im[k][q] = 0.f;
+		if (c + V <= a.cols) {
+			if (V == 4) {
+				const float4 x = ld4(zr + c, policy), y = ld4(zi + c, policy);
+				re[k][0] = x.x, re[k][1 % V] = x.y, re[k][2 % V] = x.z, re[k][3 % V] = x.w;
+				im[k][0] = y.x, im[k][1 % V] = y.y, im[k][2 % V] = y.z, im[k][3 % V] = y.w;
+			} else {
+				re[k][0] = zr[c];
+				im[k][0] = zi[c];
+			}
+		} else if (V > 1) {
+#pragma unroll
+			for (int q = 0; q < V; ++q)
+				if (c + q < a.cols) {
+					re[k][q] = zr[c + q];
+					im[k][q] = zi[c + q];
+				}
+		}
+	}
+	fetch_entries<T>(a, e, row, t);
 	float S;
-	if (FWD) {
+	if (a.loss) {
 		double sum = 0.0;
-		for (int c = t; c < a.cols; c += TPB) sum = fma((double) zi[c], (double) zi[c], fma((double) zr[c], (double) zr[c], sum));
-		sum = group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane);
-		S = clamped((float) sum);
-		float terms = 0.f;
-		for (int j = t; j < a.top; j += TPB) {
-			const int id = ids[j];
-			const float q = probs[j];
-			if (id < 0 || q == 0.f) continue;
-			double p = (double) __builtin_nanf("");
-			if (id < a.cols) p = clamped(((double) zr[id] * zr[id] + (double) zi[id] * zi[id]) / (double) S);
-			terms += q * logf((float) (q / p));
-		}
-		terms = group_reduce<float, WAVES>(terms, SumF(), lds_f, 0, wave, lane);
-		if (t == 0) {
-			a.s[row] = S;
-			a.loss[row] = terms;
-		}
+#pragma unroll
+		for (int k = 0; k < NIT; ++k)
+#pragma unroll
+			for (int q = 0; q < V; ++q) sum = fma((double) im[k][q], (double) im[k][q], fma((double) re[k][q], (double) re[k][q], sum));
+		S = clamped((float) group_reduce<double, G>(sum, SumD(), lds_d, 0, wave, lane));
 	} else {
 		S = a.s[row];
 	}
-	if (!BWD) return;
-	float total = 0.f;
-	for (int j = t; j < a.top; j += TPB)
-		if (ids[j] >= 0) total += probs[j];
-	total = group_reduce<float, WAVES>(total, SumF(), lds_f, 0, wave, lane);
-	const float share = total / S;
-	float *or_ = a.dz_re + row * a.lddz, *oi = a.dz_im + row * a.lddz;
-	float *sr = a.dzs_re ? a.dzs_re + row * a.lddz : nullptr, *si = a.dzs_re ? a.dzs_im + row * a.lddz : nullptr;
-	auto store = [&](int c, float re, float im) {
-		or_[c] = re;
-		oi[c] = im;
-		if (sr) {
-			sr[c] = re;
-			si[c] = -im;
-		}
-	};
-	for (int c = t; c < a.cols; c += TPB) store(c, zr[c] * share, -(zi[c] * share));
-	__syncthreads();
-	for (int j = t; j < a.top; j += TPB) {
-		const int id = ids[j];
-		if (id < 0 || id >= a.cols) continue;
-		float q = 0.f;
-		bool first = true;
-		for (int i = 0; i < a.top; ++i)
-			if (ids[i] == id) {
-				if (i < j) first = false;
-				q += probs[i];
-			}
-		if (!first) continue;
-		const double m = clamped((double) zr[id] * zr[id] + (double) zi[id] * zi[id]);
-		const float k = (float) ((double) total / S - q / m);
-		store(id, zr[id] * k, -(zi[id] * k));
+	if (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the entries are this wavefront's own
+	else __syncthreads();
+	float2 sums;
+	entry_sums<T>(a, e, S, t, sums.x, sums.y);
+	sums = group_reduce<float2, G>(sums, SumF2(), lds_f, 0, wave, lane);
+	if (a.loss && t == 0 && live) {
+		a.s[row] = S;
+		a.loss[row] = sums.x;
 	}
+	if (!a.dz_re) return;
+	const float share = sums.y / S;
+	if (live) {
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			const int c = (k * T + t) * V;
+			if (V == 4 && c + V <= a.cols) {
+				const long o = row * a.lddz + c;
+				const float4 u = make_float4(re[k][0] * share, re[k][1 % V] * share, re[k][2 % V] * share, re[k][3 % V] * share);
+				const float4 v = make_float4(im[k][0] * share, im[k][1 % V] * share, im[k][2 % V] * share, im[k][3 % V] * share);
+				const float4 n = make_float4(-v.x, -v.y, -v.z, -v.w);
+				st4(a.dz_re + o, u, policy);
+				st4(a.dz_im + o, n, policy);
+				if (a.dzs_re) {
+					st4(a.dzs_re + o, u, policy);
+					st4(a.dzs_im + o, v, policy);
+				}
+			} else {
+#pragma unroll
+				for (int q = 0; q < V; ++q)
+					if (c + q < a.cols) distill_store(a, row, c + q, re[k][q] * share, -(im[k][q] * share));
+			}
+		}
+	}
+	if (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+	else __syncthreads();
+	if (live) entry_gradients<T>(a, e, row, S, sums.y, t, 0, a.cols);
+}
+
+// Rows too long for that, or too few: a row is dealt out to `slabs` workgroups of `width` columns each, in two launches.
+__global__ __launch_bounds__(TPB) void distill_slab_sum_kernel(const DistillArgs a, double *__restrict__ part, int width) {
+	__shared__ double lds_d[WAVES];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+	const long row = blockIdx.y;
+	const int c0 = blockIdx.x * width, c1 = min(a.cols, c0 + width);
+	const float *zr = a.z_re + row * a.ldz, *zi = a.z_im + row * a.ldz;
+	double sum = 0.0;
+#pragma unroll 8
+	for (int c = c0 + t; c < c1; c += TPB) sum = fma((double) zi[c], (double) zi[c], fma((double) zr[c], (double) zr[c], sum));
+	sum = group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane);
+	if (t == 0) part[row * gridDim.x + blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, const double *__restrict__ part, int width) {
+	extern __shared__ float lds[];
+	__shared__ double lds_d[WAVES];
+	__shared__ float2 lds_f[WAVES];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+	const long row = blockIdx.y;
+	const int c0 = blockIdx.x * width, c1 = min(a.cols, c0 + width);
+	const Entries e = entries_at(lds, a.top);
+	fetch_entries<TPB>(a, e, row, t);
+	float S;
+	if (a.loss) {
+		double sum = 0.0;
+		for (int k = t; k < (int) gridDim.x; k += TPB) sum += part[row * gridDim.x + k];
+		S = clamped((float) group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane));
+	} else {
+		S = a.s[row];
+	}
+	__syncthreads();
+	float2 sums;
+	entry_sums<TPB>(a, e, S, t, sums.x, sums.y);
+	sums = group_reduce<float2, WAVES>(sums, SumF2(), lds_f, 0, wave, lane);
+	if (a.loss && t == 0 && blockIdx.x == 0) {
+		a.s[row] = S;
+		a.loss[row] = sums.x;
+	}
+	if (!a.dz_re) return;
+	const float share = sums.y / S;
+	const float *zr = a.z_re + row * a.ldz, *zi = a.z_im + row * a.ldz;
+#pragma unroll 4
+	for (int c = c0 + t; c < c1; c += TPB) distill_store(a, row, c, zr[c] * share, -(zi[c] * share));
+	__syncthreads();
+	entry_gradients<TPB>(a, e, row, S, sums.y, t, c0, c1);
 }
 
 // ------------------------------------------------------------------------------------------------ vocabulary head
@@ -598,9 +733,51 @@ __global__ __launch_bounds__(TPB) void head_clear_kernel(float *p, long ld, int 
 
 using namespace cnet;
 
-template <bool FWD, bool BWD>
+// loss == NULL: the backward pass alone, dz_re == NULL: the forward pass alone
 static int distill(const DistillArgs &a) {
-	hipLaunchKernelGGL((distill_kernel<FWD, BWD>), dim3((unsigned) a.rows), dim3(TPB), 0, rt().stream, a);
+	const bool vec = a.ldz % 4 == 0 && aligned16(a.z_re) && aligned16(a.z_im) && (!a.dz_re || a.lddz % 4 == 0) && aligned16(a.dz_re) &&
+			aligned16(a.dz_im) && aligned16(a.dzs_re) && aligned16(a.dzs_im);
+	const size_t entries = (size_t) 4 * a.top * sizeof(float);
+	const int cus = rt().prop.multiProcessorCount;
+	// a workgroup holds a row of up to 32768 columns; a longer one, and one of more than 8192 where there are fewer rows than a
+	// quarter of the compute units, is dealt out
+	if (a.cols > 32768 || (a.cols > 8192 && 4 * a.rows < cus)) {
+		const int want = std::max(1, std::min((a.cols + 2047) / 2048, 4 * cus / std::min(a.rows, 4 * cus)));
+		const int width = (a.cols + want - 1) / want, slabs = (a.cols + width - 1) / width;
+		for (int r0 = 0; r0 < a.rows; r0 += 65535) {  // (rows on the y axis of the grid)
+			DistillArgs p = a;
+			p.rows = std::min(a.rows - r0, 65535);
+			p.z_re += (long) r0 * a.ldz, p.z_im += (long) r0 * a.ldz;
+			p.ids += (long) r0 * a.top, p.probs += (long) r0 * a.top;
+			p.s += r0;
+			if (p.loss) p.loss += r0;
+			if (p.dz_re) p.dz_re += (long) r0 * a.lddz, p.dz_im += (long) r0 * a.lddz;
+			if (p.dzs_re) p.dzs_re += (long) r0 * a.lddz, p.dzs_im += (long) r0 * a.lddz;
+			double *part = (double *) workspace((size_t) p.rows * slabs * sizeof(double));
+			if (!part) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
+			const dim3 grid((unsigned) slabs, (unsigned) p.rows);
+			if (p.loss) hipLaunchKernelGGL(distill_slab_sum_kernel, grid, dim3(TPB), 0, rt().stream, p, part, width);
+			hipLaunchKernelGGL(distill_slab_kernel, grid, dim3(TPB), entries, rt().stream, p, part, width);
+			CNET_LAUNCH_CHECK();
+		}
+		return CNET_OK;
+	}
+	// (8192 x 32768, read once and written once: 772 us with the streaming hint on both sides, 801 on the stores, 862 on the loads, 824
+	// with none; 5.6 TB/s)
+	const int policy = stream_policy(a.dz_re ? ST_BOTH : ST_LOADS, !a.dz_re ? 2 : a.dzs_re ? 6 : 4, (long) a.rows * a.cols);
+#define CNET_DISTILL(T, E)                                                                                                                     \
+	do {                                                                                                                                       \
+		const dim3 grid((unsigned) ((a.rows + (T < TPB ? TPB / T : 1) - 1) / (T < TPB ? TPB / T : 1))), block(T < TPB ? TPB : T);                \
+		if (vec) hipLaunchKernelGGL((distill_kernel<T, E / 4, 4>), grid, block, entries * (T < TPB ? TPB / T : 1), rt().stream, a, policy);       \
+		else hipLaunchKernelGGL((distill_kernel<T, E, 1>), grid, block, entries * (T < TPB ? TPB / T : 1), rt().stream, a, policy);               \
+	} while (0)
+	if (a.cols <= 512 && a.top <= 64) CNET_DISTILL(64, 8);
+	else if (a.cols <= 2048) CNET_DISTILL(256, 8);
+	else if (a.cols <= 4096) CNET_DISTILL(256, 16);
+	else if (a.cols <= 8192) CNET_DISTILL(256, 32);
+	else if (a.cols <= 16384) CNET_DISTILL(1024, 16);
+	else CNET_DISTILL(1024, 32);
+#undef CNET_DISTILL
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
@@ -849,7 +1026,7 @@ int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const in
 	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 24) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && loss && ldz >= cols);
-	return distill<true, false>(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, s, loss, nullptr, nullptr, nullptr, nullptr, 0, rows, cols});
+	return distill(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, s, loss, nullptr, nullptr, nullptr, nullptr, 0, rows, cols});
 }
 
 int cnet_distill_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, const float *s, const int32_t *ids, const float *probs, int top,
@@ -859,7 +1036,7 @@ int cnet_distill_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, cons
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && ldz >= cols);
 	CNET_CHECK_ARG(dz_dz_re && dz_dz_im && ((dz_dzs_re == nullptr) == (dz_dzs_im == nullptr)) && lddz >= cols);
-	return distill<false, true>(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, const_cast<float *>(s), nullptr, dz_dz_re, dz_dz_im, dz_dzs_re,
+	return distill(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, const_cast<float *>(s), nullptr, dz_dz_re, dz_dz_im, dz_dzs_re,
 			dz_dzs_im, (long) lddz, rows, cols});
 }
 
@@ -870,7 +1047,7 @@ int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, 
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && loss && ldz >= cols);
 	CNET_CHECK_ARG(dz_dz_re && dz_dz_im && ((dz_dzs_re == nullptr) == (dz_dzs_im == nullptr)) && lddz >= cols);
-	return distill<true, true>(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, s, loss, dz_dz_re, dz_dz_im, dz_dzs_re, dz_dzs_im, (long) lddz, rows,
+	return distill(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, s, loss, dz_dz_re, dz_dz_im, dz_dzs_re, dz_dzs_im, (long) lddz, rows,
 			cols});
 }
 
