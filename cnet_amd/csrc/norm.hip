@@ -56,23 +56,26 @@ __device__ __forceinline__ float inv_rms(float sum, int cols, float eps) {
 
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
 
-// V consecutive columns from c on; what lies behind the row's end reads as zero and is not written
+// V consecutive columns from c on (V = 4: the row is a multiple of four).  A thread beyond the row's end gets the row's last columns:
+// the load has no branch around it, behind which everything already on its way would have to be waited for (16384 x 128 backward:
+// 58 us so, 32 without), and whoever uses the values for a sum masks them there, when they have arrived.
 template <int V>
 __device__ __forceinline__ void load_cols(float *v, const float *p, int c, int cols, int policy = 0) {
-	if (V == 4 && c + V <= cols) {
-		const float4 x = ld4(p + c, policy);
+	const int at = min(c, cols - V);
+	if (V == 4) {
+		const float4 x = ld4(p + at, policy);
 		v[0] = x.x;
 		v[1 % V] = x.y;
 		v[2 % V] = x.z;
 		v[3 % V] = x.w;
 	} else {
-#pragma unroll
-		for (int k = 0; k < V; ++k) v[k] = c + k < cols ? p[c + k] : 0.f;
+		v[0] = p[at];
 	}
 }
 template <int V>
 __device__ __forceinline__ void store_cols(float *p, const float *v, int c, int cols, int accumulate, int policy) {
-	if (V == 4 && c + V <= cols) {
+	if (c >= cols) return;
+	if (V == 4) {
 		float4 x = make_float4(v[0], v[1 % V], v[2 % V], v[3 % V]);
 		if (accumulate) {
 			const float4 o = *reinterpret_cast<const float4 *>(p + c);
@@ -80,9 +83,7 @@ __device__ __forceinline__ void store_cols(float *p, const float *v, int c, int 
 		}
 		st4(p + c, x, policy);
 	} else {
-#pragma unroll
-		for (int k = 0; k < V; ++k)
-			if (c + k < cols) put(p + c + k, v[k], accumulate);
+		put(p + c, v[0], accumulate);
 	}
 }
 // a gradient (dz) into its planes, and its conjugate where the dz* half is wanted
@@ -125,9 +126,14 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdAr
 	}
 	float sum = 0.f;
 #pragma unroll
-	for (int k = 0; k < NIT; ++k)
+	for (int k = 0; k < NIT; ++k) {
+		const bool in = (k * T + t) * V < a.cols;
 #pragma unroll
-		for (int q = 0; q < V; ++q) sum += x_r[k][q] * x_r[k][q] + x_i[k][q] * x_i[k][q];
+		for (int q = 0; q < V; ++q) {
+			const float d = x_r[k][q] * x_r[k][q] + x_i[k][q] * x_i[k][q];
+			sum += in ? d : 0.f;
+		}
+	}
 	sum = group_reduce<float, G>(sum, SumF(), lds, slot, wave, lane);
 	const float s = inv_rms(sum, a.cols, a.eps);
 	if (t == 0 && live && a.s) a.s[row] = s;
@@ -145,7 +151,8 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdAr
 			if (JOIN) {
 				y_r = u_r[k][q] + a.scale * y_r;
 				y_i = u_i[k][q] + a.scale * y_i;
-				sum2 += y_r * y_r + y_i * y_i;
+				const float d = y_r * y_r + y_i * y_i;
+				sum2 += c < a.cols ? d : 0.f;
 			}
 			x_r[k][q] = y_r;
 			x_i[k][q] = y_i;
@@ -189,11 +196,12 @@ struct Sum3Op {
 // One exchange per row: with e = gh + s2 p (p = g w) and z = v n1, t2 = mean Re(p n2) and the mean of Re(dh z), which is
 // Re(e z) - s2 t2 Re(conj(n2) z), come from three sums that do not wait for each other.
 // SECOND: the next block's norm takes part (the join with a gradient at y).
-template <int T, int NIT, int V, bool SECOND>
+// KEEP: the weights stay in registers, and the next row's operands are requested before the exchange of this one.
+template <int T, int NIT, int V, bool SECOND, bool KEEP>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdArgs a, const int policy) {
 	constexpr int G = T / 64, R = T < TPB ? TPB / T : 1, NP = SECOND ? 4 : 2;
 	__shared__ Sum3 lds[R * G];
-	extern __shared__ float sums[];  // [R - 1][NP][cols]
+	extern __shared__ __align__(16) float sums[];  // [R - 1][NP][NIT][T][V]
 	const int group = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
 	const int r0 = blockIdx.x * a.rows_per_slab, r1 = min(a.rows, r0 + a.rows_per_slab);
 	const bool shared = a.v.ld == 0;
@@ -205,12 +213,19 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 		for (int k = 0; k < NIT; ++k)
 #pragma unroll
 			for (int q = 0; q < V; ++q) acc[p][k][q] = 0.f;
-	// (every group makes the same number of rounds: the exchange is the whole workgroup's; a round beyond the rows stores nothing)
-	for (int base = r0; base < r1; base += R) {
-		const bool live = base + group < r1;
-		const long row = live ? base + group : r1 - 1;
-		const float s = a.s[row], s2 = SECOND ? a.s2[row] : 0.f;
-		float x_r[NIT][V], x_i[NIT][V], e_r[NIT][V], e_i[NIT][V], h_r[NIT][V], h_i[NIT][V], g_r[NIT][V], g_i[NIT][V], v_r[NIT][V], v_i[NIT][V];
+	float x_r[NIT][V], x_i[NIT][V], e_r[NIT][V], e_i[NIT][V], h_r[NIT][V], h_i[NIT][V], g_r[NIT][V], g_i[NIT][V];
+	float v_r[NIT][V], v_i[NIT][V], w_r[NIT][V], w_i[NIT][V];
+	float s, s2;
+	auto fetch_gate = [&](long row) {
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			load_cols<V>(v_r[k], a.v.re + row * a.v.ld, (k * T + t) * V, a.cols);
+			load_cols<V>(v_i[k], a.v.im + row * a.v.ld, (k * T + t) * V, a.cols);
+		}
+	};
+	auto fetch = [&](long row) {
+		s = a.s[row];
+		s2 = SECOND ? a.s2[row] : 0.f;
 #pragma unroll
 		for (int k = 0; k < NIT; ++k) {
 			const int c = (k * T + t) * V;
@@ -229,39 +244,57 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 				load_cols<V>(g_r[k], a.g.re + row * a.g.ld, c, a.cols, policy);
 				load_cols<V>(g_i[k], a.g.im + row * a.g.ld, c, a.cols, policy);
 			}
-			load_cols<V>(v_r[k], a.v.re + row * a.v.ld, c, a.cols);
-			load_cols<V>(v_i[k], a.v.im + row * a.v.ld, c, a.cols);
 		}
-		Sum3 m = {0.f, 0.f, 0.f};
+	};
+	auto fetch_weights = [&]() {
 #pragma unroll
 		for (int k = 0; k < NIT; ++k) {
-			const int c = (k * T + t) * V;
-			float w_r[V], w_i[V];
-			if (SECOND) {
-				load_cols<V>(w_r, a.w.re, c, a.cols);
-				load_cols<V>(w_i, a.w.im, c, a.cols);
-			}
+			load_cols<V>(w_r[k], a.w.re, (k * T + t) * V, a.cols);
+			load_cols<V>(w_i[k], a.w.im, (k * T + t) * V, a.cols);
+		}
+	};
+	if (SECOND && KEEP) fetch_weights();
+	if (shared && KEEP) fetch_gate(0);
+	if (KEEP) fetch(min(r0 + group, r1 - 1));
+	// (every group makes the same number of rounds: the exchange is the whole workgroup's; a round beyond the rows stores nothing)
+	for (int base = r0; base < r1; base += R) {
+		const bool live = base + group < r1;
+		const long row = live ? base + group : r1 - 1;
+		if (!KEEP) fetch(row);
+		if (!shared || !KEEP) fetch_gate(row);
+		if (SECOND && !KEEP) fetch_weights();
+		Sum3 m = {0.f, 0.f, 0.f};
+		// what the row's second half needs, out of the way of the next row's operands: n1, e, n2, g
+		float n_r[NIT][V], n_i[NIT][V], f_r[NIT][V], f_i[NIT][V], k_r[NIT][V], k_i[NIT][V], y_r[NIT][V], y_i[NIT][V];
+		const float s_row = s;
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			const bool in = (k * T + t) * V < a.cols;  // (beyond the row n1 and n2 are zero, and with them every sum)
 #pragma unroll
 			for (int q = 0; q < V; ++q) {
-				const float n_r = x_r[k][q] * s, n_i = x_i[k][q] * s;
-				x_r[k][q] = n_r;
-				x_i[k][q] = n_i;
-				const float z_r = v_r[k][q] * n_r - v_i[k][q] * n_i, z_i = v_r[k][q] * n_i + v_i[k][q] * n_r;
+				n_r[k][q] = in ? x_r[k][q] * s : 0.f;
+				n_i[k][q] = in ? x_i[k][q] * s : 0.f;
+				f_r[k][q] = e_r[k][q];
+				f_i[k][q] = e_i[k][q];
+				const float z_r = v_r[k][q] * n_r[k][q] - v_i[k][q] * n_i[k][q], z_i = v_r[k][q] * n_i[k][q] + v_i[k][q] * n_r[k][q];
 				if (SECOND) {
-					const float p_r = g_r[k][q] * w_r[q] - g_i[k][q] * w_i[q], p_i = g_r[k][q] * w_i[q] + g_i[k][q] * w_r[q];
-					const float k_r = h_r[k][q] * s2, k_i = h_i[k][q] * s2;
-					h_r[k][q] = k_r;
-					h_i[k][q] = k_i;
-					m.b += p_r * k_r - p_i * k_i;
-					m.c += k_r * z_r + k_i * z_i;
-					e_r[k][q] += s2 * p_r;
-					e_i[k][q] += s2 * p_i;
+					y_r[k][q] = g_r[k][q];
+					y_i[k][q] = g_i[k][q];
+					k_r[k][q] = in ? h_r[k][q] * s2 : 0.f;
+					k_i[k][q] = in ? h_i[k][q] * s2 : 0.f;
+					const float p_r = y_r[k][q] * w_r[k][q] - y_i[k][q] * w_i[k][q], p_i = y_r[k][q] * w_i[k][q] + y_i[k][q] * w_r[k][q];
+					m.b += p_r * k_r[k][q] - p_i * k_i[k][q];
+					m.c += k_r[k][q] * z_r + k_i[k][q] * z_i;
+					f_r[k][q] += s2 * p_r;
+					f_i[k][q] += s2 * p_i;
 				}
-				m.a += e_r[k][q] * z_r - e_i[k][q] * z_i;
+				m.a += f_r[k][q] * z_r - f_i[k][q] * z_i;
 			}
 		}
+		const float s2_row = s2;
+		if (KEEP && base + R < r1) fetch(min(base + R + group, r1 - 1));
 		m = group_reduce<Sum3, G>(m, Sum3Op(), lds, group, wave, lane);
-		const float t2 = m.b * inv_n * s2, t1 = a.scale * (m.a - t2 * m.c) * inv_n;
+		const float t2 = m.b * inv_n * s2_row, t1 = a.scale * (m.a - t2 * m.c) * inv_n;
 		if (!live) continue;
 #pragma unroll
 		for (int k = 0; k < NIT; ++k) {
@@ -269,27 +302,29 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 			float o_r[V], o_i[V], d_r[V], d_i[V];
 #pragma unroll
 			for (int q = 0; q < V; ++q) {
-				d_r[q] = e_r[k][q];
-				d_i[q] = e_i[k][q];
+				d_r[q] = f_r[k][q];
+				d_i[q] = f_i[k][q];
 				if (SECOND) {
-					d_r[q] -= h_r[k][q] * t2;
-					d_i[q] += h_i[k][q] * t2;
-					acc[2 % NP][k][q] += g_r[k][q] * h_r[k][q] - g_i[k][q] * h_i[k][q];
-					acc[3 % NP][k][q] += g_r[k][q] * h_i[k][q] + g_i[k][q] * h_r[k][q];
+					d_r[q] -= k_r[k][q] * t2;
+					d_i[q] += k_i[k][q] * t2;
 				}
-				e_r[k][q] = a.scale * d_r[q];
-				e_i[k][q] = a.scale * d_i[q];
-				o_r[q] = s * (e_r[k][q] * v_r[k][q] - e_i[k][q] * v_i[k][q] - x_r[k][q] * t1);
-				o_i[q] = s * (e_r[k][q] * v_i[k][q] + e_i[k][q] * v_r[k][q] + x_i[k][q] * t1);
+				f_r[k][q] = a.scale * d_r[q];
+				f_i[k][q] = a.scale * d_i[q];
+				o_r[q] = s_row * (f_r[k][q] * v_r[k][q] - f_i[k][q] * v_i[k][q] - n_r[k][q] * t1);
+				o_i[q] = s_row * (f_r[k][q] * v_i[k][q] + f_i[k][q] * v_r[k][q] + n_i[k][q] * t1);
 			}
 			if (a.du.re) store_grad<V>(a.du, row, d_r, d_i, c, a.cols, a.accumulate, policy);
 			store_grad<V>(a.dx, row, o_r, o_i, c, a.cols, a.accumulate, policy);
 #pragma unroll
 			for (int q = 0; q < V; ++q) {
-				d_r[q] = e_r[k][q] * x_r[k][q] - e_i[k][q] * x_i[k][q];
-				d_i[q] = e_r[k][q] * x_i[k][q] + e_i[k][q] * x_r[k][q];
+				d_r[q] = f_r[k][q] * n_r[k][q] - f_i[k][q] * n_i[k][q];
+				d_i[q] = f_r[k][q] * n_i[k][q] + f_i[k][q] * n_r[k][q];
 				acc[0][k][q] += d_r[q];
 				acc[1][k][q] += d_i[q];
+				if (SECOND) {
+					acc[2 % NP][k][q] += y_r[k][q] * k_r[k][q] - y_i[k][q] * k_i[k][q];
+					acc[3 % NP][k][q] += y_r[k][q] * k_i[k][q] + y_i[k][q] * k_r[k][q];
+				}
 			}
 			if (!shared) store_grad<V>(a.dv, row, d_r, d_i, c, a.cols, a.accumulate_w, policy);
 		}
@@ -299,7 +334,7 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 #pragma unroll
 		for (int p = 0; p < NP; ++p)
 #pragma unroll
-			for (int k = 0; k < NIT; ++k) store_cols<V>(sums + ((group - 1) * NP + p) * (T * NIT * V), acc[p][k], (k * T + t) * V, T * NIT * V, 0, 0);
+			for (int k = 0; k < NIT; ++k) store_cols<V>(sums + (((group - 1) * NP + p) * NIT + k) * (T * V) + t * V, acc[p][k], 0, V, 0, 0);
 	}
 	if (R > 1) __syncthreads();
 	if (group > 0) return;
@@ -312,7 +347,7 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 			const int c = (k * T + t) * V;
 			for (int r = 1; r < R; ++r) {
 				float more[V];
-				load_cols<V>(more, sums + ((r - 1) * NP + p) * (T * NIT * V), c, T * NIT * V);
+				load_cols<V>(more, sums + (((r - 1) * NP + p) * NIT + k) * (T * V) + t * V, 0, V);
 #pragma unroll
 				for (int q = 0; q < V; ++q) acc[p][k][q] += more[q];
 			}
@@ -321,6 +356,125 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 			for (int q = 0; q < V; ++q)
 				if (c + q < a.cols) dst[c + q] = acc[p][k][q];
 		}
+	}
+}
+
+// Rows whose operands do not fit in registers, up to T x V x NIT columns: the same sums, then the operands once more (from the caches:
+// a row of 8192 columns is half a megabyte), of which a thread keeps only its columns' sums over the rows.
+template <int T, int NIT, int V, bool SECOND>
+__global__ __launch_bounds__(T) void norm_bwd_twice_kernel(const BwdArgs a) {
+	constexpr int G = T / 64, NP = SECOND ? 4 : 2;
+	__shared__ Sum3 lds[G];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+	const int r0 = blockIdx.x * a.rows_per_slab, r1 = min(a.rows, r0 + a.rows_per_slab);
+	const bool shared = a.v.ld == 0;
+	float acc[NP][NIT][V];
+#pragma unroll
+	for (int p = 0; p < NP; ++p)
+#pragma unroll
+		for (int k = 0; k < NIT; ++k)
+#pragma unroll
+			for (int q = 0; q < V; ++q) acc[p][k][q] = 0.f;
+	for (long row = r0; row < r1; ++row) {
+		const float s = a.s[row], s2 = SECOND ? a.s2[row] : 0.f;
+		float n_r[V], n_i[V], f_r[V], f_i[V], v_r[V], v_i[V], k_r[V], k_i[V], y_r[V], y_i[V], p_r[V], p_i[V];
+		// one thread's columns from c on: n1, e without its share of t2, v and, SECOND, n2, g and p
+		auto fetch = [&](int c) {
+			load_cols<V>(n_r, a.x.re + row * a.x.ld, c, a.cols);
+			load_cols<V>(n_i, a.x.im + row * a.x.ld, c, a.cols);
+			load_cols<V>(v_r, a.v.re + row * a.v.ld, c, a.cols);
+			load_cols<V>(v_i, a.v.im + row * a.v.ld, c, a.cols);
+#pragma unroll
+			for (int q = 0; q < V; ++q) f_r[q] = f_i[q] = 0.f;
+			if (a.gh.re) {
+				load_cols<V>(f_r, a.gh.re + row * a.gh.ld, c, a.cols);
+				load_cols<V>(f_i, a.gh.im + row * a.gh.ld, c, a.cols);
+			}
+			if (SECOND) {
+				load_cols<V>(k_r, a.h.re + row * a.h.ld, c, a.cols);
+				load_cols<V>(k_i, a.h.im + row * a.h.ld, c, a.cols);
+				load_cols<V>(y_r, a.g.re + row * a.g.ld, c, a.cols);
+				load_cols<V>(y_i, a.g.im + row * a.g.ld, c, a.cols);
+				load_cols<V>(p_r, a.w.re, c, a.cols);
+				load_cols<V>(p_i, a.w.im, c, a.cols);
+			}
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				n_r[q] = c < a.cols ? n_r[q] * s : 0.f;
+				n_i[q] = c < a.cols ? n_i[q] * s : 0.f;
+				if (SECOND) {
+					k_r[q] = c < a.cols ? k_r[q] * s2 : 0.f;
+					k_i[q] = c < a.cols ? k_i[q] * s2 : 0.f;
+					const float w_r = p_r[q], w_i = p_i[q];
+					p_r[q] = y_r[q] * w_r - y_i[q] * w_i;
+					p_i[q] = y_r[q] * w_i + y_i[q] * w_r;
+					f_r[q] += s2 * p_r[q];
+					f_i[q] += s2 * p_i[q];
+				}
+			}
+		};
+		Sum3 m = {0.f, 0.f, 0.f};
+#pragma unroll 1
+		for (int k = 0; k < NIT; ++k) {
+			if (k * T * V >= a.cols) break;
+			fetch((k * T + t) * V);
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				const float z_r = v_r[q] * n_r[q] - v_i[q] * n_i[q], z_i = v_r[q] * n_i[q] + v_i[q] * n_r[q];
+				if (SECOND) {
+					m.b += p_r[q] * k_r[q] - p_i[q] * k_i[q];
+					m.c += k_r[q] * z_r + k_i[q] * z_i;
+				}
+				m.a += f_r[q] * z_r - f_i[q] * z_i;
+			}
+		}
+		m = group_reduce<Sum3, G>(m, Sum3Op(), lds, 0, wave, lane);
+		const float inv_n = 1.0f / (float) a.cols, t2 = m.b * inv_n * s2, t1 = a.scale * (m.a - t2 * m.c) * inv_n;
+#pragma unroll
+		for (int k = 0; k < NIT; ++k) {
+			if (k * T * V >= a.cols) break;
+			const int c = (k * T + t) * V;
+			fetch(c);
+			float o_r[V], o_i[V], d_r[V], d_i[V];
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				d_r[q] = f_r[q];
+				d_i[q] = f_i[q];
+				if (SECOND) {
+					d_r[q] -= k_r[q] * t2;
+					d_i[q] += k_i[q] * t2;
+					acc[2 % NP][k][q] += y_r[q] * k_r[q] - y_i[q] * k_i[q];
+					acc[3 % NP][k][q] += y_r[q] * k_i[q] + y_i[q] * k_r[q];
+				}
+				f_r[q] = a.scale * d_r[q];
+				f_i[q] = a.scale * d_i[q];
+				o_r[q] = s * (f_r[q] * v_r[q] - f_i[q] * v_i[q] - n_r[q] * t1);
+				o_i[q] = s * (f_r[q] * v_i[q] + f_i[q] * v_r[q] + n_i[q] * t1);
+			}
+			if (a.du.re) store_grad<V>(a.du, row, d_r, d_i, c, a.cols, a.accumulate, 0);
+			store_grad<V>(a.dx, row, o_r, o_i, c, a.cols, a.accumulate, 0);
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				d_r[q] = f_r[q] * n_r[q] - f_i[q] * n_i[q];
+				d_i[q] = f_r[q] * n_i[q] + f_i[q] * n_r[q];
+				acc[0][k][q] += d_r[q];
+				acc[1][k][q] += d_i[q];
+			}
+			if (!shared) store_grad<V>(a.dv, row, d_r, d_i, c, a.cols, a.accumulate_w, 0);
+		}
+	}
+	if (!a.planes) return;
+	float *part = a.partial + (long) blockIdx.x * a.planes * a.cols;
+#pragma unroll
+	for (int p = 0; p < NP; ++p) {
+		if (p < 2 && !shared) continue;
+#pragma unroll
+		for (int k = 0; k < NIT; ++k)
+#pragma unroll
+			for (int q = 0; q < V; ++q) {
+				const int c = (k * T + t) * V + q;
+				if (c < a.cols) part[(long) (shared ? p : p - 2) * a.cols + c] = acc[p][k][q];
+			}
 	}
 }
 
@@ -523,7 +677,7 @@ static bool vec_ok(const Planes &p) { return p.ld % 4 == 0 && aligned16(p.re) &&
 static bool vec_ok(const Out4 &o) { return o.ld % 4 == 0 && aligned16(o.re) && aligned16(o.im) && aligned16(o.sre) && aligned16(o.sim); }
 
 static int norm_fwd(const FwdArgs &a, bool join) {
-	const bool vec = vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.u) && vec_ok(a.w) && vec_ok(Planes{a.y_re, a.y_im, a.ldy}) &&
+	const bool vec = a.cols % 4 == 0 && vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.u) && vec_ok(a.w) && vec_ok(Planes{a.y_re, a.y_im, a.ldy}) &&
 			vec_ok(Planes{a.h_re, a.h_im, a.ldh});
 	const int policy = stream_policy(ST_STORES, join ? 8 : 4, (long) a.rows * a.cols);
 	if (a.cols <= 256) launch_fwd<64, 4>(a, join, vec, policy);
@@ -544,10 +698,10 @@ static void launch_bwd(const BwdArgs &a, bool second, bool vec, int nslabs, int 
 	constexpr int R = T < TPB ? TPB / T : 1;
 	const dim3 grid((unsigned) nslabs), block(T < TPB ? TPB : T);
 	const size_t lds = (size_t) (R - 1) * (second ? 4 : 2) * T * E * sizeof(float);
-	if (second && vec) hipLaunchKernelGGL((norm_bwd_kernel<T, E / 4, 4, true>), grid, block, lds, rt().stream, a, policy);
-	else if (second) hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, true>), grid, block, lds, rt().stream, a, policy);
-	else if (vec) hipLaunchKernelGGL((norm_bwd_kernel<T, E / 4, 4, false>), grid, block, lds, rt().stream, a, policy);
-	else hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, false>), grid, block, lds, rt().stream, a, policy);
+	if (second && vec) hipLaunchKernelGGL((norm_bwd_kernel<T, E / 4, 4, true, true>), grid, block, lds, rt().stream, a, policy);
+	else if (second) hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, true, true>), grid, block, lds, rt().stream, a, policy);
+	else if (vec) hipLaunchKernelGGL((norm_bwd_kernel<T, E / 4, 4, false, true>), grid, block, lds, rt().stream, a, policy);
+	else hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, false, true>), grid, block, lds, rt().stream, a, policy);
 }
 
 // The gate alone is the join without a second norm, without a residual path to hand its gradient to, and with scale 1: its gradient
@@ -555,11 +709,11 @@ static void launch_bwd(const BwdArgs &a, bool second, bool vec, int nslabs, int 
 static int norm_bwd(BwdArgs &a, const Out4 &dv, const Out4 &dw) {
 	const bool shared = a.v.ld == 0, second = a.g.re != nullptr;
 	a.planes = (shared ? 2 : 0) + (second ? 2 : 0);
-	const bool vec = vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.h) && vec_ok(a.w) && vec_ok(a.g) && vec_ok(a.gh) && vec_ok(a.du) && vec_ok(a.dx) && vec_ok(a.dv);
-	// Two or three workgroups to a compute unit, each with as many rows: a workgroup's sums are written and read again, which more of
-	// them would do more often.
-	const int groups = a.cols <= 512 ? 4 : a.cols <= 1024 ? 2 : 1;  // rows that a workgroup works on at a time
-	const int want = std::max(1, std::min((a.rows + groups - 1) / groups, 3 * rt().prop.multiProcessorCount));
+	const bool vec = a.cols % 4 == 0 && vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.h) && vec_ok(a.w) && vec_ok(a.g) && vec_ok(a.gh) && vec_ok(a.du) && vec_ok(a.dx) && vec_ok(a.dv);
+	// Two workgroups to a compute unit, all with as many rows: a workgroup's sums are written and read again, which more of them
+	// would do more often (8192 x 1024: 81 us with 512 workgroups, 89 with 768, 93 with 1024).
+	const int groups = a.cols <= 256 ? 4 : a.cols <= 512 ? 2 : 1;  // rows that a workgroup works on at a time
+	const int want = std::max(1, std::min((a.rows + groups - 1) / groups, 2 * rt().prop.multiProcessorCount));
 	a.rows_per_slab = (a.rows + want - 1) / want;
 	const int nslabs = (a.rows + a.rows_per_slab - 1) / a.rows_per_slab;
 	if (a.planes) {
@@ -567,10 +721,16 @@ static int norm_bwd(BwdArgs &a, const Out4 &dv, const Out4 &dw) {
 		if (!a.partial) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
 	}
 	const int policy = stream_policy(ST_LOADS, second ? 12 : 6, (long) a.rows * a.cols);
-	if (a.cols <= 512) launch_bwd<64, 8>(a, second, vec, nslabs, policy);
-	else if (a.cols <= 1024) launch_bwd<128, 8>(a, second, vec, nslabs, policy);
-	else if (a.cols <= 2048) launch_bwd<256, 8>(a, second, vec, nslabs, policy);
-	else if (a.cols <= 4096) launch_bwd<512, 8>(a, second, vec, nslabs, policy);
+	if (a.cols <= 256) launch_bwd<64, 4>(a, second, vec, nslabs, policy);
+	else if (a.cols <= 512) launch_bwd<128, 4>(a, second, vec, nslabs, policy);
+	else if (a.cols <= 1024) launch_bwd<256, 4>(a, second, vec, nslabs, policy);
+	else if (a.cols <= 2048) launch_bwd<512, 4>(a, second, vec, nslabs, policy);
+	else if (a.cols <= 4096 && vec && second) hipLaunchKernelGGL((norm_bwd_kernel<512, 2, 4, true, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a, policy);
+	else if (a.cols <= 4096 && vec) hipLaunchKernelGGL((norm_bwd_kernel<512, 2, 4, false, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a, policy);
+	else if (a.cols <= 8192 && vec && second) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 4, 4, true>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
+	else if (a.cols <= 8192 && vec) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 4, 4, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
+	else if (a.cols <= 8192 && second) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 16, 1, true>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
+	else if (a.cols <= 8192) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 16, 1, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
 	else if (second) hipLaunchKernelGGL(norm_bwd_wide_kernel<true>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
 	else hipLaunchKernelGGL(norm_bwd_wide_kernel<false>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
 	CNET_LAUNCH_CHECK();

@@ -148,25 +148,17 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 	float re[NIT][V], im[NIT][V];
 #pragma unroll
 	for (int k = 0; k < NIT; ++k) {
-		const int c = (k * T + t) * V;
-#pragma unroll
-		for (int q = 0; q < V; ++q) re[k][q] = im[k][q] = 0.f;
-		if (c + V <= a.cols) {
-			if (V == 4) {
-				const float4 x = ld4(zr + c, policy), y = ld4(zi + c, policy);
-				re[k][0] = x.x, re[k][1 % V] = x.y, re[k][2 % V] = x.z, re[k][3 % V] = x.w;
-				im[k][0] = y.x, im[k][1 % V] = y.y, im[k][2 % V] = y.z, im[k][3 % V] = y.w;
-			} else {
-				re[k][0] = zr[c];
-				im[k][0] = zi[c];
-			}
-		} else if (V > 1) {
-#pragma unroll
-			for (int q = 0; q < V; ++q)
-				if (c + q < a.cols) {
-					re[k][q] = zr[c + q];
-					im[k][q] = zi[c + q];
-				}
+		// (no branch around the loads: a column of the row is read in any case and the result chosen afterwards)
+		const int c = (k * T + t) * V, at = min(c, a.cols - V);
+		const bool in = c < a.cols;
+		if (V == 4) {
+			const float4 x = ld4(zr + at, policy), y = ld4(zi + at, policy);
+			re[k][0] = in ? x.x : 0.f, re[k][1 % V] = in ? x.y : 0.f, re[k][2 % V] = in ? x.z : 0.f, re[k][3 % V] = in ? x.w : 0.f;
+			im[k][0] = in ? y.x : 0.f, im[k][1 % V] = in ? y.y : 0.f, im[k][2 % V] = in ? y.z : 0.f, im[k][3 % V] = in ? y.w : 0.f;
+		} else {
+			const float x = zr[at], y = zi[at];
+			re[k][0] = in ? x : 0.f;
+			im[k][0] = in ? y : 0.f;
 		}
 	}
 	fetch_entries<T>(a, e, row, t);
@@ -196,7 +188,8 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 #pragma unroll
 		for (int k = 0; k < NIT; ++k) {
 			const int c = (k * T + t) * V;
-			if (V == 4 && c + V <= a.cols) {
+			if (c >= a.cols) continue;
+			if (V == 4) {
 				const long o = row * a.lddz + c;
 				const float4 u = make_float4(re[k][0] * share, re[k][1 % V] * share, re[k][2 % V] * share, re[k][3 % V] * share);
 				const float4 v = make_float4(im[k][0] * share, im[k][1 % V] * share, im[k][2 % V] * share, im[k][3 % V] * share);
@@ -208,9 +201,7 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 					st4(a.dzs_im + o, v, policy);
 				}
 			} else {
-#pragma unroll
-				for (int q = 0; q < V; ++q)
-					if (c + q < a.cols) distill_store(a, row, c + q, re[k][q] * share, -(im[k][q] * share));
+				distill_store(a, row, c, re[k][0] * share, -(im[k][0] * share));
 			}
 		}
 	}
@@ -735,7 +726,7 @@ using namespace cnet;
 
 // loss == NULL: the backward pass alone, dz_re == NULL: the forward pass alone
 static int distill(const DistillArgs &a) {
-	const bool vec = a.ldz % 4 == 0 && aligned16(a.z_re) && aligned16(a.z_im) && (!a.dz_re || a.lddz % 4 == 0) && aligned16(a.dz_re) &&
+	const bool vec = a.cols % 4 == 0 && a.ldz % 4 == 0 && aligned16(a.z_re) && aligned16(a.z_im) && (!a.dz_re || a.lddz % 4 == 0) && aligned16(a.dz_re) &&
 			aligned16(a.dz_im) && aligned16(a.dzs_re) && aligned16(a.dzs_im);
 	const size_t entries = (size_t) 4 * a.top * sizeof(float);
 	const int cus = rt().prop.multiProcessorCount;
