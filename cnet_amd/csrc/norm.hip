@@ -710,10 +710,10 @@ static int norm_bwd(BwdArgs &a, const Out4 &dv, const Out4 &dw) {
 	const bool shared = a.v.ld == 0, second = a.g.re != nullptr;
 	a.planes = (shared ? 2 : 0) + (second ? 2 : 0);
 	const bool vec = a.cols % 4 == 0 && vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.h) && vec_ok(a.w) && vec_ok(a.g) && vec_ok(a.gh) && vec_ok(a.du) && vec_ok(a.dx) && vec_ok(a.dv);
-	// Two workgroups to a compute unit, all with as many rows: a workgroup's sums are written and read again, which more of them
-	// would do more often (8192 x 1024: 81 us with 512 workgroups, 89 with 768, 93 with 1024).
+	// Two workgroups to a compute unit, one of the wide ones, all with as many rows: a workgroup's sums are written and read again, which more of them
+	// would do more often (8192 x 1024: 81 us with 512 workgroups, 89 with 768, 93 with 1024; 1024 x 8192: 139 with 256, 154 with 512).
 	const int groups = a.cols <= 256 ? 4 : a.cols <= 512 ? 2 : 1;  // rows that a workgroup works on at a time
-	const int want = std::max(1, std::min((a.rows + groups - 1) / groups, 2 * rt().prop.multiProcessorCount));
+	const int want = std::max(1, std::min((a.rows + groups - 1) / groups, (a.cols > 1024 ? 1 : 2) * rt().prop.multiProcessorCount));
 	a.rows_per_slab = (a.rows + want - 1) / want;
 	const int nslabs = (a.rows + a.rows_per_slab - 1) / a.rows_per_slab;
 	if (a.planes) {

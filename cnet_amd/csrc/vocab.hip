@@ -537,6 +537,155 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__
 	}
 }
 
+// ---- A few rows against the whole vocabulary (the next tokens of a batch of sequences): w is read once, and nothing of the logits
+// leaves the registers.  A wavefront forms the logits of 16 entries for up to 16 MT rows with v_mfma_f32_16x16x4_f32, walking K
+// with both operands straight from memory in the layout of the matrix instruction: lane (r, q), r = lane % 16, q = lane / 16, holds
+// row r of x (entry r of w) at k = 16 g + 4 q + s for step s of group g, so a group is one 128-bit load per plane and DEPTH
+// groups are on their way.  No LDS on the way (x is small and comes from the caches), no barrier in the loop.
+// Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one).
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+struct ScoreTile {   // what a workgroup leaves for every row
+	double sum;
+	float best;
+	int index;
+};
+
+template <bool V4>
+__device__ __forceinline__ floatx4 load_group(const float *p) {
+	if (V4) return *reinterpret_cast<const floatx4 *>(p);
+	return floatx4{p[0], p[1], p[2], p[3]};
+}
+
+template <int MT, bool V4>
+__global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B, ScoreTile *__restrict__ part) {
+	constexpr int DEPTH = MT == 1 ? 4 : MT == 2 ? 3 : 2;
+	__shared__ ScoreTile met[WAVES][16 * MT];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, q = lane >> 4;
+	const int n0 = (blockIdx.x * WAVES + wave) * 16;
+	// lanes beyond the last entry or row read the last one again; their results are masked
+	const long entry = (long) min(n0 + r, a.N - 1) * a.ldw + 4 * q;
+	const float *w_re = a.w_re + entry, *w_im = a.w_im + entry;
+	long x_at[MT];
+#pragma unroll
+	for (int m = 0; m < MT; ++m) x_at[m] = (long) min(16 * m + r, B - 1) * a.ldx + 4 * q;
+	floatx4 rr[MT], ii[MT], ri[MT];  // sums of xr wr, xi wi, and xr wi + xi wr
+#pragma unroll
+	for (int m = 0; m < MT; ++m) rr[m] = ii[m] = ri[m] = floatx4{0.f, 0.f, 0.f, 0.f};
+	auto multiply = [&](const floatx4 &wr, const floatx4 &wi, const floatx4 (&xr)[MT], const floatx4 (&xi)[MT]) {
+#pragma unroll
+		for (int s = 0; s < 4; ++s)
+#pragma unroll
+			for (int m = 0; m < MT; ++m) {
+				rr[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xr[m][s], wr[s], rr[m], 0, 0, 0);
+				ii[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xi[m][s], wi[s], ii[m], 0, 0, 0);
+				ri[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xr[m][s], wi[s], ri[m], 0, 0, 0);
+				ri[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xi[m][s], wr[s], ri[m], 0, 0, 0);
+			}
+	};
+	const int groups = a.K / 16;
+	if (groups > 0) {
+		floatx4 wr[DEPTH], wi[DEPTH], xr[DEPTH][MT], xi[DEPTH][MT];
+		auto load = [&](int u, int g) {
+			const int k = 16 * min(g, groups - 1);
+			wr[u] = load_group<V4>(w_re + k);
+			wi[u] = load_group<V4>(w_im + k);
+#pragma unroll
+			for (int m = 0; m < MT; ++m) {
+				xr[u][m] = load_group<V4>(a.x_re + x_at[m] + k);
+				xi[u][m] = load_group<V4>(a.x_im + x_at[m] + k);
+			}
+		};
+#pragma unroll
+		for (int u = 0; u < DEPTH; ++u) load(u, u);
+		int g = 0;
+		for (; g + DEPTH <= groups; g += DEPTH) {
+#pragma unroll
+			for (int u = 0; u < DEPTH; ++u) {
+				multiply(wr[u], wi[u], xr[u], xi[u]);
+				load(u, g + DEPTH + u);
+			}
+		}
+#pragma unroll
+		for (int u = 0; u < DEPTH; ++u)
+			if (g + u < groups) multiply(wr[u], wi[u], xr[u], xi[u]);
+	}
+	if (a.K % 16) {  // the rest of K, element by element; what lies behind K is zero on both sides
+		floatx4 wr, wi, xr[MT], xi[MT];
+#pragma unroll
+		for (int s = 0; s < 4; ++s) {
+			const int k = 16 * groups + s;
+			const bool in = k + 4 * q < a.K;
+			wr[s] = in ? w_re[k] : 0.f;
+			wi[s] = in ? w_im[k] : 0.f;
+#pragma unroll
+			for (int m = 0; m < MT; ++m) {
+				xr[m][s] = in ? a.x_re[x_at[m] + k] : 0.f;
+				xi[m][s] = in ? a.x_im[x_at[m] + k] : 0.f;
+			}
+		}
+		multiply(wr, wi, xr, xi);
+	}
+	// element i of a lane: entry n0 + r, row 16 m + 4 q + i; the 16 lanes of a quarter are combined in a fixed order
+	const bool in = n0 + r < a.N;
+#pragma unroll
+	for (int m = 0; m < MT; ++m)
+#pragma unroll
+		for (int i = 0; i < 4; ++i) {
+			const float z_r = rr[m][i] - ii[m][i], z_i = ri[m][i];
+			double sum = in ? fma((double) z_i, (double) z_i, (double) z_r * z_r) : 0.0;
+			ArgMax best = {in ? fmaf(z_r, z_r, z_i * z_i) : -1.f, n0 + r};
+			sum += exchange<double, 0>(sum);
+			sum += exchange<double, 1>(sum);
+			sum += exchange<double, 2>(sum);
+			sum += exchange<double, 3>(sum);
+			best = ArgMaxOp()(best, exchange<ArgMax, 0>(best));
+			best = ArgMaxOp()(best, exchange<ArgMax, 1>(best));
+			best = ArgMaxOp()(best, exchange<ArgMax, 2>(best));
+			best = ArgMaxOp()(best, exchange<ArgMax, 3>(best));
+			if (r == 0) met[wave][16 * m + 4 * q + i] = ScoreTile{sum, best.v, best.i};
+		}
+	__syncthreads();
+	if (t < B) {
+		ScoreTile x = met[0][t];
+#pragma unroll
+		for (int w = 1; w < WAVES; ++w) {
+			const ScoreTile y = met[w][t];
+			x.sum += y.sum;
+			if (y.best > x.best) {  // (the entries of a later wavefront are larger numbers)
+				x.best = y.best;
+				x.index = y.index;
+			}
+		}
+		part[(long) t * gridDim.x + blockIdx.x] = x;
+	}
+}
+
+// One workgroup per row: its tiles, then its label
+__global__ __launch_bounds__(TPB) void head_score_finish_kernel(const HeadArgs a, const ScoreTile *__restrict__ part, int tiles) {
+	__shared__ double lds_d[WAVES];
+	__shared__ ArgMax lds_a[WAVES];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+	const long row = blockIdx.x;
+	double sum = 0.0;
+	ArgMax top = {-1.0f, 0x7fffffff};
+	for (int k = t; k < tiles; k += TPB) {
+		const ScoreTile x = part[row * tiles + k];
+		sum += x.sum;
+		if (x.best > top.v) top = ArgMax{x.best, x.index};
+	}
+	sum = group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane);
+	top = group_reduce<ArgMax, WAVES>(top, ArgMaxOp(), lds_a, 0, wave, lane);
+	const float S = clamped((float) sum);
+	const int best = top.i < 0 || top.i >= a.N ? 0 : top.i;  // a row of NaN has no largest entry
+	const LabelTerm l = label_term<WAVES>(a, row, a.labels ? a.labels[row] : best, S, lds_d, t, lane, wave);
+	if (t == 0) {
+		a.s[row] = S;
+		if (a.loss) a.loss[row] = l.loss;
+		if (a.argmax) a.argmax[row] = best;
+	}
+}
+
 struct ScatterArgs {
 	const int *row_of, *label_of;  // the rows in order of their labels
 	const float *c_re, *c_im, *x_re, *x_im;
@@ -924,9 +1073,35 @@ static int head_labels(const HeadArgs &a, const HeadBuffers &b, int B, float *dw
 	return CNET_OK;
 }
 
+// rows that head_score_kernel takes, where their logits are too many for the small-C kernel (4 tiles of 16 x 16 per compute unit, in a
+// few microseconds with the pass over them)
+constexpr int SCORE_ROWS = 64;
+
+static int head_score(const HeadArgs &a, int B) {
+	const int tiles = (a.N + 16 * WAVES - 1) / (16 * WAVES);
+	ScoreTile *part = (ScoreTile *) vocab_workspace((size_t) tiles * B * sizeof(ScoreTile));
+	if (!part) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
+	const bool v4 = a.ldx % 4 == 0 && a.ldw % 4 == 0 && aligned16(a.x_re) && aligned16(a.x_im) && aligned16(a.w_re) && aligned16(a.w_im);
+#define CNET_SCORE(MT)                                                                                                          \
+	do {                                                                                                                        \
+		if (v4) hipLaunchKernelGGL((head_score_kernel<MT, true>), dim3((unsigned) tiles), dim3(TPB), 0, rt().stream, a, B, part);  \
+		else hipLaunchKernelGGL((head_score_kernel<MT, false>), dim3((unsigned) tiles), dim3(TPB), 0, rt().stream, a, B, part);    \
+	} while (0)
+	if (B <= 16) CNET_SCORE(1);
+	else if (B <= 32) CNET_SCORE(2);
+	else if (B <= 48) CNET_SCORE(3);
+	else CNET_SCORE(4);
+#undef CNET_SCORE
+	CNET_LAUNCH_CHECK();
+	hipLaunchKernelGGL(head_score_finish_kernel, dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, part, tiles);
+	CNET_LAUNCH_CHECK();
+	return CNET_OK;
+}
+
 static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float *dws_re, float *dws_im, long lddw, int accumulate_dw, bool bwd) {
 	HeadArgs a = proto;
 	const int K = a.K, N = a.N;
+	if (!bwd && B <= SCORE_ROWS && (long) ((B + 15) / 16) * ((N + 15) / 16) > 4L * rt().prop.multiProcessorCount) return head_score(a, B);
 	const HeadPlan plan = head_plan(B, K, N, bwd, a.argmax || !a.labels);
 	HeadBuffers b;
 	int rc = head_buffers(B, K, plan, b);

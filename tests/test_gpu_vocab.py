@@ -286,6 +286,33 @@ def test_vocab_head_rows_in_directions_that_the_weights_hardly_have(gpu, weak):
     head_check(B, K, N, argmax=False, data=(x, w, labels))
 
 
+@pytest.mark.parametrize("B,K,N,pad,off", [(1, 40, 17000, 0, 0), (3, 5, 20001, 0, 0), (16, 64, 16500, 4, 0), (17, 33, 9001, 2, 1), (32, 100, 8300, 0, 0),
+                                           (40, 30, 6001, 0, 0), (48, 48, 5600, 0, 4), (63, 1, 4200, 0, 0), (64, 130, 4100, 0, 0), (1, 1024, 32768, 0, 0)])
+def test_vocab_head_few_rows_against_a_large_vocabulary(gpu, B, K, N, pad, off):
+    rng = np.random.default_rng(B + K + N)
+    x, w, labels = head_data(rng, B, K, N)
+    if N > 5000:
+        w[4999] = w[137]                                  # the same entry twice: the lower index
+        x[0] = 3 * w[137].conj()
+    x, w = (z.real.astype(np.float32).astype(np.float64) + 1j * z.imag.astype(np.float32) for z in (x, w))
+    ref = head_ref(x, w, labels)
+    X, W = cmat(x, K + pad + off, off), cmat(w, K + pad + off, off)
+    s, loss, am = capi.empty(B), capi.empty(B), capi.empty(B, np.int32)
+    ops.vocab_head_fwd(X, W, ops.ints(labels), s, loss, am)
+    near(s.download(), ref["s"], ref["size_s"], 2 * K + 32, "s")
+    ok = np.isfinite(ref["loss"])
+    assert np.array_equal(np.isnan(loss.download()), ~ok)
+    bound = 2 * (2 * K + 32) * HALF * ref["size_s"] / ref["s"] + 8 * HALF * (1 + np.abs(ref["loss"]))
+    assert np.all(np.abs(loss.download() - ref["loss"])[ok] <= bound[ok])
+    check_argmax(am.download(), ref)
+    assert N <= 5000 or K < 30 or am.download()[0] == 137
+    loss1, am1 = capi.empty(B), capi.empty(B, np.int32)
+    ops.vocab_head_fwd(X, W, None, s, loss1, am1)
+    assert np.array_equal(am1.download(), am.download())
+    p = ref["power"][np.arange(B), am.download()] / ref["s"]
+    assert np.all(np.abs(loss1.download() + np.log(p)) <= np.nanmax(bound) + 8 * HALF * (1 + np.abs(np.log(p))))
+
+
 def test_vocab_head_gives_what_the_separate_calls_give(gpu):
     """Linear, CrossEntropy and their backward passes over kept logits"""
     rng = np.random.default_rng(8)
