@@ -538,10 +538,11 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__
 }
 
 // ---- A few rows against the whole vocabulary (the next tokens of a batch of sequences): w is read once, and nothing of the logits
-// leaves the registers.  A wavefront forms the logits of 16 entries for up to 16 MT rows with v_mfma_f32_16x16x4_f32, walking K
-// with both operands straight from memory in the layout of the matrix instruction: lane (r, q), r = lane % 16, q = lane / 16, holds
-// row r of x (entry r of w) at k = 16 g + 4 q + s for step s of group g, so a group is one 128-bit load per plane and DEPTH
-// groups are on their way.  No LDS on the way (x is small and comes from the caches), no barrier in the loop.
+// leaves the registers.  A wavefront forms the logits of 16 entries for up to 16 MT rows with v_mfma_f32_16x16x4_f32, K in chunks of
+// 64.  Lane (r, q), r = lane % 16, q = lane / 16, holds entry r of w at k = 16 q .. 16 q + 15 of the chunk: 64 bytes in a row, so
+// that every line of w is fetched whole by one lane quarter after the other, and step j of the chunk multiplies the lanes' j-th
+// values (the four k of a matrix instruction are 16 apart; x is laid out in LDS to match).  The next chunk of w is on its way in
+// registers, and that of x for all four wavefronts, while the present one is multiplied.
 // Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one).
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
@@ -551,80 +552,95 @@ struct ScoreTile {   // what a workgroup leaves for every row
 	int index;
 };
 
-template <bool V4>
-__device__ __forceinline__ floatx4 load_group(const float *p) {
-	if (V4) return *reinterpret_cast<const floatx4 *>(p);
-	return floatx4{p[0], p[1], p[2], p[3]};
+// four floats from element k of a row of K on; GUARD: what lies behind K is zero and not read
+template <bool V4, bool GUARD>
+__device__ __forceinline__ floatx4 load_quad(const float *p, int k, int K) {
+	if (GUARD) {
+		floatx4 v;
+#pragma unroll
+		for (int j = 0; j < 4; ++j) v[j] = k + j < K ? p[k + j] : 0.f;
+		return v;
+	}
+	if (V4) return *reinterpret_cast<const floatx4 *>(p + k);
+	return floatx4{p[k], p[k + 1], p[k + 2], p[k + 3]};
 }
 
 template <int MT, bool V4>
 __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B, ScoreTile *__restrict__ part) {
-	constexpr int DEPTH = MT == 1 ? 4 : MT == 2 ? 3 : 2;
-	__shared__ ScoreTile met[WAVES][16 * MT];
+	constexpr int CHUNK_K = 64, ROWS = 16 * MT, PITCH = ROWS + 1;  // (an odd pitch: the 16 k groups of a row go to different banks)
+	__shared__ floatx4 xs[2][2][CHUNK_K / 4][PITCH];               // [buffer][plane][four k][row]
+	__shared__ ScoreTile met[WAVES][ROWS];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, q = lane >> 4;
 	const int n0 = (blockIdx.x * WAVES + wave) * 16;
 	// lanes beyond the last entry or row read the last one again; their results are masked
-	const long entry = (long) min(n0 + r, a.N - 1) * a.ldw + 4 * q;
+	const long entry = (long) min(n0 + r, a.N - 1) * a.ldw;
 	const float *w_re = a.w_re + entry, *w_im = a.w_im + entry;
-	long x_at[MT];
-#pragma unroll
-	for (int m = 0; m < MT; ++m) x_at[m] = (long) min(16 * m + r, B - 1) * a.ldx + 4 * q;
 	floatx4 rr[MT], ii[MT], ri[MT];  // sums of xr wr, xi wi, and xr wi + xi wr
 #pragma unroll
 	for (int m = 0; m < MT; ++m) rr[m] = ii[m] = ri[m] = floatx4{0.f, 0.f, 0.f, 0.f};
-	auto multiply = [&](const floatx4 &wr, const floatx4 &wi, const floatx4 (&xr)[MT], const floatx4 (&xi)[MT]) {
+	floatx4 w[2][4], w_next[2][4], x_next[2 * MT];
+	const int chunks = (a.K + CHUNK_K - 1) / CHUNK_K;
+	auto fetch = [&](int c) {
+		const int k0 = c * CHUNK_K;
+		if (k0 + CHUNK_K <= a.K) {
 #pragma unroll
-		for (int s = 0; s < 4; ++s)
-#pragma unroll
-			for (int m = 0; m < MT; ++m) {
-				rr[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xr[m][s], wr[s], rr[m], 0, 0, 0);
-				ii[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xi[m][s], wi[s], ii[m], 0, 0, 0);
-				ri[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xr[m][s], wi[s], ri[m], 0, 0, 0);
-				ri[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xi[m][s], wr[s], ri[m], 0, 0, 0);
+			for (int j = 0; j < 4; ++j) {
+				w_next[0][j] = load_quad<V4, false>(w_re, k0 + 16 * q + 4 * j, a.K);
+				w_next[1][j] = load_quad<V4, false>(w_im, k0 + 16 * q + 4 * j, a.K);
 			}
+#pragma unroll
+			for (int i = 0; i < 2 * MT; ++i) {
+				const int at = t + TPB * (i % MT), row = min(at / 16, B - 1);
+				x_next[i] = load_quad<V4, false>((i < MT ? a.x_re : a.x_im) + row * a.ldx, k0 + 4 * (at % 16), a.K);
+			}
+		} else {
+#pragma unroll
+			for (int j = 0; j < 4; ++j) {
+				w_next[0][j] = load_quad<V4, true>(w_re, k0 + 16 * q + 4 * j, a.K);
+				w_next[1][j] = load_quad<V4, true>(w_im, k0 + 16 * q + 4 * j, a.K);
+			}
+#pragma unroll
+			for (int i = 0; i < 2 * MT; ++i) {
+				const int at = t + TPB * (i % MT), row = min(at / 16, B - 1);
+				x_next[i] = load_quad<V4, true>((i < MT ? a.x_re : a.x_im) + row * a.ldx, k0 + 4 * (at % 16), a.K);
+			}
+		}
 	};
-	const int groups = a.K / 16;
-	if (groups > 0) {
-		floatx4 wr[DEPTH], wi[DEPTH], xr[DEPTH][MT], xi[DEPTH][MT];
-		auto load = [&](int u, int g) {
-			const int k = 16 * min(g, groups - 1);
-			wr[u] = load_group<V4>(w_re + k);
-			wi[u] = load_group<V4>(w_im + k);
+	fetch(0);
+	for (int c = 0; c < chunks; ++c) {
+#pragma unroll
+		for (int p = 0; p < 2; ++p)
+#pragma unroll
+			for (int j = 0; j < 4; ++j) w[p][j] = w_next[p][j];
+		// (the buffer was last read two chunks ago, before the barrier of the chunk between)
+#pragma unroll
+		for (int i = 0; i < 2 * MT; ++i) {
+			const int at = t + TPB * (i % MT);
+			xs[c & 1][i / MT][at % 16][at / 16] = x_next[i];
+		}
+		__syncthreads();
+		if (c + 1 < chunks) fetch(c + 1);
+		__builtin_amdgcn_sched_barrier(0);  // (the loads go out before the products, not after them)
+#pragma unroll
+		for (int j = 0; j < 4; ++j) {
+			floatx4 xr[MT], xi[MT];
 #pragma unroll
 			for (int m = 0; m < MT; ++m) {
-				xr[u][m] = load_group<V4>(a.x_re + x_at[m] + k);
-				xi[u][m] = load_group<V4>(a.x_im + x_at[m] + k);
+				xr[m] = xs[c & 1][0][4 * q + j][16 * m + r];
+				xi[m] = xs[c & 1][1][4 * q + j][16 * m + r];
 			}
-		};
 #pragma unroll
-		for (int u = 0; u < DEPTH; ++u) load(u, u);
-		int g = 0;
-		for (; g + DEPTH <= groups; g += DEPTH) {
+			for (int e = 0; e < 4; ++e) {
 #pragma unroll
-			for (int u = 0; u < DEPTH; ++u) {
-				multiply(wr[u], wi[u], xr[u], xi[u]);
-				load(u, g + DEPTH + u);
-			}
-		}
+				for (int m = 0; m < MT; ++m) rr[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xr[m][e], w[0][j][e], rr[m], 0, 0, 0);
 #pragma unroll
-		for (int u = 0; u < DEPTH; ++u)
-			if (g + u < groups) multiply(wr[u], wi[u], xr[u], xi[u]);
-	}
-	if (a.K % 16) {  // the rest of K, element by element; what lies behind K is zero on both sides
-		floatx4 wr, wi, xr[MT], xi[MT];
+				for (int m = 0; m < MT; ++m) ii[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xi[m][e], w[1][j][e], ii[m], 0, 0, 0);
 #pragma unroll
-		for (int s = 0; s < 4; ++s) {
-			const int k = 16 * groups + s;
-			const bool in = k + 4 * q < a.K;
-			wr[s] = in ? w_re[k] : 0.f;
-			wi[s] = in ? w_im[k] : 0.f;
+				for (int m = 0; m < MT; ++m) ri[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xr[m][e], w[1][j][e], ri[m], 0, 0, 0);
 #pragma unroll
-			for (int m = 0; m < MT; ++m) {
-				xr[m][s] = in ? a.x_re[x_at[m] + k] : 0.f;
-				xi[m][s] = in ? a.x_im[x_at[m] + k] : 0.f;
+				for (int m = 0; m < MT; ++m) ri[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(xi[m][e], w[0][j][e], ri[m], 0, 0, 0);
 			}
 		}
-		multiply(wr, wi, xr, xi);
 	}
 	// element i of a lane: entry n0 + r, row 16 m + 4 q + i; the 16 lanes of a quarter are combined in a fixed order
 	const bool in = n0 + r < a.N;
