@@ -716,57 +716,80 @@ struct ScatterArgs {
 // ---- The label's term of the weights' gradient: dw[label[r]] -= c_r x_r for every row r.  Labels of a text repeat (the most
 // frequent token of a batch of 8192 names hundreds of rows), so the rows are put in order of their labels first and then worked
 // off in chunks of equal length, whatever the labels.  The order is the stable one, so a label's rows are added in order.
-constexpr int ORDER_ROWS = 8192;  // rows ordered together (their keys fill 64 KB of LDS); longer batches go block by block
+constexpr int ORDER_ROWS = 8192;  // rows ordered together (their labels fill 32 KB of LDS); longer batches go block by block
 constexpr int CHUNK = 16;         // ordered rows of one workgroup
+constexpr int RANK_ROWS = 64;     // rows of one workgroup of head_order_kernel
 
-// Workgroup b sorts rows [b ORDER_ROWS, ..) by (label, row), rows without a label of the vocabulary last (a bitonic network in
-// LDS: 8192 rows take 91 exchanges of four pairs a thread).  row_of = -1 and label_of = N where there is no label.
-__global__ __launch_bounds__(1024) void head_order_kernel(const int *__restrict__ labels, int B, int N, int n2, int *__restrict__ row_of,
+// Orders the rows [y ORDER_ROWS, ..) by (label, row), rows without a label of the vocabulary last: workgroup (x, y) counts for each of
+// 64 rows how many come before it, its 16 wavefronts sharing the labels to compare with (8192 rows: 67 million comparisons over
+// 128 workgroups; a sorting network in one workgroup takes 80 us for them, this 6).  row_of = -1 and label_of = N where there
+// is no label.
+__global__ __launch_bounds__(1024) void head_order_kernel(const int *__restrict__ labels, int B, int N, int *__restrict__ row_of,
 		int *__restrict__ label_of) {
-	extern __shared__ unsigned long long keys[];
-	const int first = blockIdx.x * ORDER_ROWS, n = min(ORDER_ROWS, B - first);
-	for (int i = threadIdx.x; i < n2; i += 1024) {
-		const int label = i < n ? labels[first + i] : -1;
-		keys[i] = ((unsigned long long) (unsigned) (label >= 0 && label < N ? label : N) << 32) | (unsigned) i;
+	__shared__ __align__(16) int keys[ORDER_ROWS];
+	__shared__ int count[16][RANK_ROWS];
+	const int first = blockIdx.y * ORDER_ROWS, n = min(ORDER_ROWS, B - first), n4 = (n + 3) / 4 * 4;
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = blockIdx.x * RANK_ROWS, i = lo + lane;
+	if (lo >= n) return;
+	for (int k = threadIdx.x; k < n4; k += 1024) {
+		const int label = k < n ? labels[first + k] : -1;
+		keys[k] = k >= n ? 0x7fffffff : label >= 0 && label < N ? label : N;
 	}
-	for (int k = 2; k <= n2; k *= 2)
-		for (int j = k / 2; j > 0; j /= 2) {
-			__syncthreads();
-			for (int h = threadIdx.x; h < n2 / 2; h += 1024) {
-				const int lo = 2 * h - (h & (j - 1)), hi = lo + j;
-				const unsigned long long u = keys[lo], v = keys[hi];
-				if ((u > v) == ((lo & k) == 0)) {
-					keys[lo] = v;
-					keys[hi] = u;
-				}
-			}
-		}
 	__syncthreads();
-	for (int i = threadIdx.x; i < n; i += 1024) {
-		const int label = (int) (keys[i] >> 32);
-		label_of[first + i] = label;
-		row_of[first + i] = label < N ? first + (int) (unsigned) keys[i] : -1;
+	const int key = keys[min(i, n - 1)];
+	const int per = ((n4 / 4 + 15) / 16) * 4, j0 = min(n4, wave * per), j1 = min(n4, j0 + per);
+	int before = 0;
+#pragma unroll 4
+	for (int j = j0; j < j1; j += 4) {
+		const int4 other = *reinterpret_cast<const int4 *>(keys + j);
+		// an equal label counts where its row comes first: j + d < i
+		if (j >= lo && j < lo + RANK_ROWS) {
+			before += (other.x < key + (j < i)) + (other.y < key + (j + 1 < i)) + (other.z < key + (j + 2 < i)) + (other.w < key + (j + 3 < i));
+		} else {
+			const int limit = key + (j < lo);
+			before += (other.x < limit) + (other.y < limit) + (other.z < limit) + (other.w < limit);
+		}
 	}
+	count[wave][lane] = before;
+	__syncthreads();
+	if (wave || i >= n) return;
+	int rank = 0;
+#pragma unroll
+	for (int w = 0; w < 16; ++w) rank += count[w][lane];
+	label_of[first + rank] = key;
+	row_of[first + rank] = key < N ? first + i : -1;
 }
 
-// subtracts V columns of one label's sum from its row of the gradient
+// V columns of one label's row of the gradient: its planes, and the label's sum subtracted from them
 template <int V>
-__device__ __forceinline__ void subtract_label(const ScatterArgs &a, int label, int c, const float *re, const float *im) {
-	const long o = (long) label * a.lddw + c;
-	float v[V];
-	auto apply = [&](float *p, const float *d, float sign) {
-		load_v<V>(v, p + o);
-#pragma unroll
-		for (int k = 0; k < V; ++k) v[k] -= sign * d[k];
-		store_v<V>(p + o, v);
-	};
-	apply(a.dw_re, re, 1.f);
-	apply(a.dw_im, im, 1.f);
-	if (a.dws_re) {
-		apply(a.dws_re, re, 1.f);
-		apply(a.dws_im, im, -1.f);
+struct LabelRow {
+	float v[4][V];
+	__device__ __forceinline__ void load(const ScatterArgs &a, int label, int c) {
+		const long o = (long) label * a.lddw + c;
+		load_v<V>(v[0], a.dw_re + o);
+		load_v<V>(v[1], a.dw_im + o);
+		if (a.dws_re) {
+			load_v<V>(v[2], a.dws_re + o);
+			load_v<V>(v[3], a.dws_im + o);
+		}
 	}
-}
+	__device__ __forceinline__ void subtract(const ScatterArgs &a, int label, int c, const float *re, const float *im) {
+		const long o = (long) label * a.lddw + c;
+#pragma unroll
+		for (int k = 0; k < V; ++k) {
+			v[0][k] -= re[k];
+			v[1][k] -= im[k];
+			v[2][k] -= re[k];
+			v[3][k] += im[k];
+		}
+		store_v<V>(a.dw_re + o, v[0]);
+		store_v<V>(a.dw_im + o, v[1]);
+		if (a.dws_re) {
+			store_v<V>(a.dws_re + o, v[2]);
+			store_v<V>(a.dws_im + o, v[3]);
+		}
+	}
+};
 
 // Workgroup (x, y): the ordered rows [CHUNK x, CHUNK x + CHUNK) of the block that starts at `first`, V columns per thread.  A run of
 // one label that lies inside the chunk is subtracted at once; the part of a run that reaches over the chunk's ends goes to
@@ -792,14 +815,16 @@ __global__ __launch_bounds__(TPB) void head_label_kernel(const ScatterArgs a, in
 	if (c >= a.K) return;
 	float re[V], im[V];
 	int begin = 0;
-	constexpr int AHEAD = 8;  // rows of x in flight
+	constexpr int AHEAD = V == 4 ? 4 : 8;  // rows of x, and of the gradient they may end up in, in flight
 #pragma unroll
 	for (int k0 = 0; k0 < CHUNK; k0 += AHEAD) {
 		float x_r[AHEAD][V], x_i[AHEAD][V];
+		LabelRow<V> dst[AHEAD];
 #pragma unroll
 		for (int u = 0; u < AHEAD; ++u) {  // (a place without a label reads row 0 and is not used)
 			load_v<V>(x_r[u], a.x_re + (long) row_at[k0 + u] * a.ldx + c);
 			load_v<V>(x_i[u], a.x_im + (long) row_at[k0 + u] * a.ldx + c);
+			dst[u].load(a, max(label_at[k0 + u + 1], 0), c);
 		}
 #pragma unroll
 		for (int u = 0; u < AHEAD; ++u) {
@@ -820,7 +845,7 @@ __global__ __launch_bounds__(TPB) void head_label_kernel(const ScatterArgs a, in
 			if (same && k + 1 < CHUNK) continue;
 			const bool began = begin == 0 && label_at[0] == label;
 			if (!began && !same) {
-				subtract_label<V>(a, label, c, re, im);
+				dst[u].subtract(a, label, c, re, im);
 			} else {
 				float *part = a.part + ((long) blockIdx.x * 2 + (began ? 0 : 1)) * 2 * a.ldk + c;
 				store_v<V>(part, re);
@@ -842,6 +867,8 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 	int chunks = 1;                                                 // further chunks that hold a part of it
 	while (p1 + chunks * CHUNK < block_end && a.label_of[p1 + chunks * CHUNK] == label) ++chunks;
 	const float *part = a.part + ((long) blockIdx.x * 2 + 1) * 2 * a.ldk + c;
+	LabelRow<V> dst;
+	dst.load(a, label, c);
 	float re[V], im[V];
 	load_v<V>(re, part);
 	load_v<V>(im, part + a.ldk);
@@ -857,7 +884,7 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 			im[q] += y[q];
 		}
 	}
-	subtract_label<V>(a, label, c, re, im);
+	dst.subtract(a, label, c, re, im);
 }
 
 // Fills the rows behind `panel` wide diagonal blocks of a Hermitian matrix from the columns above them: C[j][i] = conj(C[i][j]).
@@ -1065,10 +1092,8 @@ static int gram_product(int K, int L, const float *a_re, const float *a_im, long
 }
 
 static int head_labels(const HeadArgs &a, const HeadBuffers &b, int B, float *dw_re, float *dw_im, float *dws_re, float *dws_im, long lddw) {
-	int n2 = 2;
-	while (n2 < std::min(B, ORDER_ROWS)) n2 *= 2;
-	hipLaunchKernelGGL(head_order_kernel, dim3((unsigned) ((B + ORDER_ROWS - 1) / ORDER_ROWS)), dim3(1024), n2 * sizeof(unsigned long long), rt().stream,
-			a.labels, B, a.N, n2, b.row_of, b.label_of);
+	const dim3 blocks((unsigned) ((std::min(B, ORDER_ROWS) + RANK_ROWS - 1) / RANK_ROWS), (unsigned) ((B + ORDER_ROWS - 1) / ORDER_ROWS));
+	hipLaunchKernelGGL(head_order_kernel, blocks, dim3(1024), 0, rt().stream, a.labels, B, a.N, b.row_of, b.label_of);
 	CNET_LAUNCH_CHECK();
 	const ScatterArgs sc = {b.row_of, b.label_of, b.st.c_re, b.st.c_im, a.x_re, a.x_im, a.ldx, dw_re, dw_im, dws_re, dws_im, lddw, b.label_part, b.ldk,
 			B, a.K, a.N};
