@@ -401,18 +401,19 @@ struct HeadArgs {
 	float *s, *loss;
 	int *argmax;
 	const float *y_re, *y_im;  // conj(z) w, not yet divided by S
-	float *xs_re, *xs_im;      // x / S, for the weights' gradient
-	long ldy;
+	float *xs_re, *xs_im;      // the rows that are trained on, as the weights' gradient reads them; zeros elsewhere
+	long ldy;                  // leading dimension of y and xs
 	float *dx_re, *dx_im, *dxs_re, *dxs_im;
 	long lddx;
 	int accumulate_dx;
-	int K, N;
+	int B, K, N;
 };
 
 // what a row's label makes of it
 struct LabelTerm {
 	int label;          // -1: none in the vocabulary
-	float loss, inv;    // inv: 1 / S, 0 for a row that is left out
+	bool live;          // false: the row is left out
+	float loss;
 	float c_re, c_im;   // conj(z_label) / m
 };
 
@@ -436,18 +437,24 @@ __device__ __forceinline__ LabelTerm label_term(const HeadArgs &a, long row, int
 	LabelTerm l;
 	l.label = known ? label : -1;
 	l.loss = label < 0 ? 0.f : known ? -logf((float) clamped(power / (double) S)) : __builtin_nanf("");
-	l.inv = label < 0 ? 0.f : 1.0f / S;
+	l.live = label >= 0;
 	l.c_re = known ? (float) (re / m) : 0.f;
 	l.c_im = known ? (float) (-im / m) : 0.f;
 	return l;
 }
 
 // One workgroup per row: S, the label's logit, loss, and the gradient at x: y / S minus the label's row of w times conj(z_label) / m.
+// xs = x / sqrt(S), so that both operands of the weights' gradient come from it: a row that is left out is zero in either, whatever
+// it holds (padding may hold anything), and so are the rows beyond B that fill up the last chunk of that product.
 template <bool BWD>
 __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st) {
 	__shared__ double lds_d[WAVES];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.x;
+	if (BWD && row >= a.B) {
+		for (int c = t; c < a.ldy; c += TPB) a.xs_re[row * a.ldy + c] = a.xs_im[row * a.ldy + c] = 0.f;
+		return;
+	}
 	double sum = st.sum[row];
 	if (sum < 0.0) {
 		sum = 0.0;
@@ -469,18 +476,28 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 	}
 	const float *xr = a.x_re + row * a.ldx, *xi = a.x_im + row * a.ldx;
 	const long label_row = (l.label < 0 ? 0 : l.label) * a.ldw;
-	for (int c = t; c < a.K; c += TPB) {
+	const float inv = 1.0f / S, root = (float) (1.0 / sqrt((double) S));
+	for (int c = t; c < a.ldy; c += TPB) {
 		const long o = row * a.ldy + c, d = row * a.lddx + c;
-		const float w_r = a.w_re[label_row + c], w_i = a.w_im[label_row + c];
-		const float g_r = a.y_re[o] * l.inv - (l.c_re * w_r - l.c_im * w_i), g_i = a.y_im[o] * l.inv - (l.c_re * w_i + l.c_im * w_r);
-		put(a.dx_re + d, g_r, a.accumulate_dx);
-		put(a.dx_im + d, g_i, a.accumulate_dx);
-		if (a.dxs_re) {
-			put(a.dxs_re + d, g_r, a.accumulate_dx);
-			put(a.dxs_im + d, -g_i, a.accumulate_dx);
+		float s_r = 0.f, s_i = 0.f;
+		if (c < a.K) {
+			float g_r = 0.f, g_i = 0.f;
+			if (l.live) {
+				const float w_r = a.w_re[label_row + c], w_i = a.w_im[label_row + c];
+				g_r = a.y_re[o] * inv - (l.c_re * w_r - l.c_im * w_i);
+				g_i = a.y_im[o] * inv - (l.c_re * w_i + l.c_im * w_r);
+				s_r = xr[c] * root;
+				s_i = xi[c] * root;
+			}
+			put(a.dx_re + d, g_r, a.accumulate_dx);
+			put(a.dx_im + d, g_i, a.accumulate_dx);
+			if (a.dxs_re) {
+				put(a.dxs_re + d, g_r, a.accumulate_dx);
+				put(a.dxs_im + d, -g_i, a.accumulate_dx);
+			}
 		}
-		a.xs_re[o] = xr[c] * l.inv;
-		a.xs_im[o] = xi[c] * l.inv;
+		a.xs_re[o] = s_r;
+		a.xs_im[o] = s_i;
 	}
 }
 
@@ -494,6 +511,23 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.x;
 	float *zr = z_re + row * ldz, *zi = z_im + row * ldz;
+	// xs: the row as it is, zero if it is left out (whatever it holds) or beyond B
+	auto keep = [&](bool live) {
+		for (int c = t; c < a.ldy; c += T) {
+			const bool in = live && c < a.K;
+			a.xs_re[row * a.ldy + c] = in ? a.x_re[row * a.ldx + c] : 0.f;
+			a.xs_im[row * a.ldy + c] = in ? a.x_im[row * a.ldx + c] : 0.f;
+		}
+	};
+	const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+	if (BWD && row >= a.B) {
+		for (int c = 4 * t; c < a.N; c += 4 * T) {
+			store_v<4>(zr + c, zero);
+			store_v<4>(zi + c, zero);
+		}
+		keep(false);
+		return;
+	}
 	double sum = 0.0;
 	ArgMax top = {-1.0f, 0x7fffffff};
 	for (int c = 4 * t; c < a.N; c += 4 * T) {
@@ -519,14 +553,21 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__
 		if (a.argmax) a.argmax[row] = best;
 	}
 	if (!BWD) return;
+	keep(l.live);
+	const float inv = 1.0f / S;
 	for (int c = 4 * t; c < a.N; c += 4 * T) {
+		if (!l.live) {
+			store_v<4>(zr + c, zero);
+			store_v<4>(zi + c, zero);
+			continue;
+		}
 		float u[4], v[4];
 		load_v<4>(u, zr + c);
 		load_v<4>(v, zi + c);
 #pragma unroll
 		for (int k = 0; k < 4; ++k) {
-			u[k] *= l.inv;
-			v[k] *= -l.inv;
+			u[k] *= inv;
+			v[k] *= -inv;
 			if (c + k == l.label) {
 				u[k] -= l.c_re;
 				v[k] -= l.c_im;
@@ -887,12 +928,14 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 	dst.subtract(a, label, c, re, im);
 }
 
-// Fills the rows behind `panel` wide diagonal blocks of a Hermitian matrix from the columns above them: C[j][i] = conj(C[i][j]).
+// Fills what lies below the diagonal blocks of a Hermitian matrix (`panel` wide, the last, number `last`, as wide as is left) from
+// what lies above them: C[j][i] = conj(C[i][j]).
 // Tiles of 32 x 32 turned over in LDS; blockIdx (x, y) = tile (column, row) of the part that is there.
-__global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K, int panel) {
+__global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K, int panel,
+		int last) {
 	__shared__ float tile[2][32][33];
 	const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
-	if (c0 / panel <= r0 / panel) return;  // (panel is a multiple of 32)
+	if (min(c0 / panel, last) <= min(r0 / panel, last)) return;  // (panel is a multiple of 32)
 	const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 	for (int k = ty; k < 32; k += 8)
 		if (r0 + k < K && c0 + tx < K) {
@@ -905,6 +948,24 @@ __global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_
 			c_re[(long) (c0 + k) * ldc + r0 + tx] = tile[0][tx][k];
 			c_im[(long) (c0 + k) * ldc + r0 + tx] = -tile[1][tx][k];
 		}
+}
+
+// dst[plane][r][c] = src_plane[r][c] inside rows x cols, zero outside; blockIdx.y = plane.  One thread per four columns of dst.
+__global__ __launch_bounds__(TPB) void head_pack_kernel(const float *__restrict__ s_re, const float *__restrict__ s_im, long lds, int rows, int cols,
+		float *__restrict__ dst, long rows_d, int ldd) {
+	const int groups = ldd / 4;
+	const long idx = (long) blockIdx.x * TPB + threadIdx.x;
+	if (idx >= rows_d * groups) return;
+	const long r = idx / groups;
+	const int c0 = (int) (idx - r * groups) * 4;
+	const float *s = (blockIdx.y ? s_im : s_re) + r * lds;
+	float v[4] = {0.f, 0.f, 0.f, 0.f};
+	if (r < rows) {
+#pragma unroll
+		for (int k = 0; k < 4; ++k)
+			if (c0 + k < cols) v[k] = s[c0 + k];
+	}
+	store_v<4>(dst + (blockIdx.y * rows_d + r) * ldd + c0, v);
 }
 
 // the gradient of no rows at all
@@ -969,6 +1030,7 @@ static int distill(const DistillArgs &a) {
 struct HeadBuffers {
 	RowState st;
 	float *piece, *y, *xs, *gram;  // planes re, im
+	float *x, *w;                  // copies of the operands (HeadPad)
 	int *row_of, *label_of;
 	float *label_part;
 	int piece_cols;                // columns of one piece, also its leading dimension
@@ -1027,16 +1089,39 @@ static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	return p;
 }
 
-static int head_buffers(int B, int K, const HeadPlan &plan, HeadBuffers &b) {
+// Widths that do not suit the matrix kernels (128-bit transfers, whole chunks of 16 along the summed axis) cost them a copy of w in
+// front of every product, or a second launch over the whole result for the rest of a chunk (300 x 1500 -> 40000: 0.9 ms for the
+// last 12 of 300 rows).  A large head therefore copies x and w once, zeros filling the last chunks, and its own buffers
+// have rows to spare.
+struct HeadPad {
+	bool copy;  // of x and w
+	int B, K, N;
+};
+static HeadPad head_pad(const HeadArgs &a, int B, const HeadPlan &plan) {
+	auto up = [](int v) { return (v + 15) / 16 * 16; };
+	HeadPad p = {false, B, a.K, a.N};
+	if ((double) a.N * a.K < (double) (1 << 18)) return p;
+	if (plan.bwd) p.B = up(B);
+	const bool odd = a.K % 16 || a.ldx % 4 || a.ldw % 4 || !aligned16(a.x_re) || !aligned16(a.x_im) || !aligned16(a.w_re) || !aligned16(a.w_im);
+	if (odd && 8.0 * up(a.N) * up(a.K) <= (double) (1L << 31)) {
+		p.copy = true;
+		p.K = up(a.K);
+		p.N = up(a.N);
+	}
+	return p;
+}
+
+static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b) {
 	b.piece_cols = plan.piece_cols;
-	b.ldk = ((long) K + 3) / 4 * 4;
-	const size_t rows = ((size_t) B + 63) / 64 * 64;
-	const size_t piece = plan.pieces || plan.whole ? 2 * (size_t) B * b.piece_cols : 0;
-	const size_t wide = (plan.bwd && !plan.whole) || plan.gram ? 2 * (size_t) B * b.ldk : 0, square = plan.gram ? 2 * (size_t) K * b.ldk : 0;
+	b.ldk = ((long) pad.K + 3) / 4 * 4;
+	const size_t rows = ((size_t) pad.B + 63) / 64 * 64;
+	const size_t piece = plan.pieces || plan.whole ? 2 * (size_t) pad.B * b.piece_cols : 0;
+	const size_t wide = plan.bwd || plan.gram ? 2 * (size_t) pad.B * b.ldk : 0, square = plan.gram ? 2 * (size_t) pad.K * b.ldk : 0;
 	const size_t part = plan.gram && !plan.pieces ? 2 * HEAD_SLABS * rows : 0;
 	const bool label = plan.bwd && !plan.whole;
-	const size_t order = label ? rows : 0, label_part = label ? (size_t) (std::min(B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
-	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part) * sizeof(float));
+	const size_t order = label ? rows : 0, label_part = label ? (size_t) (std::min(pad.B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
+	const size_t copy_x = pad.copy ? 2 * (size_t) pad.B * b.ldk : 0, copy_w = pad.copy ? 2 * (size_t) pad.N * b.ldk : 0;
+	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part + copy_x + copy_w) * sizeof(float));
 	if (!p) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
 	auto take = [&](size_t floats) {
 		float *q = p;
@@ -1056,7 +1141,15 @@ static int head_buffers(int B, int K, const HeadPlan &plan, HeadBuffers &b) {
 	b.label_part = take(label_part);
 	b.row_of = (int *) take(order);
 	b.label_of = (int *) take(order);
+	b.x = take(copy_x);
+	b.w = take(copy_w);
 	return CNET_OK;
+}
+
+static void head_pack(const float *s_re, const float *s_im, long lds, int rows, int cols, float *dst, long rows_d, int ldd) {
+	const long threads = rows_d * (ldd / 4);
+	hipLaunchKernelGGL(head_pack_kernel, dim3((unsigned) ((threads + TPB - 1) / TPB), 2), dim3(TPB), 0, rt().stream, s_re, s_im, lds, rows, cols, dst, rows_d,
+			ldd);
 }
 
 // C = conj(A) B, A row-major or k-major, B k-major
@@ -1080,13 +1173,15 @@ static int conj_product_pair(bool a_kmajor, int M, int N, int K, const float *a_
 static int gram_product(int K, int L, const float *a_re, const float *a_im, long lda, const float *b_re, const float *b_im, long ldb, float *c_re, float *c_im,
 		long ldc) {
 	if (!in_panels(K, L)) return conj_product(1, K, K, L, a_re, a_im, lda, b_re, b_im, ldb, c_re, c_im, ldc, 0);
-	for (int k0 = 0; k0 < K; k0 += PANEL) {
+	const int last = K / PANEL - 1;  // (the last panel takes what is left, up to twice as much: a small one would not fill the device)
+	for (int i = 0; i <= last; ++i) {
+		const int k0 = i * PANEL;
 		const long o = (long) k0 * ldc + k0;
-		const int rc = conj_product(1, std::min(PANEL, K - k0), K - k0, L, a_re + k0, a_im + k0, lda, b_re + k0, b_im + k0, ldb, c_re + o, c_im + o, ldc, 0);
+		const int rc = conj_product(1, i < last ? PANEL : K - k0, K - k0, L, a_re + k0, a_im + k0, lda, b_re + k0, b_im + k0, ldb, c_re + o, c_im + o, ldc, 0);
 		if (rc) return rc;
 	}
 	const unsigned tiles = (unsigned) ((K + 31) / 32);
-	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, PANEL);
+	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, PANEL, last);
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
@@ -1141,56 +1236,71 @@ static int head_score(const HeadArgs &a, int B) {
 
 static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float *dws_re, float *dws_im, long lddw, int accumulate_dw, bool bwd) {
 	HeadArgs a = proto;
+	a.B = B;
 	const int K = a.K, N = a.N;
 	if (!bwd && B <= SCORE_ROWS && (long) ((B + 15) / 16) * ((N + 15) / 16) > 4L * rt().prop.multiProcessorCount) return head_score(a, B);
 	const HeadPlan plan = head_plan(B, K, N, bwd, a.argmax || !a.labels);
+	const HeadPad pad = head_pad(a, B, plan);
 	HeadBuffers b;
-	int rc = head_buffers(B, K, plan, b);
+	int rc = head_buffers(pad, plan, b);
 	if (rc) return rc;
-	const int np = b.piece_cols;
+	const int np = b.piece_cols, Kp = pad.K;  // Kp: K, or K filled up with zeros where the operands are copies
 	const long ldk = b.ldk;
-	float *z_re = b.piece, *z_im = b.piece + (size_t) B * np;
-	float *y_re = b.y, *y_im = b.y + (size_t) B * ldk;
-	float *g_re = b.gram, *g_im = b.gram + (size_t) K * ldk;
+	if (pad.copy) {
+		head_pack(a.x_re, a.x_im, a.ldx, B, K, b.x, pad.B, (int) ldk);
+		head_pack(a.w_re, a.w_im, a.ldw, N, K, b.w, pad.N, (int) ldk);
+		CNET_LAUNCH_CHECK();
+		a.x_re = b.x;
+		a.x_im = b.x + (size_t) pad.B * ldk;
+		a.w_re = b.w;
+		a.w_im = b.w + (size_t) pad.N * ldk;
+		a.ldx = a.ldw = ldk;
+	}
+	float *z_re = b.piece, *z_im = b.piece + (size_t) pad.B * np;
+	float *y_re = b.y, *y_im = b.y + (size_t) pad.B * ldk;
+	float *g_re = b.gram, *g_im = b.gram + (size_t) Kp * ldk;
 	a.y_re = y_re;
 	a.y_im = y_im;
 	a.xs_re = b.xs;
-	a.xs_im = b.xs + (size_t) B * ldk;
+	a.xs_im = b.xs + (size_t) pad.B * ldk;
 	a.ldy = ldk;
-	auto logits = [&](int n0, int n) {
-		return cnet_clinear_fwd(a.x_re, a.x_im, a.ldx, a.w_re + (size_t) n0 * a.ldw, a.w_im + (size_t) n0 * a.ldw, a.ldw, z_re, z_im, np, B, K, n, 0);
-	};
+	auto w_at = [&](const float *w, int n0) { return w + (size_t) n0 * a.ldw; };
 	if (plan.whole) {
-		rc = logits(0, N);
+		rc = cnet_clinear_fwd(a.x_re, a.x_im, a.ldx, a.w_re, a.w_im, a.ldw, z_re, z_im, np, B, Kp, N, 0);
 		if (rc) return rc;
 		// a row of its own workgroup: many threads where the rows are long
+		const dim3 grid((unsigned) (bwd ? pad.B : B));
 		if (N > 4096) {
-			if (bwd) hipLaunchKernelGGL((head_row_kernel<1024, true>), dim3((unsigned) B), dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
-			else hipLaunchKernelGGL((head_row_kernel<1024, false>), dim3((unsigned) B), dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
+			if (bwd) hipLaunchKernelGGL((head_row_kernel<1024, true>), grid, dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
+			else hipLaunchKernelGGL((head_row_kernel<1024, false>), grid, dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
 		} else {
-			if (bwd) hipLaunchKernelGGL((head_row_kernel<TPB, true>), dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
-			else hipLaunchKernelGGL((head_row_kernel<TPB, false>), dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
+			if (bwd) hipLaunchKernelGGL((head_row_kernel<TPB, true>), grid, dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
+			else hipLaunchKernelGGL((head_row_kernel<TPB, false>), grid, dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
 		}
 		CNET_LAUNCH_CHECK();
 		if (!bwd) return CNET_OK;
-		return cnet_clinear_bwd_sym(z_re, z_im, np, a.x_re, a.x_im, a.ldx, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx,
-				a.accumulate_dx, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw, B, K, N);
+		if (pad.B == B)  // both in one launch where they are small
+			return cnet_clinear_bwd_sym(z_re, z_im, np, a.xs_re, a.xs_im, ldk, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx,
+					a.accumulate_dx, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw, B, K, N);
+		rc = cnet_clinear_bwd_input_sym(z_re, z_im, np, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx, B, K, N, a.accumulate_dx);
+		if (rc) return rc;
+		return cnet_clinear_bwd_weight_sym(z_re, z_im, np, a.xs_re, a.xs_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, pad.B, K, N, accumulate_dw);
 	}
 	for (int n0 = 0; plan.pieces && n0 < N; n0 += np) {
 		const int n = std::min(np, N - n0);
-		rc = logits(n0, n);
+		rc = cnet_clinear_fwd(a.x_re, a.x_im, a.ldx, w_at(a.w_re, n0), w_at(a.w_im, n0), a.ldw, z_re, z_im, np, B, Kp, n, 0);
 		if (rc) return rc;
 		hipLaunchKernelGGL(head_piece_kernel, dim3((unsigned) B), dim3(TPB), 0, rt().stream, z_re, z_im, (long) np, n, n0, b.st);
 		CNET_LAUNCH_CHECK();
 		if (bwd && !plan.gram) {  // y += conj(z) w: linear in z, so the division by S can wait until S is whole
-			rc = conj_product(0, B, K, n, z_re, z_im, np, a.w_re + (size_t) n0 * a.ldw, a.w_im + (size_t) n0 * a.ldw, a.ldw, y_re, y_im, ldk, n0 > 0);
+			rc = conj_product(0, B, K, n, z_re, z_im, np, w_at(a.w_re, n0), w_at(a.w_im, n0), a.ldw, y_re, y_im, ldk, n0 > 0);
 			if (rc) return rc;
 		}
 	}
 	if (plan.gram) {
-		rc = gram_product(K, N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk);
+		rc = gram_product(Kp, pad.N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk);
 		if (rc) return rc;
-		rc = conj_product(0, B, K, K, a.x_re, a.x_im, a.ldx, g_re, g_im, ldk, y_re, y_im, ldk, 0);
+		rc = conj_product(0, B, K, Kp, a.x_re, a.x_im, a.ldx, g_re, g_im, ldk, y_re, y_im, ldk, 0);
 		if (rc) return rc;
 		if (!plan.pieces) {
 			hipLaunchKernelGGL(head_gram_norm_kernel, dim3((unsigned) ((B + WAVES - 1) / WAVES)), dim3(TPB), 0, rt().stream, a.x_re, a.x_im, a.ldx, y_re,
@@ -1201,24 +1311,22 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 			CNET_LAUNCH_CHECK();
 		}
 	}
-	if (bwd) hipLaunchKernelGGL(head_finish_kernel<true>, dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, b.st);
+	if (bwd) hipLaunchKernelGGL(head_finish_kernel<true>, dim3((unsigned) pad.B), dim3(TPB), 0, rt().stream, a, b.st);
 	else hipLaunchKernelGGL(head_finish_kernel<false>, dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, b.st);
 	CNET_LAUNCH_CHECK();
 	if (!bwd) return CNET_OK;
 	if (plan.gram) {
-		rc = gram_product(K, B, a.x_re, a.x_im, a.ldx, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk);
+		rc = gram_product(Kp, pad.B, a.xs_re, a.xs_im, ldk, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk);
 		if (rc) return rc;
-		rc = conj_product_pair(false, N, K, K, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw);
+		rc = conj_product_pair(false, N, K, Kp, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw);
 		if (rc) return rc;
 	}
-	for (int n0 = 0; !plan.gram && n0 < N; n0 += np) {
+	for (int n0 = 0; !plan.gram && n0 < N; n0 += np) {  // the logits again, over sqrt(S) and zero where a row is left out
 		const int n = std::min(np, N - n0);
-		if (N > np) {
-			rc = logits(n0, n);
-			if (rc) return rc;
-		}
+		rc = cnet_clinear_fwd(a.xs_re, a.xs_im, ldk, w_at(a.w_re, n0), w_at(a.w_im, n0), a.ldw, z_re, z_im, np, pad.B, Kp, n, 0);
+		if (rc) return rc;
 		const size_t o = (size_t) n0 * lddw;
-		rc = conj_product_pair(true, n, K, B, z_re, z_im, np, a.xs_re, a.xs_im, ldk, dw_re + o, dw_im + o, dws_re ? dws_re + o : nullptr,
+		rc = conj_product_pair(true, n, K, pad.B, z_re, z_im, np, a.xs_re, a.xs_im, ldk, dw_re + o, dw_im + o, dws_re ? dws_re + o : nullptr,
 				dws_re ? dws_im + o : nullptr, lddw, accumulate_dw);
 		if (rc) return rc;
 	}

@@ -383,6 +383,27 @@ def test_vocab_head_a_row_of_nan_stays_in_its_row(gpu):
     assert 0 <= am.download()[4] < N
 
 
+@pytest.mark.parametrize("B,K,N", [(20, 48, 300), (300, 40, 260), (100, 300, 1001), (700, 333, 1100)])
+def test_vocab_head_rows_left_out_may_hold_anything(gpu, B, K, N):
+    """NaN and infinities in rows without a label touch neither the other rows nor the gradient of the weights"""
+    rng = np.random.default_rng(16)
+    x, w, labels = head_data(rng, B, K, N)
+    labels[7] = 2
+    labels[10:15] = -1
+    ref = head_ref(x, w, labels)
+    bad = x.copy()
+    bad[1], bad[10], bad[12, 3] = np.nan, np.inf, -np.inf
+    s, loss, dX, dW = capi.empty(B), capi.empty(B), grad(x.shape, K), grad(w.shape, K)
+    with np.errstate(invalid="ignore"):
+        X = cmat(bad, K)
+    ops.vocab_head_fwd_bwd_sym(X, cmat(w, K), ops.ints(labels), s, loss, None, dX, dW)
+    n = 2 * (K + N) + 64
+    label_n = 24 + np.bincount(labels[labels >= 0], minlength=N).max()
+    near(dz_of(dX), ref["dx"], ref["size_dx"] + label_n / n * ref["label_dx"], n, "dx")
+    near(dz_of(dW), ref["dw"], ref["size_dw"] + label_n / n * ref["label_dw"], n + 2 * B, "dw")
+    assert not loss.download()[labels < 0].any()
+
+
 def test_vocab_head_in_a_graph(gpu):
     rng = np.random.default_rng(14)
     B, K, N = 260, 64, 1000
