@@ -312,25 +312,7 @@ constexpr int HEAD_SLABS = 32;      // parts of the vocabulary that such a row's
 constexpr int HEAD_ROWS = 64;       // rows whose marks one workgroup looks at
 constexpr double TO_DO = -1.0;
 
-// One wavefront per row: S, or the mark that asks for the direct sum (also for a NaN or an overflow on the way)
-__global__ __launch_bounds__(TPB) void head_gram_norm_kernel(const float *__restrict__ xr, const float *__restrict__ xi, long ldx,
-		const float *__restrict__ yr, const float *__restrict__ yi, long ldy, const float *__restrict__ t_re, long ldt, int B, int K, RowState st) {
-	const int lane = threadIdx.x & 63;
-	const long row = (long) blockIdx.x * WAVES + (threadIdx.x >> 6);
-	if (row >= B) return;
-	double sum = 0.0;
-	float diag = 0.f;
-	for (int c = lane; c < K; c += 64) {
-		const float a = xr[row * ldx + c], b = xi[row * ldx + c];
-		sum += (double) a * yr[row * ldy + c] - (double) b * yi[row * ldy + c];
-		diag += (a * a + b * b) * t_re[c * ldt + c];
-	}
-	sum = wave_reduce(sum, SumD());
-	diag = wave_reduce(diag, SumF());
-	if (lane == 0) st.sum[row] = sum >= (double) (GRAM_LEAST * diag) && diag < 3.0e38f ? sum : TO_DO;
-}
-
-// The rows that head_gram_norm_kernel has marked, from w: part[row][slab] = sum |z|^2 over the slab of the vocabulary blockIdx.y.
+// The rows that head_finish_kernel has marked, from w: part[row][slab] = sum |z|^2 over the slab of the vocabulary blockIdx.y.
 // The workgroup lists the marked ones of its HEAD_ROWS rows (in order; usually there are none) and takes them four at a time;
 // a wavefront forms four logits of four rows together, its lanes sharing K.
 __global__ __launch_bounds__(TPB) void head_direct_norm_kernel(const float *__restrict__ xr, const float *__restrict__ xi, long ldx,
@@ -339,7 +321,7 @@ __global__ __launch_bounds__(TPB) void head_direct_norm_kernel(const float *__re
 	__shared__ double lds_d[WAVES];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const int mine = blockIdx.x * HEAD_ROWS + lane;
-	const bool marked = mine < B && st.sum[mine] < 0.0;
+	const bool marked = mine < B && st.sum[min(mine, B - 1)] < 0.0;
 	const unsigned long long set = __ballot(marked);
 	const int count = __popcll(set);
 	if (!count) return;
@@ -443,27 +425,15 @@ __device__ __forceinline__ LabelTerm label_term(const HeadArgs &a, long row, int
 	return l;
 }
 
-// One workgroup per row: S, the label's logit, loss, and the gradient at x: y / S minus the label's row of w times conj(z_label) / m.
-// xs = x / sqrt(S), so that both operands of the weights' gradient come from it: a row that is left out is zero in either, whatever
-// it holds (padding may hold anything), and so are the rows beyond B that fill up the last chunk of that product.
-template <bool BWD>
-__global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st) {
-	__shared__ double lds_d[WAVES];
-	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-	const long row = blockIdx.x;
-	if (BWD && row >= a.B) {
-		for (int c = t; c < a.ldy; c += TPB) a.xs_re[row * a.ldy + c] = a.xs_im[row * a.ldy + c] = 0.f;
-		return;
-	}
-	double sum = st.sum[row];
-	if (sum < 0.0) {
-		sum = 0.0;
-		for (int k = 0; k < HEAD_SLABS; ++k) sum += st.part[row * HEAD_SLABS + k];
-	}
+// What is left to do for a row once its sum |z|^2 is known, by G wavefronts: S, the label's logit, loss, and the gradient at x: y / S
+// minus the label's row of w times conj(z_label) / m.  xs = x / sqrt(S), so that both operands of the weights' gradient come
+// from it: a row that is left out is zero in either, whatever it holds (padding may hold anything).
+template <int G, int V, bool BWD>
+__device__ __forceinline__ void finish_row(const HeadArgs &a, const RowState &st, long row, double sum, double *lds, int t, int lane, int wave) {
 	const float S = clamped((float) sum);
 	int best = a.labels && !a.argmax ? 0 : st.index[row];
 	if (best < 0 || best >= a.N) best = 0;  // a row of NaN has no largest entry
-	const LabelTerm l = label_term<WAVES>(a, row, a.labels ? a.labels[row] : best, S, lds_d, t, lane, wave);
+	const LabelTerm l = label_term<G>(a, row, a.labels ? a.labels[row] : best, S, lds, t, lane, wave);
 	if (t == 0) {
 		a.s[row] = S;
 		if (a.loss) a.loss[row] = l.loss;
@@ -477,27 +447,103 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 	const float *xr = a.x_re + row * a.ldx, *xi = a.x_im + row * a.ldx;
 	const long label_row = (l.label < 0 ? 0 : l.label) * a.ldw;
 	const float inv = 1.0f / S, root = (float) (1.0 / sqrt((double) S));
-	for (int c = t; c < a.ldy; c += TPB) {
+	for (int c = t * V; c < a.ldy; c += 64 * G * V) {
 		const long o = row * a.ldy + c, d = row * a.lddx + c;
-		float s_r = 0.f, s_i = 0.f;
+		float s_r[V] = {}, s_i[V] = {};
 		if (c < a.K) {
-			float g_r = 0.f, g_i = 0.f;
+			float g_r[V] = {}, g_i[V] = {};
 			if (l.live) {
-				const float w_r = a.w_re[label_row + c], w_i = a.w_im[label_row + c];
-				g_r = a.y_re[o] * inv - (l.c_re * w_r - l.c_im * w_i);
-				g_i = a.y_im[o] * inv - (l.c_re * w_i + l.c_im * w_r);
-				s_r = xr[c] * root;
-				s_i = xi[c] * root;
+				float w_r[V], w_i[V];
+				load_v<V>(g_r, a.y_re + o);
+				load_v<V>(g_i, a.y_im + o);
+				load_v<V>(w_r, a.w_re + label_row + c);
+				load_v<V>(w_i, a.w_im + label_row + c);
+				load_v<V>(s_r, xr + c);
+				load_v<V>(s_i, xi + c);
+#pragma unroll
+				for (int k = 0; k < V; ++k) {
+					g_r[k] = g_r[k] * inv - (l.c_re * w_r[k] - l.c_im * w_i[k]);
+					g_i[k] = g_i[k] * inv - (l.c_re * w_i[k] + l.c_im * w_r[k]);
+					s_r[k] *= root;
+					s_i[k] *= root;
+				}
 			}
-			put(a.dx_re + d, g_r, a.accumulate_dx);
-			put(a.dx_im + d, g_i, a.accumulate_dx);
+			auto give = [&](float *p, const float *v, float sign) {
+				float u[V];
+#pragma unroll
+				for (int k = 0; k < V; ++k) u[k] = 0.f;
+				if (a.accumulate_dx) load_v<V>(u, p + d);
+#pragma unroll
+				for (int k = 0; k < V; ++k) u[k] = a.accumulate_dx ? u[k] + sign * v[k] : sign * v[k];
+				store_v<V>(p + d, u);
+			};
+			give(a.dx_re, g_r, 1.f);
+			give(a.dx_im, g_i, 1.f);
 			if (a.dxs_re) {
-				put(a.dxs_re + d, g_r, a.accumulate_dx);
-				put(a.dxs_im + d, -g_i, a.accumulate_dx);
+				give(a.dxs_re, g_r, 1.f);
+				give(a.dxs_im, g_i, -1.f);
 			}
 		}
-		a.xs_re[o] = s_r;
-		a.xs_im[o] = s_i;
+		store_v<V>(a.xs_re + o, s_r);
+		store_v<V>(a.xs_im + o, s_i);
+	}
+}
+
+// T threads per row (64: four rows to a workgroup).  GRAM: the sum is formed here, from x and y; a row whose terms cancel (or that
+// holds a NaN or an overflow) is marked and left to the two kernels behind this one.  Rows beyond B, which fill up the last
+// chunk of the weights' product, become zero.
+template <int T, int V, bool BWD, bool GRAM>
+__global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st, const float *__restrict__ diag_at, long diag_step, int rows) {
+	constexpr int G = T / 64, ROWS = TPB / T;
+	__shared__ double lds_d[WAVES];
+	__shared__ float lds_f[WAVES];
+	const int slot = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
+	const long row = (long) blockIdx.x * ROWS + slot;
+	if (row >= rows) return;
+	if (BWD && row >= a.B) {
+		for (int c = t; c < a.ldy; c += T) a.xs_re[row * a.ldy + c] = a.xs_im[row * a.ldy + c] = 0.f;
+		return;
+	}
+	double sum;
+	if (GRAM) {
+		sum = 0.0;
+		float diag = 0.f;
+		for (int c = t * V; c < a.K; c += T * V) {
+			float x_r[V], x_i[V], y_r[V], y_i[V];
+			load_v<V>(x_r, a.x_re + row * a.ldx + c);
+			load_v<V>(x_i, a.x_im + row * a.ldx + c);
+			load_v<V>(y_r, a.y_re + row * a.ldy + c);
+			load_v<V>(y_i, a.y_im + row * a.ldy + c);
+#pragma unroll
+			for (int k = 0; k < V; ++k) {
+				sum += (double) x_r[k] * y_r[k] - (double) x_i[k] * y_i[k];
+				diag += (x_r[k] * x_r[k] + x_i[k] * x_i[k]) * diag_at[(c + k) * diag_step];
+			}
+		}
+		sum = group_reduce<double, G>(sum, SumD(), lds_d, slot, wave, lane);
+		diag = group_reduce<float, G>(diag, SumF(), lds_f, slot, wave, lane);
+		const bool good = sum >= (double) (GRAM_LEAST * diag) && diag < 3.0e38f;
+		if (t == 0) st.sum[row] = good ? sum : TO_DO;
+		if (!good) return;
+	} else {
+		sum = st.sum[row];
+	}
+	finish_row<G, V, BWD>(a, st, row, sum, lds_d + slot * G, t, lane, wave);
+}
+
+// the marked rows among HEAD_ROWS, once their sums are in st.part
+template <int V, bool BWD>
+__global__ __launch_bounds__(TPB) void head_finish_marked_kernel(const HeadArgs a, RowState st) {
+	__shared__ double lds_d[WAVES];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+	const int first = blockIdx.x * HEAD_ROWS;
+	unsigned long long set = __ballot(first + lane < a.B && st.sum[min(first + lane, a.B - 1)] < 0.0);
+	while (set) {
+		const long row = first + __ffsll((long long) set) - 1;
+		set &= set - 1;
+		double sum = 0.0;
+		for (int k = 0; k < HEAD_SLABS; ++k) sum += st.part[row * HEAD_SLABS + k];
+		finish_row<WAVES, V, BWD>(a, st, row, sum, lds_d, t, lane, wave);
 	}
 }
 
@@ -759,18 +805,19 @@ struct ScatterArgs {
 // off in chunks of equal length, whatever the labels.  The order is the stable one, so a label's rows are added in order.
 constexpr int ORDER_ROWS = 8192;  // rows ordered together (their labels fill 32 KB of LDS); longer batches go block by block
 constexpr int CHUNK = 16;         // ordered rows of one workgroup
-constexpr int RANK_ROWS = 64;     // rows of one workgroup of head_order_kernel
+constexpr int RANK_ROWS = 32;     // rows of one workgroup of head_order_kernel
 
 // Orders the rows [y ORDER_ROWS, ..) by (label, row), rows without a label of the vocabulary last: workgroup (x, y) counts for each of
-// 64 rows how many come before it, its 16 wavefronts sharing the labels to compare with (8192 rows: 67 million comparisons over
-// 128 workgroups; a sorting network in one workgroup takes 80 us for them, this 6).  row_of = -1 and label_of = N where there
+// 32 rows how many come before it, its 32 half wavefronts sharing the labels to compare with (8192 rows: 67 million comparisons over
+// 256 workgroups, 12 us; a sorting network in one workgroup took 80).  row_of = -1 and label_of = N where there
 // is no label.
 __global__ __launch_bounds__(1024) void head_order_kernel(const int *__restrict__ labels, int B, int N, int *__restrict__ row_of,
 		int *__restrict__ label_of) {
 	__shared__ __align__(16) int keys[ORDER_ROWS];
-	__shared__ int count[16][RANK_ROWS];
+	constexpr int SHARES = 1024 / RANK_ROWS;
+	__shared__ int count[SHARES][RANK_ROWS];
 	const int first = blockIdx.y * ORDER_ROWS, n = min(ORDER_ROWS, B - first), n4 = (n + 3) / 4 * 4;
-	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lo = blockIdx.x * RANK_ROWS, i = lo + lane;
+	const int lane = threadIdx.x % RANK_ROWS, share = threadIdx.x / RANK_ROWS, lo = blockIdx.x * RANK_ROWS, i = lo + lane;
 	if (lo >= n) return;
 	for (int k = threadIdx.x; k < n4; k += 1024) {
 		const int label = k < n ? labels[first + k] : -1;
@@ -778,7 +825,7 @@ __global__ __launch_bounds__(1024) void head_order_kernel(const int *__restrict_
 	}
 	__syncthreads();
 	const int key = keys[min(i, n - 1)];
-	const int per = ((n4 / 4 + 15) / 16) * 4, j0 = min(n4, wave * per), j1 = min(n4, j0 + per);
+	const int per = ((n4 / 4 + SHARES - 1) / SHARES) * 4, j0 = min(n4, share * per), j1 = min(n4, j0 + per);
 	int before = 0;
 #pragma unroll 4
 	for (int j = j0; j < j1; j += 4) {
@@ -791,12 +838,12 @@ __global__ __launch_bounds__(1024) void head_order_kernel(const int *__restrict_
 			before += (other.x < limit) + (other.y < limit) + (other.z < limit) + (other.w < limit);
 		}
 	}
-	count[wave][lane] = before;
+	count[share][lane] = before;
 	__syncthreads();
-	if (wave || i >= n) return;
+	if (share || i >= n) return;
 	int rank = 0;
 #pragma unroll
-	for (int w = 0; w < 16; ++w) rank += count[w][lane];
+	for (int k = 0; k < SHARES; ++k) rank += count[k][lane];
 	label_of[first + rank] = key;
 	row_of[first + rank] = key < N ? first + i : -1;
 }
@@ -930,11 +977,13 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 
 // Fills what lies below the diagonal blocks of a Hermitian matrix (`panel` wide, the last, number `last`, as wide as is left) from
 // what lies above them: C[j][i] = conj(C[i][j]).
-// Tiles of 32 x 32 turned over in LDS; blockIdx (x, y) = tile (column, row) of the part that is there.
+// Tiles of 32 x 32 turned over in LDS; blockIdx (x, y) = tile (column, row) of the part that is there.  diag (or NULL) receives the
+// diagonal, which a pass over the rows of x would otherwise gather line by line.
 __global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K, int panel,
-		int last) {
+		int last, float *__restrict__ diag) {
 	__shared__ float tile[2][32][33];
 	const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
+	if (r0 == c0 && diag && threadIdx.x < 32 && r0 + (int) threadIdx.x < K) diag[r0 + threadIdx.x] = c_re[(r0 + threadIdx.x) * (ldc + 1)];
 	if (min(c0 / panel, last) <= min(r0 / panel, last)) return;  // (panel is a multiple of 32)
 	const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 	for (int k = ty; k < 32; k += 8)
@@ -1030,6 +1079,7 @@ static int distill(const DistillArgs &a) {
 struct HeadBuffers {
 	RowState st;
 	float *piece, *y, *xs, *gram;  // planes re, im
+	float *diag;
 	float *x, *w;                  // copies of the operands (HeadPad)
 	int *row_of, *label_of;
 	float *label_part;
@@ -1121,7 +1171,7 @@ static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b
 	const bool label = plan.bwd && !plan.whole;
 	const size_t order = label ? rows : 0, label_part = label ? (size_t) (std::min(pad.B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
 	const size_t copy_x = pad.copy ? 2 * (size_t) pad.B * b.ldk : 0, copy_w = pad.copy ? 2 * (size_t) pad.N * b.ldk : 0;
-	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part + copy_x + copy_w) * sizeof(float));
+	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part + copy_x + copy_w + (plan.gram ? b.ldk : 0)) * sizeof(float));
 	if (!p) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
 	auto take = [&](size_t floats) {
 		float *q = p;
@@ -1138,6 +1188,7 @@ static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b
 	b.y = take(wide);
 	b.xs = take(wide);
 	b.gram = take(square);
+	b.diag = take(plan.gram ? b.ldk : 0);
 	b.label_part = take(label_part);
 	b.row_of = (int *) take(order);
 	b.label_of = (int *) take(order);
@@ -1169,9 +1220,9 @@ static int conj_product_pair(bool a_kmajor, int M, int N, int K, const float *a_
 	return cgemm_pair(a_kmajor, true, 1, M, N, K, ar, ai, lda, br, bi, ldb, cj, cr, ci, ldc, accumulate, 0, 1);
 }
 
-// C = conj(A)^T B, Hermitian
+// C = conj(A)^T B, Hermitian; in panels, its diagonal also goes to diag (or NULL)
 static int gram_product(int K, int L, const float *a_re, const float *a_im, long lda, const float *b_re, const float *b_im, long ldb, float *c_re, float *c_im,
-		long ldc) {
+		long ldc, float *diag) {
 	if (!in_panels(K, L)) return conj_product(1, K, K, L, a_re, a_im, lda, b_re, b_im, ldb, c_re, c_im, ldc, 0);
 	const int last = K / PANEL - 1;  // (the last panel takes what is left, up to twice as much: a small one would not fill the device)
 	for (int i = 0; i <= last; ++i) {
@@ -1181,7 +1232,7 @@ static int gram_product(int K, int L, const float *a_re, const float *a_im, long
 		if (rc) return rc;
 	}
 	const unsigned tiles = (unsigned) ((K + 31) / 32);
-	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, PANEL, last);
+	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, PANEL, last, diag);
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
@@ -1230,6 +1281,39 @@ static int head_score(const HeadArgs &a, int B) {
 #undef CNET_SCORE
 	CNET_LAUNCH_CHECK();
 	hipLaunchKernelGGL(head_score_finish_kernel, dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, part, tiles);
+	CNET_LAUNCH_CHECK();
+	return CNET_OK;
+}
+
+template <int T, int V>
+static void launch_finish(const HeadArgs &a, const RowState &st, bool bwd, bool gram, const float *diag_at, long diag_step, int rows) {
+	const dim3 grid((unsigned) ((rows + TPB / T - 1) / (TPB / T)));
+	if (bwd && gram) hipLaunchKernelGGL((head_finish_kernel<T, V, true, true>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
+	else if (bwd) hipLaunchKernelGGL((head_finish_kernel<T, V, true, false>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
+	else if (gram) hipLaunchKernelGGL((head_finish_kernel<T, V, false, true>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
+	else hipLaunchKernelGGL((head_finish_kernel<T, V, false, false>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
+}
+
+// the pass over the rows behind the products that give y; gram: the sums come from it, with the diagonal of T, one element every diag_step
+static int head_finish(const HeadArgs &a, const RowState &st, bool bwd, bool gram, const float *diag_at, long diag_step, int rows) {
+	auto m4 = [](long v) { return v % 4 == 0; };
+	const bool vec = m4(a.K) && m4(a.ldx) && m4(a.ldw) && (!bwd || m4(a.lddx)) && aligned16(a.x_re) && aligned16(a.x_im) && aligned16(a.w_re) &&
+			aligned16(a.w_im) && aligned16(a.dx_re) && aligned16(a.dx_im) && aligned16(a.dxs_re) && aligned16(a.dxs_im);
+	// a wavefront per row up to 512 columns (or what 128-bit accesses make of them), a workgroup beyond
+	if (vec && a.K <= 512) launch_finish<64, 4>(a, st, bwd, gram, diag_at, diag_step, rows);
+	else if (vec) launch_finish<256, 4>(a, st, bwd, gram, diag_at, diag_step, rows);
+	else if (a.K <= 256) launch_finish<64, 1>(a, st, bwd, gram, diag_at, diag_step, rows);
+	else launch_finish<256, 1>(a, st, bwd, gram, diag_at, diag_step, rows);
+	CNET_LAUNCH_CHECK();
+	if (!gram) return CNET_OK;
+	const unsigned groups = (unsigned) ((a.B + HEAD_ROWS - 1) / HEAD_ROWS);
+	hipLaunchKernelGGL(head_direct_norm_kernel, dim3(groups, HEAD_SLABS), dim3(TPB), 0, rt().stream, a.x_re, a.x_im, a.ldx, a.w_re, a.w_im, a.ldw, a.B, a.K,
+			a.N, st);
+	CNET_LAUNCH_CHECK();
+	if (vec && bwd) hipLaunchKernelGGL((head_finish_marked_kernel<4, true>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
+	else if (vec) hipLaunchKernelGGL((head_finish_marked_kernel<4, false>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
+	else if (bwd) hipLaunchKernelGGL((head_finish_marked_kernel<1, true>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
+	else hipLaunchKernelGGL((head_finish_marked_kernel<1, false>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
@@ -1298,25 +1382,17 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 		}
 	}
 	if (plan.gram) {
-		rc = gram_product(Kp, pad.N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk);
+		rc = gram_product(Kp, pad.N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, b.diag);
 		if (rc) return rc;
 		rc = conj_product(0, B, K, Kp, a.x_re, a.x_im, a.ldx, g_re, g_im, ldk, y_re, y_im, ldk, 0);
 		if (rc) return rc;
-		if (!plan.pieces) {
-			hipLaunchKernelGGL(head_gram_norm_kernel, dim3((unsigned) ((B + WAVES - 1) / WAVES)), dim3(TPB), 0, rt().stream, a.x_re, a.x_im, a.ldx, y_re,
-					y_im, ldk, g_re, ldk, B, K, b.st);
-			CNET_LAUNCH_CHECK();
-			hipLaunchKernelGGL(head_direct_norm_kernel, dim3((unsigned) ((B + HEAD_ROWS - 1) / HEAD_ROWS), HEAD_SLABS), dim3(TPB), 0, rt().stream,
-					a.x_re, a.x_im, a.ldx, a.w_re, a.w_im, a.ldw, B, K, N, b.st);
-			CNET_LAUNCH_CHECK();
-		}
 	}
-	if (bwd) hipLaunchKernelGGL(head_finish_kernel<true>, dim3((unsigned) pad.B), dim3(TPB), 0, rt().stream, a, b.st);
-	else hipLaunchKernelGGL(head_finish_kernel<false>, dim3((unsigned) B), dim3(TPB), 0, rt().stream, a, b.st);
-	CNET_LAUNCH_CHECK();
+	const bool apart = in_panels(Kp, pad.N);  // the diagonal of T lies by itself
+	rc = head_finish(a, b.st, bwd, plan.gram && !plan.pieces, apart ? b.diag : g_re, apart ? 1 : ldk + 1, bwd ? pad.B : B);
+	if (rc) return rc;
 	if (!bwd) return CNET_OK;
 	if (plan.gram) {
-		rc = gram_product(Kp, pad.B, a.xs_re, a.xs_im, ldk, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk);
+		rc = gram_product(Kp, pad.B, a.xs_re, a.xs_im, ldk, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk, nullptr);
 		if (rc) return rc;
 		rc = conj_product_pair(false, N, K, Kp, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw);
 		if (rc) return rc;
