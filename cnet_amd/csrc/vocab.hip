@@ -66,18 +66,23 @@ struct DistillArgs {
 	int rows, cols;
 };
 
-// A row's entries in LDS, `top` of each (floats): index, weight, and the row's values there
+// A row's entries in LDS, each array filled up to a multiple of four: index, weight, and the row's values there
 struct Entries {
 	int *id;
 	float *q, *re, *im;
+	int count;  // with the filling
 };
-__device__ __forceinline__ Entries entries_at(float *lds, int top) { return Entries{(int *) lds, lds + top, lds + 2 * top, lds + 3 * top}; }
+__host__ __device__ __forceinline__ int entry_slots(int top) { return (top + 3) / 4 * 4; }
+__device__ __forceinline__ Entries entries_at(float *lds, int top) {
+	const int n = entry_slots(top);
+	return Entries{(int *) lds, lds + n, lds + 2 * n, lds + 3 * n, n};
+}
 
 // T threads fetch the entries of their row
 template <int T>
 __device__ __forceinline__ void fetch_entries(const DistillArgs &a, const Entries &e, long row, int t) {
-	for (int j = t; j < a.top; j += T) {
-		const int id = a.ids[row * a.top + j];
+	for (int j = t; j < e.count; j += T) {
+		const int id = j < a.top ? a.ids[row * a.top + j] : -1;
 		const bool there = id >= 0 && id < a.cols;
 		e.id[j] = id;
 		e.q[j] = id < 0 ? 0.f : a.probs[row * a.top + j];
@@ -119,11 +124,17 @@ __device__ __forceinline__ void entry_gradients(const DistillArgs &a, const Entr
 		if (id < c0 || id >= c1) continue;
 		float q = 0.f;
 		int first = j;
-		for (int i = a.top - 1; i >= 0; --i)
-			if (e.id[i] == id) {
-				first = i;
-				q += e.q[i];
-			}
+#pragma unroll 4
+		for (int i = 0; i < e.count; i += 4) {
+			const int4 n = *reinterpret_cast<const int4 *>(e.id + i);
+			const float4 p = *reinterpret_cast<const float4 *>(e.q + i);
+			q += n.x == id ? p.x : 0.f;
+			q += n.y == id ? p.y : 0.f;
+			q += n.z == id ? p.z : 0.f;
+			q += n.w == id ? p.w : 0.f;
+			const int at = n.x == id ? i : n.y == id ? i + 1 : n.z == id ? i + 2 : n.w == id ? i + 3 : j;
+			first = min(first, at);
+		}
 		if (first != j) continue;
 		const double m = clamped((double) e.re[j] * e.re[j] + (double) e.im[j] * e.im[j]);
 		const float k = (float) ((double) total / S - q / m);
@@ -134,16 +145,17 @@ __device__ __forceinline__ void entry_gradients(const DistillArgs &a, const Entr
 // The row in registers: T threads hold V x NIT columns each, so z is read once and the gradient written once, 16 bytes per element
 // each way (24 with dz*).  The entries and their values are fetched while the row is on its way.  T = 64: four rows to a workgroup.
 // 
-template <int T, int NIT, int V>
+// LONG: the columns that the registers do not hold are read once more for the gradient (4096 x 50257: 36 of 100).
+template <int T, int NIT, int V, bool LONG>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const DistillArgs a, const int policy) {
 	constexpr int G = T / 64, ROWS = T < TPB ? TPB / T : 1;
-	extern __shared__ float lds[];
+	extern __shared__ __align__(16) float lds[];
 	__shared__ double lds_d[G];
 	__shared__ float2 lds_f[G];
 	const int slot = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
 	const bool live = (long) blockIdx.x * ROWS + slot < a.rows;
 	const long row = live ? (long) blockIdx.x * ROWS + slot : a.rows - 1;
-	const Entries e = entries_at(lds + slot * 4 * a.top, a.top);
+	const Entries e = entries_at(lds + slot * 4 * entry_slots(a.top), a.top);
 	const float *zr = a.z_re + row * a.ldz, *zi = a.z_im + row * a.ldz;
 	float re[NIT][V], im[NIT][V];
 #pragma unroll
@@ -169,6 +181,16 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 		for (int k = 0; k < NIT; ++k)
 #pragma unroll
 			for (int q = 0; q < V; ++q) sum = fma((double) im[k][q], (double) im[k][q], fma((double) re[k][q], (double) re[k][q], sum));
+		if (LONG) {
+#pragma unroll 2
+			for (int c = (NIT * T + t) * V; c < a.cols; c += T * V) {
+				float u[V], v[V];
+				load_v<V>(u, zr + c);
+				load_v<V>(v, zi + c);
+#pragma unroll
+				for (int q = 0; q < V; ++q) sum = fma((double) v[q], (double) v[q], fma((double) u[q], (double) u[q], sum));
+			}
+		}
 		S = clamped((float) group_reduce<double, G>(sum, SumD(), lds_d, 0, wave, lane));
 	} else {
 		S = a.s[row];
@@ -204,43 +226,78 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 				distill_store(a, row, c, re[k][0] * share, -(im[k][0] * share));
 			}
 		}
+		if (LONG) {
+#pragma unroll 2
+			for (int c = (NIT * T + t) * V; c < a.cols; c += T * V) {
+				const long o = row * a.lddz + c;
+				float u[V], v[V], n[V];
+				load_v<V>(u, zr + c);
+				load_v<V>(v, zi + c);
+#pragma unroll
+				for (int q = 0; q < V; ++q) {
+					u[q] *= share;
+					v[q] *= share;
+					n[q] = -v[q];
+				}
+				store_v<V>(a.dz_re + o, u);
+				store_v<V>(a.dz_im + o, n);
+				if (a.dzs_re) {
+					store_v<V>(a.dzs_re + o, u);
+					store_v<V>(a.dzs_im + o, v);
+				}
+			}
+		}
 	}
 	if (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 	else __syncthreads();
 	if (live) entry_gradients<T>(a, e, row, S, sums.y, t, 0, a.cols);
 }
 
-// Rows too long for that, or too few: a row is dealt out to `slabs` workgroups of `width` columns each, in two launches.
-__global__ __launch_bounds__(TPB) void distill_slab_sum_kernel(const DistillArgs a, double *__restrict__ part, int width) {
+// Few long rows: a row is dealt out to workgroups of SLAB columns each, in two launches (its sum, in parts; its gradient).
+constexpr int SLAB_COLS = 8;           // of one thread
+constexpr int SLAB = TPB * SLAB_COLS;
+__global__ __launch_bounds__(TPB) void distill_slab_sum_kernel(const DistillArgs a, double *__restrict__ part) {
 	__shared__ double lds_d[WAVES];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.y;
-	const int c0 = blockIdx.x * width, c1 = min(a.cols, c0 + width);
+	const int c0 = blockIdx.x * SLAB;
 	const float *zr = a.z_re + row * a.ldz, *zi = a.z_im + row * a.ldz;
+	float re[SLAB_COLS], im[SLAB_COLS];
+#pragma unroll
+	for (int k = 0; k < SLAB_COLS; ++k) {
+		const int at = min(c0 + k * TPB + t, a.cols - 1);
+		re[k] = zr[at];
+		im[k] = zi[at];
+	}
 	double sum = 0.0;
-#pragma unroll 8
-	for (int c = c0 + t; c < c1; c += TPB) sum = fma((double) zi[c], (double) zi[c], fma((double) zr[c], (double) zr[c], sum));
+#pragma unroll
+	for (int k = 0; k < SLAB_COLS; ++k)
+		if (c0 + k * TPB + t < a.cols) sum = fma((double) im[k], (double) im[k], fma((double) re[k], (double) re[k], sum));
 	sum = group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane);
 	if (t == 0) part[row * gridDim.x + blockIdx.x] = sum;
 }
 
-__global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, const double *__restrict__ part, int width) {
-	extern __shared__ float lds[];
+__global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, const double *__restrict__ part) {
+	extern __shared__ __align__(16) float lds[];
 	__shared__ double lds_d[WAVES];
 	__shared__ float2 lds_f[WAVES];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.y;
-	const int c0 = blockIdx.x * width, c1 = min(a.cols, c0 + width);
+	const int c0 = blockIdx.x * SLAB, c1 = min(a.cols, c0 + SLAB);
 	const Entries e = entries_at(lds, a.top);
-	fetch_entries<TPB>(a, e, row, t);
-	float S;
-	if (a.loss) {
-		double sum = 0.0;
-		for (int k = t; k < (int) gridDim.x; k += TPB) sum += part[row * gridDim.x + k];
-		S = clamped((float) group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane));
-	} else {
-		S = a.s[row];
+	const float *zr = a.z_re + row * a.ldz, *zi = a.z_im + row * a.ldz;
+	float re[SLAB_COLS], im[SLAB_COLS];
+#pragma unroll
+	for (int k = 0; k < SLAB_COLS; ++k) {
+		const int at = min(c0 + k * TPB + t, a.cols - 1);
+		re[k] = zr[at];
+		im[k] = zi[at];
 	}
+	double sum = 0.0;
+	if (a.loss)
+		for (int k = t; k < (int) gridDim.x; k += TPB) sum += part[row * gridDim.x + k];
+	fetch_entries<TPB>(a, e, row, t);
+	const float S = a.loss ? clamped((float) group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane)) : a.s[row];
 	__syncthreads();
 	float2 sums;
 	entry_sums<TPB>(a, e, S, t, sums.x, sums.y);
@@ -251,9 +308,11 @@ __global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, 
 	}
 	if (!a.dz_re) return;
 	const float share = sums.y / S;
-	const float *zr = a.z_re + row * a.ldz, *zi = a.z_im + row * a.ldz;
-#pragma unroll 4
-	for (int c = c0 + t; c < c1; c += TPB) distill_store(a, row, c, zr[c] * share, -(zi[c] * share));
+#pragma unroll
+	for (int k = 0; k < SLAB_COLS; ++k) {
+		const int c = c0 + k * TPB + t;
+		if (c < a.cols) distill_store(a, row, c, re[k] * share, -(im[k] * share));
+	}
 	__syncthreads();
 	entry_gradients<TPB>(a, e, row, S, sums.y, t, c0, c1);
 }
@@ -1030,46 +1089,36 @@ using namespace cnet;
 static int distill(const DistillArgs &a) {
 	const bool vec = a.cols % 4 == 0 && a.ldz % 4 == 0 && aligned16(a.z_re) && aligned16(a.z_im) && (!a.dz_re || a.lddz % 4 == 0) && aligned16(a.dz_re) &&
 			aligned16(a.dz_im) && aligned16(a.dzs_re) && aligned16(a.dzs_im);
-	const size_t entries = (size_t) 4 * a.top * sizeof(float);
+	const size_t entries = (size_t) 4 * entry_slots(a.top) * sizeof(float);
 	const int cus = rt().prop.multiProcessorCount;
-	// a workgroup holds a row of up to 32768 columns; a longer one, and one of more than 8192 where there are fewer rows than a
-	// quarter of the compute units, is dealt out
-	if (a.cols > 32768 || (a.cols > 8192 && 4 * a.rows < cus)) {
-		const int want = std::max(1, std::min((a.cols + 2047) / 2048, 4 * cus / std::min(a.rows, 4 * cus)));
-		const int width = (a.cols + want - 1) / want, slabs = (a.cols + width - 1) / width;
-		for (int r0 = 0; r0 < a.rows; r0 += 65535) {  // (rows on the y axis of the grid)
-			DistillArgs p = a;
-			p.rows = std::min(a.rows - r0, 65535);
-			p.z_re += (long) r0 * a.ldz, p.z_im += (long) r0 * a.ldz;
-			p.ids += (long) r0 * a.top, p.probs += (long) r0 * a.top;
-			p.s += r0;
-			if (p.loss) p.loss += r0;
-			if (p.dz_re) p.dz_re += (long) r0 * a.lddz, p.dz_im += (long) r0 * a.lddz;
-			if (p.dzs_re) p.dzs_re += (long) r0 * a.lddz, p.dzs_im += (long) r0 * a.lddz;
-			double *part = (double *) workspace((size_t) p.rows * slabs * sizeof(double));
-			if (!part) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
-			const dim3 grid((unsigned) slabs, (unsigned) p.rows);
-			if (p.loss) hipLaunchKernelGGL(distill_slab_sum_kernel, grid, dim3(TPB), 0, rt().stream, p, part, width);
-			hipLaunchKernelGGL(distill_slab_kernel, grid, dim3(TPB), entries, rt().stream, p, part, width);
-			CNET_LAUNCH_CHECK();
-		}
+	// rows that are longer than 8192 columns and fewer than a quarter of the compute units are dealt out; of the others, a workgroup
+	// holds one of up to 32768 columns, and as much of a longer one
+	if (a.cols > 8192 && 4L * a.rows < cus) {
+		const int slabs = (a.cols + SLAB - 1) / SLAB;
+		double *part = (double *) workspace((size_t) a.rows * slabs * sizeof(double));
+		if (!part) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
+		const dim3 grid((unsigned) slabs, (unsigned) a.rows);
+		if (a.loss) hipLaunchKernelGGL(distill_slab_sum_kernel, grid, dim3(TPB), 0, rt().stream, a, part);
+		hipLaunchKernelGGL(distill_slab_kernel, grid, dim3(TPB), entries, rt().stream, a, part);
+		CNET_LAUNCH_CHECK();
 		return CNET_OK;
 	}
 	// (8192 x 32768, read once and written once: 772 us with the streaming hint on both sides, 801 on the stores, 862 on the loads, 824
 	// with none; 5.6 TB/s)
 	const int policy = stream_policy(a.dz_re ? ST_BOTH : ST_LOADS, !a.dz_re ? 2 : a.dzs_re ? 6 : 4, (long) a.rows * a.cols);
-#define CNET_DISTILL(T, E)                                                                                                                     \
+#define CNET_DISTILL(T, E, LONG)                                                                                                                     \
 	do {                                                                                                                                       \
 		const dim3 grid((unsigned) ((a.rows + (T < TPB ? TPB / T : 1) - 1) / (T < TPB ? TPB / T : 1))), block(T < TPB ? TPB : T);                \
-		if (vec) hipLaunchKernelGGL((distill_kernel<T, E / 4, 4>), grid, block, entries * (T < TPB ? TPB / T : 1), rt().stream, a, policy);       \
-		else hipLaunchKernelGGL((distill_kernel<T, E, 1>), grid, block, entries * (T < TPB ? TPB / T : 1), rt().stream, a, policy);               \
+		if (vec) hipLaunchKernelGGL((distill_kernel<T, E / 4, 4, LONG>), grid, block, entries * (T < TPB ? TPB / T : 1), rt().stream, a, policy);       \
+		else hipLaunchKernelGGL((distill_kernel<T, E, 1, LONG>), grid, block, entries * (T < TPB ? TPB / T : 1), rt().stream, a, policy);               \
 	} while (0)
-	if (a.cols <= 512 && a.top <= 64) CNET_DISTILL(64, 8);
-	else if (a.cols <= 2048) CNET_DISTILL(256, 8);
-	else if (a.cols <= 4096) CNET_DISTILL(256, 16);
-	else if (a.cols <= 8192) CNET_DISTILL(256, 32);
-	else if (a.cols <= 16384) CNET_DISTILL(1024, 16);
-	else CNET_DISTILL(1024, 32);
+	if (a.cols <= 512 && a.top <= 64) CNET_DISTILL(64, 8, false);
+	else if (a.cols <= 2048) CNET_DISTILL(256, 8, false);
+	else if (a.cols <= 4096) CNET_DISTILL(256, 16, false);
+	else if (a.cols <= 8192) CNET_DISTILL(256, 32, false);
+	else if (a.cols <= 16384) CNET_DISTILL(1024, 16, false);
+	else if (a.cols <= 32768) CNET_DISTILL(1024, 32, false);
+	else CNET_DISTILL(1024, 32, true);
 #undef CNET_DISTILL
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
@@ -1414,7 +1463,7 @@ extern "C" {
 int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top, float *s, float *loss,
 		int rows, int cols) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 24) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && loss && ldz >= cols);
 	return distill(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, s, loss, nullptr, nullptr, nullptr, nullptr, 0, rows, cols});
@@ -1423,7 +1472,7 @@ int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const in
 int cnet_distill_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, const float *s, const int32_t *ids, const float *probs, int top,
 		float *dz_dz_re, float *dz_dz_im, float *dz_dzs_re, float *dz_dzs_im, int64_t lddz, int rows, int cols) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 24) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && ldz >= cols);
 	CNET_CHECK_ARG(dz_dz_re && dz_dz_im && ((dz_dzs_re == nullptr) == (dz_dzs_im == nullptr)) && lddz >= cols);
@@ -1434,7 +1483,7 @@ int cnet_distill_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, cons
 int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top, float *s, float *loss,
 		float *dz_dz_re, float *dz_dz_im, float *dz_dzs_re, float *dz_dzs_im, int64_t lddz, int rows, int cols) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 24) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && loss && ldz >= cols);
 	CNET_CHECK_ARG(dz_dz_re && dz_dz_im && ((dz_dzs_re == nullptr) == (dz_dzs_im == nullptr)) && lddz >= cols);

@@ -63,7 +63,7 @@ def teacher(rng, rows, cols, top, pad=True):
 
 DISTILL = [(1, 1, 1, 0, 0), (1, 5, 3, 0, 1), (4, 64, 8, 0, 0), (7, 333, 9, 3, 1), (96, 512, 8, 0, 0), (5, 1001, 64, 2, 0), (300, 700, 4, 4, 0),
            (3, 4096, 300, 0, 0), (6, 8200, 1024, 0, 0), (3, 20000, 7, 0, 0), (2, 33000, 50, 0, 0), (1, 100003, 64, 0, 0), (5, 131072, 16, 4, 4),
-           (1030, 36, 2, 0, 0)]
+           (1030, 36, 2, 0, 0), (65, 32772, 5, 0, 0), (66, 33001, 33, 0, 0), (64, 9000, 3, 0, 0), (63, 9001, 3, 0, 0), (2, 300000, 9, 0, 0)]
 
 
 @pytest.mark.parametrize("rows,cols,top,pad,off", DISTILL)
