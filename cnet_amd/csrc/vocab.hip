@@ -49,10 +49,6 @@ __device__ __forceinline__ void store_v(float *p, const float *v) {
 	else p[0] = v[0];
 }
 
-struct SumF2 {
-	__device__ float2 operator()(float2 a, float2 b) const { return make_float2(a.x + b.x, a.y + b.y); }
-};
-
 // ------------------------------------------------------------------------------------------------ distillation
 struct DistillArgs {
 	const float *z_re, *z_im;
@@ -84,25 +80,33 @@ __device__ __forceinline__ void fetch_entries(const DistillArgs &a, const Entrie
 	for (int j = t; j < e.count; j += T) {
 		const int id = j < a.top ? a.ids[row * a.top + j] : -1;
 		const bool there = id >= 0 && id < a.cols;
+		const float q = id < 0 ? 0.f : a.probs[row * a.top + j];
 		e.id[j] = id;
-		e.q[j] = id < 0 ? 0.f : a.probs[row * a.top + j];
+		e.q[j] = q;
 		e.re[j] = there ? a.z_re[row * a.ldz + id] : 0.f;
 		e.im[j] = there ? a.z_im[row * a.ldz + id] : 0.f;
 	}
 }
 
-// one thread's part of the loss, and of the entries' total weight
+// the sum of the weights, formed by every wavefront for itself
+__device__ __forceinline__ float total_weight(const Entries &e, int lane) {
+	float total = 0.f;
+	for (int j = lane; j < e.count; j += 64) total += e.q[j];
+	return wave_reduce(total, SumF());
+}
+
+// one thread's part of the loss
 template <int T>
-__device__ __forceinline__ void entry_sums(const DistillArgs &a, const Entries &e, float S, int t, float &terms, float &total) {
-	terms = total = 0.f;
+__device__ __forceinline__ float loss_terms(const DistillArgs &a, const Entries &e, float S, int t) {
+	float terms = 0.f;
 	for (int j = t; j < a.top; j += T) {
 		const float q = e.q[j];
-		total += q;
 		if (q == 0.f) continue;
 		double p = (double) __builtin_nanf("");
 		if (e.id[j] < a.cols) p = clamped(((double) e.re[j] * e.re[j] + (double) e.im[j] * e.im[j]) / (double) S);
 		terms += q * logf((float) (q / p));
 	}
+	return terms;
 }
 
 __device__ __forceinline__ void distill_store(const DistillArgs &a, long row, int c, float re, float im) {
@@ -150,8 +154,8 @@ template <int T, int NIT, int V, bool LONG>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const DistillArgs a, const int policy) {
 	constexpr int G = T / 64, ROWS = T < TPB ? TPB / T : 1;
 	extern __shared__ __align__(16) float lds[];
-	__shared__ double lds_d[G];
-	__shared__ float2 lds_f[G];
+	__shared__ double lds_d[ROWS * G];
+	__shared__ float lds_f[ROWS * G];
 	const int slot = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
 	const bool live = (long) blockIdx.x * ROWS + slot < a.rows;
 	const long row = live ? (long) blockIdx.x * ROWS + slot : a.rows - 1;
@@ -191,22 +195,15 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 				for (int q = 0; q < V; ++q) sum = fma((double) v[q], (double) v[q], fma((double) u[q], (double) u[q], sum));
 			}
 		}
-		S = clamped((float) group_reduce<double, G>(sum, SumD(), lds_d, 0, wave, lane));
+		S = clamped((float) group_reduce<double, G>(sum, SumD(), lds_d, slot, wave, lane));
 	} else {
 		S = a.s[row];
 	}
 	if (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the entries are this wavefront's own
-	else __syncthreads();
-	float2 sums;
-	entry_sums<T>(a, e, S, t, sums.x, sums.y);
-	sums = group_reduce<float2, G>(sums, SumF2(), lds_f, 0, wave, lane);
-	if (a.loss && t == 0 && live) {
-		a.s[row] = S;
-		a.loss[row] = sums.x;
-	}
-	if (!a.dz_re) return;
-	const float share = sums.y / S;
-	if (live) {
+	else if (!a.loss) __syncthreads();                                   // (the exchange of the sum has had its barriers)
+	const float total = total_weight(e, lane), share = total / S;
+	// the gradient first, the loss while it is on its way to memory
+	if (live && a.dz_re) {
 #pragma unroll
 		for (int k = 0; k < NIT; ++k) {
 			const int c = (k * T + t) * V;
@@ -248,9 +245,17 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 			}
 		}
 	}
+	if (a.loss) {
+		const float loss = group_reduce<float, G>(loss_terms<T>(a, e, S, t), SumF(), lds_f, slot, wave, lane);
+		if (t == 0 && live) {
+			a.s[row] = S;
+			a.loss[row] = loss;
+		}
+	}
+	if (!a.dz_re) return;
 	if (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 	else __syncthreads();
-	if (live) entry_gradients<T>(a, e, row, S, sums.y, t, 0, a.cols);
+	if (live) entry_gradients<T>(a, e, row, S, total, t, 0, a.cols);
 }
 
 // Few long rows: a row is dealt out to workgroups of SLAB columns each, in two launches (its sum, in parts; its gradient).
@@ -280,7 +285,7 @@ __global__ __launch_bounds__(TPB) void distill_slab_sum_kernel(const DistillArgs
 __global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, const double *__restrict__ part) {
 	extern __shared__ __align__(16) float lds[];
 	__shared__ double lds_d[WAVES];
-	__shared__ float2 lds_f[WAVES];
+	__shared__ float lds_f[WAVES];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.y;
 	const int c0 = blockIdx.x * SLAB, c1 = min(a.cols, c0 + SLAB);
@@ -297,24 +302,27 @@ __global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, 
 	if (a.loss)
 		for (int k = t; k < (int) gridDim.x; k += TPB) sum += part[row * gridDim.x + k];
 	fetch_entries<TPB>(a, e, row, t);
-	const float S = a.loss ? clamped((float) group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane)) : a.s[row];
-	__syncthreads();
-	float2 sums;
-	entry_sums<TPB>(a, e, S, t, sums.x, sums.y);
-	sums = group_reduce<float2, WAVES>(sums, SumF2(), lds_f, 0, wave, lane);
-	if (a.loss && t == 0 && blockIdx.x == 0) {
-		a.s[row] = S;
-		a.loss[row] = sums.x;
+	sum = group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane);  // (its barriers are the entries' as well)
+	const float S = a.loss ? clamped((float) sum) : a.s[row];
+	const float total = total_weight(e, lane);
+	if (a.dz_re) {
+		const float share = total / S;
+#pragma unroll
+		for (int k = 0; k < SLAB_COLS; ++k) {
+			const int c = c0 + k * TPB + t;
+			if (c < a.cols) distill_store(a, row, c, re[k] * share, -(im[k] * share));
+		}
+	}
+	if (a.loss && blockIdx.x == 0) {
+		const float loss = group_reduce<float, WAVES>(loss_terms<TPB>(a, e, S, t), SumF(), lds_f, 0, wave, lane);
+		if (t == 0) {
+			a.s[row] = S;
+			a.loss[row] = loss;
+		}
 	}
 	if (!a.dz_re) return;
-	const float share = sums.y / S;
-#pragma unroll
-	for (int k = 0; k < SLAB_COLS; ++k) {
-		const int c = c0 + k * TPB + t;
-		if (c < a.cols) distill_store(a, row, c, re[k] * share, -(im[k] * share));
-	}
 	__syncthreads();
-	entry_gradients<TPB>(a, e, row, S, sums.y, t, c0, c1);
+	entry_gradients<TPB>(a, e, row, S, total, t, c0, c1);
 }
 
 // ------------------------------------------------------------------------------------------------ vocabulary head
