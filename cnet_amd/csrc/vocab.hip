@@ -1085,8 +1085,9 @@ __global__ __launch_bounds__(TPB) void head_pack_kernel(const float *__restrict_
 }
 
 // the gradient of no rows at all
-__global__ __launch_bounds__(TPB) void head_clear_kernel(float *p, long ld, int cols) {
-	for (int c = threadIdx.x; c < cols; c += TPB) p[blockIdx.x * ld + c] = 0.f;
+__global__ __launch_bounds__(TPB) void head_clear_kernel(float *p, long ld, int rows, int cols) {
+	for (long r = blockIdx.x; r < rows; r += gridDim.x)
+		for (int c = threadIdx.x; c < cols; c += TPB) p[r * ld + c] = 0.f;
 }
 
 }  // namespace
@@ -1502,7 +1503,7 @@ int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, 
 int cnet_vocab_head_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw, const int32_t *labels,
 		float *s, float *loss, int32_t *argmax, int B, int K, int N) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && N > 0 && N <= (1 << 30));
+	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && N > 0 && N < (1 << 28));
 	if (!B) return CNET_OK;
 	CNET_CHECK_ARG(x_re && x_im && w_re && w_im && s && (loss || argmax));
 	CNET_CHECK_ARG(ldx >= K && ldw >= K);
@@ -1527,12 +1528,12 @@ int cnet_vocab_head_fwd_bwd_sym(const float *x_re, const float *x_im, int64_t ld
 		int64_t lddx, int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B,
 		int K, int N) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && N > 0 && N <= (1 << 30));
+	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && N > 0 && N < (1 << 28));
 	CNET_CHECK_ARG(dw_dz_re && dw_dz_im && ((dw_dzs_re == nullptr) == (dw_dzs_im == nullptr)) && lddw >= K);
 	if (!B) {
 		if (accumulate_dw) return CNET_OK;
 		for (float *p : {dw_dz_re, dw_dz_im, dw_dzs_re, dw_dzs_im})
-			if (p) hipLaunchKernelGGL(head_clear_kernel, dim3((unsigned) N), dim3(TPB), 0, rt().stream, p, (long) lddw, K);
+			if (p) hipLaunchKernelGGL(head_clear_kernel, dim3((unsigned) std::min(N, 65535)), dim3(TPB), 0, rt().stream, p, (long) lddw, N, K);
 		CNET_LAUNCH_CHECK();
 		return CNET_OK;
 	}

@@ -527,7 +527,8 @@ int cnet_embedding_bwd(const int32_t *tokens, const float *g_dzs_re, const float
  * cnet_norm_join_fwd, behind a block and in front of the next: h = u + scale v .* f s1 (u: the residual path, f: what the block
  *      computed, s1 as above from f) and y = w .* h s2 (s2 from h; w one shared row).  w and y NULL: the last block, h alone.
  *      s, s2: as above.
- * All sums in fp32 over a fixed tree; an infinity or NaN of a row stays in that row.  Results must not overlap operands. */
+ * All sums in fp32 over a fixed tree; an infinity or NaN of a row stays in that row (the weights' gradients sum over the rows).
+ * Fewer than 2^22 rows; results must not overlap operands. */
 int cnet_norm_gate_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *v_re, const float *v_im, int64_t ldv,
                        float *y_re, float *y_im, int64_t ldy, float *s, int rows, int cols, float eps);
 int cnet_norm_join_fwd(const float *u_re, const float *u_im, int64_t ldu, const float *f_re, const float *f_im, int64_t ldf,
@@ -562,7 +563,8 @@ int cnet_norm_join_bwd_sym(const float *f_re, const float *f_im, int64_t ldf, co
  * negative id is padding and left out of everything; a row of padding has loss 0 and gradient 0.  An id >= cols gives its row
  * a NaN loss and counts in Q alone, as a label outside the row does in CrossEntropy.  One entry of weight 1 is CrossEntropy.
  * The gradient is assigned; its dz* half may be NULL.  cnet_distill_fwd_bwd_sym gives the results of the other two in one
- * call.  `loss` may point into memory from cnet_host_alloc. */
+ * call, with z read once where a row fits a workgroup's registers (32768 columns).  `loss` may point into memory from
+ * cnet_host_alloc.  Fewer than 2^22 rows; results must not overlap operands. */
 #define CNET_DISTILL_MAX_TOP 1024
 int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top,
                      float *s, float *loss, int rows, int cols);
@@ -574,15 +576,23 @@ int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, 
 
 /* ---- A Linear to a large vocabulary with its CrossEntropy, without the logits: what cnet_clinear_fwd, cnet_cross_entropy_fwd,
  *      cnet_cross_entropy_bwd_sym and cnet_clinear_bwd_sym compute together, where the [B x N] planes of the logits and of their
- *      gradient (six of them in a training step) would be the largest thing in memory.  The library works on pieces of the
- *      vocabulary in a buffer of its own.
+ *      gradient (six of them in a training step) would be the largest thing in memory.
  * x[B][K], w[N][K]; z = x w^T; s = clamped sum |z|^2, loss = -log max(|z_label|^2 / s, 1e-15), argmax = first index of the largest
- * |z_k|^2.
- * labels[B]: a negative label leaves its row out (loss 0, no gradient); one >= N gives a NaN loss and acts as in
- * cnet_cross_entropy_bwd (no entry is the label).  cnet_vocab_head_fwd: labels NULL takes each row's argmax for its label
+ * |z_k|^2 (as single precision forms it).
+ * labels[B]: a negative label leaves its row out (loss 0, no gradient, whatever the row holds); one >= N gives a NaN loss and acts
+ * as in cnet_cross_entropy_bwd (no entry is the label).  cnet_vocab_head_fwd: labels NULL takes each row's argmax for its label
  * (scoring: loss is then -log of the largest probability); loss or argmax may be NULL, not both.
  * cnet_vocab_head_fwd_bwd_sym: argmax may be NULL; dx and dw are the conjugate pairs of the gradients at x and w, summed over
- * the rows in a fixed order, their dz* halves optional, each with its accumulate flag.  With B == 0 dw is zero (or left). */
+ * the rows in an order that depends on the sizes alone, their dz* halves optional, each with its accumulate flag.  With B == 0 dw
+ * is zero (or left).
+ * How: the loss depends on the logits through a quadratic form of x, so with T = w^H w and P = x^H diag(1 / s) x neither s nor
+ * either gradient needs them (N K^2 + B K^2 products for B N K); rows in directions that w hardly has are summed from w itself.
+ * The smaller heads form the logits in a buffer of the library, whole or in pieces of the vocabulary; a few rows are scored in one
+ * pass over w.  The argmax needs the logits: a step without it is the faster one.  Products of two weights, and of two entries of
+ * x / sqrt(s), are formed in single precision and have to stay within its range.
+ * The buffer holds a few planes of [B x K] and [K x K] or at most about 192 MiB of logits (more only where 64 columns of B rows
+ * are), with one aligned copy of w (up to 2 GiB) where K is not a multiple of 16 or a plane not aligned to 16 bytes.
+ * B < 2^24, N < 2^28; results must not overlap operands. */
 int cnet_vocab_head_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw,
                         const int32_t *labels, float *s, float *loss, int32_t *argmax, int B, int K, int N);
 int cnet_vocab_head_fwd_bwd_sym(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw,
@@ -608,6 +618,8 @@ int cnet_vocab_head_fwd_bwd_sym(const float *x_re, const float *x_im, int64_t ld
  *   CNET_CGEMM_SKINNY_TWO = 0    two small products of one call as two launches (and the gate behind them as launches of its own)
  *   CNET_CGEMM_3M = 0 | 1        initial value of cnet_cgemm_set_products (1: three real products per complex one)
  *   CNET_CGEMM_PACK = 0          large products of misaligned operands on the operands as they are (no aligned copies)
+ *   CNET_HEAD_GRAM = 0 | 1       the vocabulary head never / always through w^H w (default: by what its products cost)
+ *   CNET_HEAD_PIECE_MB = n       size of the buffer for logits in cnet_vocab_head_* (default 192)
  *   CNET_DFT_FOLD = 0            the transform of real samples without folding them about n/2 first
  *   CNET_STREAM_MIN_MB = n       footprint (MiB) from which an elementwise / row launch counts as streaming (default 256)
  *   CNET_STREAM_POLICY = 0..3    cache policy of every streaming launch: plain, hint on loads and stores, hinted stores,

@@ -296,7 +296,7 @@ def test_norm_refusals(gpu):
     def fwd(x_im=x.im.ptr, ldx=8, ldv=8, y_re=y.re.ptr, ldy=8, rows=rows, cols=cols, eps=EPS):
         return lib.cnet_norm_gate_fwd(x.re.ptr, x_im, ldx, *v.p(), ldv, y_re, y.im.ptr, ldy, s.ptr, rows, cols, eps)
     assert fwd() == 0 and fwd(ldv=0) == 0 and fwd(rows=0) == 0
-    assert INVALID == fwd(x_im=None) == fwd(ldx=7) == fwd(ldv=7) == fwd(y_re=None) == fwd(ldy=7) == fwd(rows=-1) == fwd(cols=0)
+    assert INVALID == fwd(x_im=None) == fwd(ldx=7) == fwd(ldv=7) == fwd(y_re=None) == fwd(ldy=7) == fwd(rows=-1) == fwd(cols=0) == fwd(rows=1 << 22)
     assert INVALID == fwd(eps=-1.0) == fwd(eps=float("nan")) == fwd(eps=float("inf")) and b"cnet_norm_gate_fwd" in lib.cnet_last_error()
 
     def bwd(s_=s.ptr, g_im=g.im.ptr, ldg=8, dzs=d.planes[3].ptr, lddx=8, dv_re=dv.planes[0].ptr, lddv=8):

@@ -263,7 +263,7 @@ def test_vocab_head(gpu, B, K, N, pad, off, argmax):
 
 
 @pytest.mark.parametrize("env", [{"CNET_HEAD_GRAM": "0", "CNET_HEAD_PIECE_MB": "1"}, {"CNET_HEAD_GRAM": "1", "CNET_HEAD_PIECE_MB": "1"},
-                                 {"CNET_HEAD_GRAM": "0"}])
+                                 {"CNET_HEAD_GRAM": "0"}, {"CNET_HEAD_GRAM": "1", "CNET_CGEMM_3M": "1"}])
 def test_vocab_head_every_way(gpu, env):
     """through pieces of the logits, through the Gram matrix, and through whole logits, whatever the sizes"""
     script = os.path.join(os.path.dirname(os.path.abspath(__file__)), "gpu_vocab_head_check.py")
@@ -479,6 +479,7 @@ def test_vocab_refusals(gpu):
         return lib.cnet_vocab_head_fwd(x.re.ptr, x_im, ldx, *w.p(), ldw, labels, s, loss, am, B, K, N)
     loss2 = capi.empty(rows)
     assert fwd(loss=loss2.ptr) == 0 and fwd(loss=loss2.ptr, am=None) == 0 and fwd(loss=None) == 0 and fwd(labels=None, loss=loss2.ptr) == 0 and fwd(B=0) == 0
+    assert INVALID == fwd(B=1 << 24) == fwd(N=1 << 28) == distill(rows=1 << 22)
     assert INVALID == fwd(x_im=None) == fwd(ldx=7) == fwd(ldw=7) == fwd(s=None) == fwd(loss=None, am=None) == fwd(B=-1) == fwd(K=0) == fwd(N=0)
 
     def step(labels=lab.ptr, loss=loss2.ptr, am=am.ptr, dx_im=dx.p()[1], dxs=dx.p()[3], lddx=8, dw_re=dw.p()[0], dws=dw.p()[2], lddw=8, ldx=8):
