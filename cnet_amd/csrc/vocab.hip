@@ -616,8 +616,9 @@ __global__ __launch_bounds__(TPB) void head_finish_marked_kernel(const HeadArgs 
 
 // The logits of one row as a whole (two planes of leading dimension ldz, a multiple of four): S, the largest, the label's logit,
 // loss; and, BWD, the logits overwritten with their gradient.  T threads per row.
+// st.c_re != NULL: the label's term is kept out of them, and goes to dx here and to dw behind the products.
 template <int T, bool BWD>
-__global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__restrict__ z_re, float *__restrict__ z_im, long ldz) {
+__global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, RowState st, float *__restrict__ z_re, float *__restrict__ z_im, long ldz) {
 	constexpr int W = T / 64;
 	__shared__ double lds_d[W];
 	__shared__ ArgMax lds_a[W];
@@ -668,6 +669,28 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__
 	if (!BWD) return;
 	keep(l.live);
 	const float inv = 1.0f / S;
+	const bool apart = st.c_re != nullptr;
+	if (apart) {
+		if (t == 0) {
+			st.c_re[row] = l.c_re;
+			st.c_im[row] = l.c_im;
+		}
+		for (int c = t; c < a.K; c += T) {
+			float d_r = 0.f, d_i = 0.f;
+			if (l.label >= 0) {
+				const float w_r = a.w_re[l.label * a.ldw + c], w_i = a.w_im[l.label * a.ldw + c];
+				d_r = l.c_im * w_i - l.c_re * w_r;
+				d_i = -(l.c_re * w_i + l.c_im * w_r);
+			}
+			const long d = row * a.lddx + c;
+			put(a.dx_re + d, d_r, a.accumulate_dx);
+			put(a.dx_im + d, d_i, a.accumulate_dx);
+			if (a.dxs_re) {
+				put(a.dxs_re + d, d_r, a.accumulate_dx);
+				put(a.dxs_im + d, -d_i, a.accumulate_dx);
+			}
+		}
+	}
 	for (int c = 4 * t; c < a.N; c += 4 * T) {
 		if (!l.live) {
 			store_v<4>(zr + c, zero);
@@ -681,7 +704,7 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, float *__
 		for (int k = 0; k < 4; ++k) {
 			u[k] *= inv;
 			v[k] *= -inv;
-			if (c + k == l.label) {
+			if (!apart && c + k == l.label) {
 				u[k] -= l.c_re;
 				v[k] -= l.c_im;
 			}
@@ -1147,6 +1170,7 @@ struct HeadBuffers {
 
 struct HeadPlan {
 	bool bwd, whole, gram, pieces;
+	bool label;  // the label's terms go to dx and dw by themselves
 	int piece_cols;
 };
 
@@ -1168,7 +1192,9 @@ static bool in_panels(int K, int L) { return K >= 2 * PANEL && (double) K * K * 
 
 // Which way the call goes, by what its launches take: a product of m complex multiplications about 4 us + 8 m flop at 130 TFLOP/s,
 // any other kernel about 3 us, plus its bytes.
-//   whole   the logits in one piece, turned into their gradient where they lie; y and dw from it: three products, one kernel
+//   whole   the logits in one piece, turned into their gradient where they lie; dx and dw from it: three products, one kernel.  The
+//           label's large entry among them would cost the products' sums digits as they get long (dx over 40000 entries:
+//           1.2e-6 off, 1e-7 without it), so beyond 4096 terms (4e-7) its terms go by themselves here too
 //   pieces  the logits piece by piece, and a second time for dw; the label's term by itself
 //   gram    T over N, y over K, P = x^H (x / S) over B, dw from it over K; the label's term by itself.  The argmax needs the logits
 //           all the same.
@@ -1188,11 +1214,12 @@ static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	const double label = bwd ? 20 + bytes(60 * b * k) : 0;
 	const double scan = pieces * (product(b * n * k / pieces) + bytes(8 * b * n / pieces));
 	double direct, gram = (in_panels(K, N) ? 0.6 : 1.0) * product(n * k * k) + product(b * k * k) + (argmax ? scan : bytes(16 * b * k) + 3) + bytes(24 * b * k);
-	if (pieces == 1) direct = scan + (bwd ? bytes(16 * b * n) + 2 * product(b * n * k) : 0);
+	if (pieces == 1) direct = scan + (bwd ? bytes(16 * b * n) + 2 * product(b * n * k) + (std::max(B, N) > 4096 ? label : 0) : 0);
 	else direct = scan + bytes(24 * b * k) + (bwd ? pieces * 3 * product(b * n * k / pieces) + label : 0);
 	if (bwd) gram += (in_panels(K, B) ? 0.6 : 1.0) * product(b * k * k) + product(n * k * k) + label;
 	p.gram = (bwd || !argmax) && (forced >= 0 ? forced != 0 : gram < direct);
 	p.whole = !p.gram && pieces == 1;
+	p.label = bwd && (!p.whole || std::max(B, N) > 4096);
 	p.pieces = !p.whole && (argmax || !p.gram);
 	return p;
 }
@@ -1226,7 +1253,7 @@ static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b
 	const size_t piece = plan.pieces || plan.whole ? 2 * (size_t) pad.B * b.piece_cols : 0;
 	const size_t wide = plan.bwd || plan.gram ? 2 * (size_t) pad.B * b.ldk : 0, square = plan.gram ? 2 * (size_t) pad.K * b.ldk : 0;
 	const size_t part = plan.gram && !plan.pieces ? 2 * HEAD_SLABS * rows : 0;
-	const bool label = plan.bwd && !plan.whole;
+	const bool label = plan.label;
 	const size_t order = label ? rows : 0, label_part = label ? (size_t) (std::min(pad.B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
 	const size_t copy_x = pad.copy ? 2 * (size_t) pad.B * b.ldk : 0, copy_w = pad.copy ? 2 * (size_t) pad.N * b.ldk : 0;
 	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part + copy_x + copy_w + (plan.gram ? b.ldk : 0)) * sizeof(float));
@@ -1412,21 +1439,25 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 		if (rc) return rc;
 		// a row of its own workgroup: many threads where the rows are long
 		const dim3 grid((unsigned) (bwd ? pad.B : B));
+		RowState st = b.st;
+		if (!plan.label) st.c_re = st.c_im = nullptr;
 		if (N > 4096) {
-			if (bwd) hipLaunchKernelGGL((head_row_kernel<1024, true>), grid, dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
-			else hipLaunchKernelGGL((head_row_kernel<1024, false>), grid, dim3(1024), 0, rt().stream, a, z_re, z_im, (long) np);
+			if (bwd) hipLaunchKernelGGL((head_row_kernel<1024, true>), grid, dim3(1024), 0, rt().stream, a, st, z_re, z_im, (long) np);
+			else hipLaunchKernelGGL((head_row_kernel<1024, false>), grid, dim3(1024), 0, rt().stream, a, st, z_re, z_im, (long) np);
 		} else {
-			if (bwd) hipLaunchKernelGGL((head_row_kernel<TPB, true>), grid, dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
-			else hipLaunchKernelGGL((head_row_kernel<TPB, false>), grid, dim3(TPB), 0, rt().stream, a, z_re, z_im, (long) np);
+			if (bwd) hipLaunchKernelGGL((head_row_kernel<TPB, true>), grid, dim3(TPB), 0, rt().stream, a, st, z_re, z_im, (long) np);
+			else hipLaunchKernelGGL((head_row_kernel<TPB, false>), grid, dim3(TPB), 0, rt().stream, a, st, z_re, z_im, (long) np);
 		}
 		CNET_LAUNCH_CHECK();
 		if (!bwd) return CNET_OK;
-		if (pad.B == B)  // both in one launch where they are small
+		if (pad.B == B && !plan.label)  // both in one launch where they are small
 			return cnet_clinear_bwd_sym(z_re, z_im, np, a.xs_re, a.xs_im, ldk, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx,
 					a.accumulate_dx, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw, B, K, N);
-		rc = cnet_clinear_bwd_input_sym(z_re, z_im, np, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx, B, K, N, a.accumulate_dx);
+		rc = cnet_clinear_bwd_input_sym(z_re, z_im, np, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx, B, K, N,
+				a.accumulate_dx || plan.label);
 		if (rc) return rc;
-		return cnet_clinear_bwd_weight_sym(z_re, z_im, np, a.xs_re, a.xs_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, pad.B, K, N, accumulate_dw);
+		rc = cnet_clinear_bwd_weight_sym(z_re, z_im, np, a.xs_re, a.xs_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, pad.B, K, N, accumulate_dw);
+		return rc || !plan.label ? rc : head_labels(a, b, B, dw_re, dw_im, dws_re, dws_im, lddw);
 	}
 	for (int n0 = 0; plan.pieces && n0 < N; n0 += np) {
 		const int n = std::min(np, N - n0);

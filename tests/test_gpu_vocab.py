@@ -286,6 +286,32 @@ def test_vocab_head_rows_in_directions_that_the_weights_hardly_have(gpu, weak):
     head_check(B, K, N, argmax=False, data=(x, w, labels))
 
 
+@pytest.mark.parametrize("B,K,N", [(70, 8, 9000), (200, 6, 30000), (5000, 4, 9)])
+def test_vocab_head_a_label_of_little_probability_keeps_its_digits(gpu, B, K, N):
+    """Where the label's logit is small its term, conj(z_l) / |z_l|^2, outweighs everything else in dx and dw.  It takes part in a few
+    operations of its own (the logit, |z_l|^2, the division, the product, for dw the sum of the rows with that label), not in as many
+    roundings as the sum over the vocabulary or the batch."""
+    rng = np.random.default_rng(B + N)
+    x, w = rnd(rng, B, K), rnd(rng, N, K, (2 * K) ** -0.5)
+    labels = rng.integers(0, N, B).astype(np.int32)
+    l = w[labels]
+    x -= ((x * l).sum(1) / (np.abs(l) ** 2).sum(1) * (1 - 1e-5))[:, None] * l.conj()
+    x = x.real.astype(np.float32).astype(np.float64) + 1j * x.imag.astype(np.float32)
+    ref = head_ref(x, w, labels)
+    X, W, L = cmat(x, K), cmat(w, K), ops.ints(labels)
+    s, loss = capi.empty(B), capi.empty(B)
+    dX, dW = grad(x.shape, K), grad(w.shape, K)
+    ops.vocab_head_fwd_bwd_sym(X, W, L, s, loss, None, dX, dW)
+    n = 2 * (K + N) + 64
+    # c: two roundings of z_l, three of |z_l|^2 with z_l's twice, one division; three of the complex product, one of the sum
+    term, same = 12, np.bincount(labels, minlength=N)[:, None]
+    err, bound = np.abs(dz_of(dX) - ref["dx"]), HALF * (term * ref["label_dx"] + 2 * n * ref["size_dx"])
+    assert np.all(err <= bound), (err / bound).max()
+    err, bound = np.abs(dz_of(dW) - ref["dw"]), HALF * ((term + np.minimum(same, 64 + same / 64)) * ref["label_dw"] + 2 * (n + B) * ref["size_dw"])
+    assert np.all(err <= bound), (err / bound).max()
+    assert np.median(ref["label_dx"] / ref["size_dx"]) > 1e4      # what the bounds are about
+
+
 @pytest.mark.parametrize("B,K,N,pad,off", [(1, 40, 17000, 0, 0), (3, 5, 20001, 0, 0), (16, 64, 16500, 4, 0), (17, 33, 9001, 2, 1), (32, 100, 8300, 0, 0),
                                            (40, 30, 6001, 0, 0), (48, 48, 5600, 0, 4), (63, 1, 4200, 0, 0), (64, 130, 4100, 0, 0), (1, 1024, 32768, 0, 0)])
 def test_vocab_head_few_rows_against_a_large_vocabulary(gpu, B, K, N, pad, off):
