@@ -1194,7 +1194,8 @@ static bool in_panels(int K, int L) { return K >= 2 * PANEL && (double) K * K * 
 // any other kernel about 3 us, plus its bytes.
 //   whole   the logits in one piece, turned into their gradient where they lie; dx and dw from it: three products, one kernel.  The
 //           label's large entry among them would cost the products' sums digits as they get long (dx over 40000 entries:
-//           1.2e-6 off, 1e-7 without it), so beyond 4096 terms (4e-7) its terms go by themselves here too
+//           1.6e-6 off, 6e-8 without it), so beyond 4096 terms (2.5e-7) its terms go by themselves here too (300 x 1500 x 40000:
+//           3761 -> 3784 us)
 //   pieces  the logits piece by piece, and a second time for dw; the label's term by itself
 //   gram    T over N, y over K, P = x^H (x / S) over B, dw from it over K; the label's term by itself.  The argmax needs the logits
 //           all the same.
