@@ -15,6 +15,7 @@ namespace cnet {
 int cgemm_pair(bool a_mcontig, bool b_ncontig, int nprob, int M, int N, int K, const float *const a_re[2], const float *const a_im[2], long lda,
 		const float *const b_re[2], const float *const b_im[2], long ldb, const bool conj_b[2], float *const c_re[2], float *const c_im[2],
 		long ldc, int accumulate, int tri, int mirror);
+int cgemm_gram(int K, int L, const float *a_re, const float *a_im, long lda, float *c_re, float *c_im, long ldc);
 }  // namespace cnet
 
 namespace {
@@ -1065,16 +1066,15 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 	dst.subtract(a, label, c, re, im);
 }
 
-// Fills what lies below the diagonal blocks of a Hermitian matrix (`panel` wide, the last, number `last`, as wide as is left) from
-// what lies above them: C[j][i] = conj(C[i][j]).
+// Fills what lies below the diagonal of a Hermitian matrix from what lies above it: C[j][i] = conj(C[i][j]).
 // Tiles of 32 x 32 turned over in LDS; blockIdx (x, y) = tile (column, row) of the part that is there.  diag (or NULL) receives the
 // diagonal, which a pass over the rows of x would otherwise gather line by line.
-__global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K, int panel,
-		int last, float *__restrict__ diag) {
+__global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K,
+		float *__restrict__ diag) {
 	__shared__ float tile[2][32][33];
 	const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
 	if (r0 == c0 && diag && threadIdx.x < 32 && r0 + (int) threadIdx.x < K) diag[r0 + threadIdx.x] = c_re[(r0 + threadIdx.x) * (ldc + 1)];
-	if (min(c0 / panel, last) <= min(r0 / panel, last)) return;  // (panel is a multiple of 32)
+	if (c0 < r0) return;
 	const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 	for (int k = ty; k < 32; k += 8)
 		if (r0 + k < K && c0 + tx < K) {
@@ -1083,7 +1083,7 @@ __global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_
 		}
 	__syncthreads();
 	for (int k = ty; k < 32; k += 8)
-		if (c0 + k < K && r0 + tx < K) {
+		if (c0 + k < K && r0 + tx < K && c0 + k > r0 + tx) {
 			c_re[(long) (c0 + k) * ldc + r0 + tx] = tile[0][tx][k];
 			c_im[(long) (c0 + k) * ldc + r0 + tx] = -tile[1][tx][k];
 		}
@@ -1184,11 +1184,13 @@ static long piece_bytes() {
 	return mb << 20;
 }
 
-// A Hermitian product C = conj(A)^T B (K x K, both operands k-major, L long) in panels of rows that leave out what lies below the
-// diagonal blocks: 1024 x 1024 over 32768 takes 1.24 ms in four panels and 2.09 ms whole, over 8192 0.35 against 0.47 ms; a shorter
-// product would not fill the device with its panels.
-constexpr int PANEL = 256;
-static bool in_panels(int K, int L) { return K >= 2 * PANEL && (double) K * K * L >= (double) (1L << 31); }
+// A Gram matrix (K x K, over L rows): the product leaves out the blocks below the diagonal and a pass of 5 us fills them in, if that
+// is less than what they would take.  A whole call, all blocks / half of them: 8192 rows x 1024 -> 32768 entries 5141 / 3933 us,
+// 2048 x 336 -> 8192 243 / 212, 4000 x 128 -> 30000 170 / 155; but 2000 x 192 -> 8000 128 / 129 and 1000 x 256 -> 4096 106 / 113.
+static bool half_product(int K, int L) { return K > 64 && (double) K * K * L >= 4.0e8; }
+static bool half_product(int K, int L, const float *re, const float *im, long ld) {
+	return half_product(K, L) && ld % 4 == 0 && ld < (1L << 22) && aligned16(re) && aligned16(im);
+}
 
 // Which way the call goes, by what its launches take: a product of m complex multiplications about 4 us + 8 m flop at 130 TFLOP/s,
 // any other kernel about 3 us, plus its bytes.
@@ -1214,10 +1216,10 @@ static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	auto bytes = [](double v) { return 3.0 + v / 4e6; };
 	const double label = bwd ? 20 + bytes(60 * b * k) : 0;
 	const double scan = pieces * (product(b * n * k / pieces) + bytes(8 * b * n / pieces));
-	double direct, gram = (in_panels(K, N) ? 0.6 : 1.0) * product(n * k * k) + product(b * k * k) + (argmax ? scan : bytes(16 * b * k) + 3) + bytes(24 * b * k);
+	double direct, gram = (half_product(K, N) ? 0.6 : 1.0) * product(n * k * k) + product(b * k * k) + (argmax ? scan : bytes(16 * b * k) + 3) + bytes(24 * b * k);
 	if (pieces == 1) direct = scan + (bwd ? bytes(16 * b * n) + 2 * product(b * n * k) + (std::max(B, N) > 4096 ? label : 0) : 0);
 	else direct = scan + bytes(24 * b * k) + (bwd ? pieces * 3 * product(b * n * k / pieces) + label : 0);
-	if (bwd) gram += (in_panels(K, B) ? 0.6 : 1.0) * product(b * k * k) + product(n * k * k) + label;
+	if (bwd) gram += (half_product(K, B) ? 0.6 : 1.0) * product(b * k * k) + product(n * k * k) + label;
 	p.gram = (bwd || !argmax) && (forced >= 0 ? forced != 0 : gram < direct);
 	p.whole = !p.gram && pieces == 1;
 	p.label = bwd && (!p.whole || std::max(B, N) > 4096);
@@ -1306,19 +1308,13 @@ static int conj_product_pair(bool a_kmajor, int M, int N, int K, const float *a_
 	return cgemm_pair(a_kmajor, true, 1, M, N, K, ar, ai, lda, br, bi, ldb, cj, cr, ci, ldc, accumulate, 0, 1);
 }
 
-// C = conj(A)^T B, Hermitian; in panels, its diagonal also goes to diag (or NULL)
-static int gram_product(int K, int L, const float *a_re, const float *a_im, long lda, const float *b_re, const float *b_im, long ldb, float *c_re, float *c_im,
-		long ldc, float *diag) {
-	if (!in_panels(K, L)) return conj_product(1, K, K, L, a_re, a_im, lda, b_re, b_im, ldb, c_re, c_im, ldc, 0);
-	const int last = K / PANEL - 1;  // (the last panel takes what is left, up to twice as much: a small one would not fill the device)
-	for (int i = 0; i <= last; ++i) {
-		const int k0 = i * PANEL;
-		const long o = (long) k0 * ldc + k0;
-		const int rc = conj_product(1, i < last ? PANEL : K - k0, K - k0, L, a_re + k0, a_im + k0, lda, b_re + k0, b_im + k0, ldb, c_re + o, c_im + o, ldc, 0);
-		if (rc) return rc;
-	}
+// C = A^H A [K][K] for an A of L rows; half of it by the product where that pays, its diagonal then to diag (or NULL) as well
+static int gram_product(int K, int L, const float *a_re, const float *a_im, long lda, float *c_re, float *c_im, long ldc, float *diag) {
+	if (!half_product(K, L, a_re, a_im, lda)) return conj_product(1, K, K, L, a_re, a_im, lda, a_re, a_im, lda, c_re, c_im, ldc, 0);
+	const int rc = cgemm_gram(K, L, a_re, a_im, lda, c_re, c_im, ldc);
+	if (rc) return rc;
 	const unsigned tiles = (unsigned) ((K + 31) / 32);
-	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, PANEL, last, diag);
+	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, diag);
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
@@ -1472,17 +1468,17 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 		}
 	}
 	if (plan.gram) {
-		rc = gram_product(Kp, pad.N, a.w_re, a.w_im, a.ldw, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, b.diag);
+		rc = gram_product(Kp, pad.N, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, b.diag);
 		if (rc) return rc;
 		rc = conj_product(0, B, K, Kp, a.x_re, a.x_im, a.ldx, g_re, g_im, ldk, y_re, y_im, ldk, 0);
 		if (rc) return rc;
 	}
-	const bool apart = in_panels(Kp, pad.N);  // the diagonal of T lies by itself
+	const bool apart = half_product(Kp, pad.N, a.w_re, a.w_im, a.ldw);  // the diagonal of T lies by itself
 	rc = head_finish(a, b.st, bwd, plan.gram && !plan.pieces, apart ? b.diag : g_re, apart ? 1 : ldk + 1, bwd ? pad.B : B);
 	if (rc) return rc;
 	if (!bwd) return CNET_OK;
 	if (plan.gram) {
-		rc = gram_product(Kp, pad.B, a.xs_re, a.xs_im, ldk, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk, nullptr);
+		rc = gram_product(Kp, pad.B, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk, nullptr);
 		if (rc) return rc;
 		rc = conj_product_pair(false, N, K, Kp, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw);
 		if (rc) return rc;

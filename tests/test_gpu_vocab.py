@@ -271,12 +271,18 @@ def test_vocab_head_every_way(gpu, env):
     assert res.returncode == 0 and res.stdout.strip().endswith("ok"), res.stdout[-500:] + res.stderr[-2000:]
 
 
+@pytest.mark.parametrize("B,K,N,pad,off", [(900, 528, 1601, 0, 0), (700, 333, 4001, 3, 1), (4100, 320, 700, 0, 4), (400, 129, 24100, 0, 0)])
+def test_vocab_head_half_of_a_gram_matrix(gpu, B, K, N, pad, off):
+    """sizes at which T = w^H w, or P = x^H x / S, is formed above its diagonal and turned over; w in whole chunks of 16 rows and not"""
+    head_check(B, K, N, pad, off, argmax=False)
+
+
+@pytest.mark.parametrize("B,K,N", [(600, 64, 1000), (300, 160, 16000)])
 @pytest.mark.parametrize("weak", [1e-1, 1e-3, 1e-6])
-def test_vocab_head_rows_in_directions_that_the_weights_hardly_have(gpu, weak):
+def test_vocab_head_rows_in_directions_that_the_weights_hardly_have(gpu, weak, B, K, N):
     """Every row of w is one strong direction plus a little noise, and a third of the rows of x is orthogonal to it: there the Gram
     matrix gives sum |z|^2 as a difference of large terms, and the rows are computed again from w."""
     rng = np.random.default_rng(15)
-    B, K, N = 600, 64, 1000
     x, w, labels = head_data(rng, B, K, N)
     axis = np.ones(K) / np.sqrt(K)
     w = rnd(rng, N, 1) * axis + weak * w
