@@ -1089,22 +1089,29 @@ __global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_
 		}
 }
 
-// dst[plane][r][c] = src_plane[r][c] inside rows x cols, zero outside; blockIdx.y = plane.  One thread per four columns of dst.
-__global__ __launch_bounds__(TPB) void head_pack_kernel(const float *__restrict__ s_re, const float *__restrict__ s_im, long lds, int rows, int cols,
-		float *__restrict__ dst, long rows_d, int ldd) {
-	const int groups = ldd / 4;
-	const long idx = (long) blockIdx.x * TPB + threadIdx.x;
+// Copies of both operands: dst[plane][r][c] = src_plane[r][c] inside rows x cols, zero outside.  The first blocks x copy x, the
+// others w; blockIdx.y = plane.  One thread per four columns of dst.
+struct PackArgs {
+	const float *re[2], *im[2];
+	long lds[2];
+	float *dst[2];
+	int rows[2], rows_d[2], blocks_x, cols, ldd;
+};
+__global__ __launch_bounds__(TPB) void head_pack_kernel(const PackArgs a) {
+	const bool w = blockIdx.x >= (unsigned) a.blocks_x;
+	const int groups = a.ldd / 4;
+	const long rows_d = w ? a.rows_d[1] : a.rows_d[0], idx = (long) (blockIdx.x - (w ? a.blocks_x : 0)) * TPB + threadIdx.x;
 	if (idx >= rows_d * groups) return;
 	const long r = idx / groups;
 	const int c0 = (int) (idx - r * groups) * 4;
-	const float *s = (blockIdx.y ? s_im : s_re) + r * lds;
+	const float *s = (w ? (blockIdx.y ? a.im[1] : a.re[1]) : (blockIdx.y ? a.im[0] : a.re[0])) + r * (w ? a.lds[1] : a.lds[0]);
 	float v[4] = {0.f, 0.f, 0.f, 0.f};
-	if (r < rows) {
+	if (r < (w ? a.rows[1] : a.rows[0])) {
 #pragma unroll
 		for (int k = 0; k < 4; ++k)
-			if (c0 + k < cols) v[k] = s[c0 + k];
+			if (c0 + k < a.cols) v[k] = s[c0 + k];
 	}
-	store_v<4>(dst + (blockIdx.y * rows_d + r) * ldd + c0, v);
+	store_v<4>((w ? a.dst[1] : a.dst[0]) + (blockIdx.y * rows_d + r) * a.ldd + c0, v);
 }
 
 // the gradient of no rows at all
@@ -1285,12 +1292,6 @@ static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b
 	return CNET_OK;
 }
 
-static void head_pack(const float *s_re, const float *s_im, long lds, int rows, int cols, float *dst, long rows_d, int ldd) {
-	const long threads = rows_d * (ldd / 4);
-	hipLaunchKernelGGL(head_pack_kernel, dim3((unsigned) ((threads + TPB - 1) / TPB), 2), dim3(TPB), 0, rt().stream, s_re, s_im, lds, rows, cols, dst, rows_d,
-			ldd);
-}
-
 // C = conj(A) B, A row-major or k-major, B k-major
 static int conj_product(int a_kmajor, int M, int N, int K, const float *a_re, const float *a_im, long lda, const float *b_re, const float *b_im, long ldb,
 		float *c_re, float *c_im, long ldc, int accumulate) {
@@ -1413,8 +1414,9 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 	const int np = b.piece_cols, Kp = pad.K;  // Kp: K, or K filled up with zeros where the operands are copies
 	const long ldk = b.ldk;
 	if (pad.copy) {
-		head_pack(a.x_re, a.x_im, a.ldx, B, K, b.x, pad.B, (int) ldk);
-		head_pack(a.w_re, a.w_im, a.ldw, N, K, b.w, pad.N, (int) ldk);
+		auto blocks = [&](int rows) { return (unsigned) (((long) rows * (ldk / 4) + TPB - 1) / TPB); };
+		const PackArgs pk = {{a.x_re, a.w_re}, {a.x_im, a.w_im}, {a.ldx, a.ldw}, {b.x, b.w}, {B, N}, {pad.B, pad.N}, (int) blocks(pad.B), K, (int) ldk};
+		hipLaunchKernelGGL(head_pack_kernel, dim3(blocks(pad.B) + blocks(pad.N), 2), dim3(TPB), 0, rt().stream, pk);
 		CNET_LAUNCH_CHECK();
 		a.x_re = b.x;
 		a.x_im = b.x + (size_t) pad.B * ldk;

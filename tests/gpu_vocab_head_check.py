@@ -10,7 +10,8 @@ from tests.test_gpu_vocab import head_check  # noqa: E402
 
 def main():
     capi.init(0)
-    for B, K, N, pad, off in ((1, 5, 9, 0, 0), (17, 33, 130, 2, 1), (300, 96, 1700, 0, 0), (700, 61, 1100, 3, 0), (9000, 8, 100, 0, 0), (400, 576, 900, 0, 0), (203, 700, 1001, 0, 0), (330, 1001, 600, 0, 0)):
+    for B, K, N, pad, off in ((1, 5, 9, 0, 0), (17, 33, 130, 2, 1), (300, 96, 1700, 0, 0), (700, 61, 1100, 3, 0), (9000, 8, 100, 0, 0), (400, 576, 900, 0, 0), (203, 700, 1001, 0, 0), (330, 1001, 600, 0, 0),
+                              (500, 600, 1200, 0, 0)):
         for argmax in (True, False):
             print(B, K, N, argmax, flush=True)
             head_check(B, K, N, pad, off, argmax)
