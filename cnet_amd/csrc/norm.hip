@@ -101,7 +101,8 @@ __device__ __forceinline__ void store_grad(const Out4 &o, long row, float *re, f
 }
 
 // T threads hold a row in registers, V x NIT columns each: every operand is read once and every result written once.  T = 64: four
-// rows to a workgroup of 256.
+// rows to a workgroup of 256.  Bound by memory: the join at 8192 x 1024 moves 268 MB in 52 us, 5.2 TB/s (a copy of 1 GiB: 5.1); one
+// row of 1024 is a launch, 4.5 us.
 template <int T, int NIT, int V, bool JOIN>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdArgs a, const int policy) {
 	constexpr int G = T / 64, ROWS = T < TPB ? TPB / T : 1;
@@ -197,6 +198,8 @@ struct Sum3Op {
 // Re(e z) - s2 t2 Re(conj(n2) z), come from three sums that do not wait for each other.
 // SECOND: the next block's norm takes part (the join with a gradient at y).
 // KEEP: the weights stay in registers, and the next row's operands are requested before the exchange of this one.
+// Bound by memory: the join at 8192 x 1024 moves 403 MB in 81 us, 5.0 TB/s, 5 us of it norm_sum_kernel (one exchange after the other,
+// with the rows read twice, took 255 us); 515 x 1001 with a gate per row, 25 MB, 8.4 us.
 template <int T, int NIT, int V, bool SECOND, bool KEEP>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdArgs a, const int policy) {
 	constexpr int G = T / 64, R = T < TPB ? TPB / T : 1, NP = SECOND ? 4 : 2;
@@ -360,7 +363,8 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 }
 
 // Rows whose operands do not fit in registers, up to T x V x NIT columns: the same sums, then the operands once more (from the caches:
-// a row of 8192 columns is half a megabyte), of which a thread keeps only its columns' sums over the rows.
+// a row of 8192 columns is half a megabyte), of which a thread keeps only its columns' sums over the rows.  The join at 1024 x 8192:
+// 121 us, and 15 for the sum over the slabs; norm_bwd_wide_kernel takes 172 (8191 columns: 172 both, 4999: 73 against 96).
 template <int T, int NIT, int V, bool SECOND>
 __global__ __launch_bounds__(T) void norm_bwd_twice_kernel(const BwdArgs a) {
 	constexpr int G = T / 64, NP = SECOND ? 4 : 2;
@@ -478,21 +482,24 @@ __global__ __launch_bounds__(T) void norm_bwd_twice_kernel(const BwdArgs a) {
 	}
 }
 
-// Rows wider than the kernels above hold in registers: one workgroup per row, which walks it once per stage.
+constexpr int WIDE = 1024;  // threads of the two kernels for wide rows
+
+// Rows wider than the kernels above hold in registers: one workgroup per row, which walks it once per stage.  400 x 20000: 60 us,
+// 4.3 TB/s (105 with 256 threads).
 template <bool JOIN>
-__global__ __launch_bounds__(TPB) void norm_fwd_wide_kernel(const FwdArgs a) {
-	__shared__ float lds[TPB / 64];
+__global__ __launch_bounds__(WIDE) void norm_fwd_wide_kernel(const FwdArgs a) {
+	__shared__ float lds[WIDE / 64];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.x;
 	const float *xr = a.x.re + row * a.x.ld, *xi = a.x.im + row * a.x.ld;
 	const float *vr = a.v.re + row * a.v.ld, *vi = a.v.im + row * a.v.ld;
 	float sum = 0.f;
-	for (int c = t; c < a.cols; c += TPB) sum += xr[c] * xr[c] + xi[c] * xi[c];
-	sum = group_reduce<float, TPB / 64>(sum, SumF(), lds, 0, wave, lane);
+	for (int c = t; c < a.cols; c += WIDE) sum += xr[c] * xr[c] + xi[c] * xi[c];
+	sum = group_reduce<float, WIDE / 64>(sum, SumF(), lds, 0, wave, lane);
 	const float s = inv_rms(sum, a.cols, a.eps);
 	if (t == 0 && a.s) a.s[row] = s;
 	if (!JOIN) {
-		for (int c = t; c < a.cols; c += TPB) {
+		for (int c = t; c < a.cols; c += WIDE) {
 			const float n_r = xr[c] * s, n_i = xi[c] * s;
 			a.y_re[row * a.ldy + c] = vr[c] * n_r - vi[c] * n_i;
 			a.y_im[row * a.ldy + c] = vr[c] * n_i + vi[c] * n_r;
@@ -500,7 +507,7 @@ __global__ __launch_bounds__(TPB) void norm_fwd_wide_kernel(const FwdArgs a) {
 		return;
 	}
 	float sum2 = 0.f;
-	for (int c = t; c < a.cols; c += TPB) {
+	for (int c = t; c < a.cols; c += WIDE) {
 		const float n_r = xr[c] * s, n_i = xi[c] * s;
 		const float h_r = a.u.re[row * a.u.ld + c] + a.scale * (vr[c] * n_r - vi[c] * n_i);
 		const float h_i = a.u.im[row * a.u.ld + c] + a.scale * (vr[c] * n_i + vi[c] * n_r);
@@ -509,22 +516,23 @@ __global__ __launch_bounds__(TPB) void norm_fwd_wide_kernel(const FwdArgs a) {
 		sum2 += h_r * h_r + h_i * h_i;
 	}
 	if (!a.y_re) return;
-	sum2 = group_reduce<float, TPB / 64>(sum2, SumF(), lds, 0, wave, lane);
+	sum2 = group_reduce<float, WIDE / 64>(sum2, SumF(), lds, 0, wave, lane);
 	const float s2 = inv_rms(sum2, a.cols, a.eps);
 	if (t == 0 && a.s2) a.s2[row] = s2;
 	const float *wr = a.w.re + row * a.w.ld, *wi = a.w.im + row * a.w.ld;
-	for (int c = t; c < a.cols; c += TPB) {
+	for (int c = t; c < a.cols; c += WIDE) {
 		const float n_r = a.h_re[row * a.ldh + c] * s2, n_i = a.h_im[row * a.ldh + c] * s2;
 		a.y_re[row * a.ldy + c] = wr[c] * n_r - wi[c] * n_i;
 		a.y_im[row * a.ldy + c] = wr[c] * n_i + wi[c] * n_r;
 	}
 }
 
-// The same for rows too wide for registers.  A workgroup takes `rows_per_slab` rows one after the other; its columns' sums of dv and dw stay in its own rows of `partial`
-// (each thread always meets the same columns: no atomics, one order), which norm_sum_kernel adds in slab order.
+// The same for rows too wide for registers.  A workgroup takes `rows_per_slab` rows one after the other; its columns' sums of dv and dw
+// stay in its own rows of `partial` (each thread always meets the same columns: no atomics, one order), which norm_sum_kernel adds
+// in slab order.  512 x 16384: 200 us (552 with 256 threads), and 31 for the sum.
 template <bool SECOND>
-__global__ __launch_bounds__(TPB) void norm_bwd_wide_kernel(const BwdArgs a) {
-	__shared__ float lds[TPB / 64];
+__global__ __launch_bounds__(WIDE) void norm_bwd_wide_kernel(const BwdArgs a) {
+	__shared__ float lds[WIDE / 64];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const int r0 = blockIdx.x * a.rows_per_slab, r1 = min(a.rows, r0 + a.rows_per_slab);
 	const bool shared = a.v.ld == 0;
@@ -543,12 +551,12 @@ __global__ __launch_bounds__(TPB) void norm_bwd_wide_kernel(const BwdArgs a) {
 		};
 		float t2 = 0.f;
 		if (SECOND) {
-			for (int c = t; c < a.cols; c += TPB) {
+			for (int c = t; c < a.cols; c += WIDE) {
 				float p_r, p_i, n_r, n_i;
 				next(c, p_r, p_i, n_r, n_i);
 				t2 += p_r * n_r - p_i * n_i;
 			}
-			t2 = group_reduce<float, TPB / 64>(t2, SumF(), lds, 0, wave, lane) * inv_n;
+			t2 = group_reduce<float, WIDE / 64>(t2, SumF(), lds, 0, wave, lane) * inv_n;
 		}
 		// the gradient at the result of the (first) norm and its weights: scale dh, or g
 		auto at = [&](int c, float &d_r, float &d_i) {
@@ -563,7 +571,7 @@ __global__ __launch_bounds__(TPB) void norm_bwd_wide_kernel(const BwdArgs a) {
 		};
 		const float k = a.scale;
 		float t1 = 0.f;
-		for (int c = t; c < a.cols; c += TPB) {
+		for (int c = t; c < a.cols; c += WIDE) {
 			float d_r, d_i;
 			at(c, d_r, d_i);
 			d_r *= k;
@@ -572,8 +580,8 @@ __global__ __launch_bounds__(TPB) void norm_bwd_wide_kernel(const BwdArgs a) {
 			const float n_r = a.x.re[row * a.x.ld + c] * s, n_i = a.x.im[row * a.x.ld + c] * s;
 			t1 += (d_r * v_r - d_i * v_i) * n_r - (d_r * v_i + d_i * v_r) * n_i;
 		}
-		t1 = group_reduce<float, TPB / 64>(t1, SumF(), lds, 0, wave, lane) * inv_n;
-		for (int c = t; c < a.cols; c += TPB) {
+		t1 = group_reduce<float, WIDE / 64>(t1, SumF(), lds, 0, wave, lane) * inv_n;
+		for (int c = t; c < a.cols; c += WIDE) {
 			float d_r, d_i;
 			at(c, d_r, d_i);
 			if (a.du.re) {
@@ -624,7 +632,7 @@ __global__ __launch_bounds__(TPB) void norm_bwd_wide_kernel(const BwdArgs a) {
 }
 
 // dst[plane][c] (+)= sum over slabs; plane 0, 1: `first`, 2, 3: `second`.  COLS (plane, column) pairs per workgroup x LANES lanes that
-// each add one contiguous part of the slabs in order; the lanes' sums are added in lane order.
+// each add one contiguous part of the slabs in order; the lanes' sums are added in lane order.  512 slabs of 4096 sums: 5 us, a launch.
 template <int LANES, int COLS>
 __global__ __launch_bounds__(LANES * COLS) void norm_sum_kernel(const float *__restrict__ partial, int nslabs, int planes, int cols, Out4 first,
 		Out4 second, int accumulate) {
@@ -687,8 +695,8 @@ static int norm_fwd(const FwdArgs &a, bool join) {
 	else if (a.cols <= 4096) launch_fwd<256, 16>(a, join, vec, policy);
 	else if (a.cols <= 8192) launch_fwd<1024, 8>(a, join, vec, policy);
 	else if (a.cols <= 16384) launch_fwd<1024, 16>(a, join, vec, policy);
-	else if (join) hipLaunchKernelGGL(norm_fwd_wide_kernel<true>, dim3((unsigned) a.rows), dim3(TPB), 0, rt().stream, a);
-	else hipLaunchKernelGGL(norm_fwd_wide_kernel<false>, dim3((unsigned) a.rows), dim3(TPB), 0, rt().stream, a);
+	else if (join) hipLaunchKernelGGL(norm_fwd_wide_kernel<true>, dim3((unsigned) a.rows), dim3(WIDE), 0, rt().stream, a);
+	else hipLaunchKernelGGL(norm_fwd_wide_kernel<false>, dim3((unsigned) a.rows), dim3(WIDE), 0, rt().stream, a);
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
@@ -702,6 +710,14 @@ static void launch_bwd(const BwdArgs &a, bool second, bool vec, int nslabs, int 
 	else if (second) hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, true, true>), grid, block, lds, rt().stream, a, policy);
 	else if (vec) hipLaunchKernelGGL((norm_bwd_kernel<T, E / 4, 4, false, true>), grid, block, lds, rt().stream, a, policy);
 	else hipLaunchKernelGGL((norm_bwd_kernel<T, E, 1, false, true>), grid, block, lds, rt().stream, a, policy);
+}
+
+static void launch_bwd_twice(const BwdArgs &a, bool second, bool vec, int nslabs) {
+	const dim3 grid((unsigned) nslabs), block(512);
+	if (second && vec) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 4, 4, true>), grid, block, 0, rt().stream, a);
+	else if (second) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 16, 1, true>), grid, block, 0, rt().stream, a);
+	else if (vec) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 4, 4, false>), grid, block, 0, rt().stream, a);
+	else hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 16, 1, false>), grid, block, 0, rt().stream, a);
 }
 
 // The gate alone is the join without a second norm, without a residual path to hand its gradient to, and with scale 1: its gradient
@@ -727,12 +743,9 @@ static int norm_bwd(BwdArgs &a, const Out4 &dv, const Out4 &dw) {
 	else if (a.cols <= 2048) launch_bwd<512, 4>(a, second, vec, nslabs, policy);
 	else if (a.cols <= 4096 && vec && second) hipLaunchKernelGGL((norm_bwd_kernel<512, 2, 4, true, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a, policy);
 	else if (a.cols <= 4096 && vec) hipLaunchKernelGGL((norm_bwd_kernel<512, 2, 4, false, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a, policy);
-	else if (a.cols <= 8192 && vec && second) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 4, 4, true>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
-	else if (a.cols <= 8192 && vec) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 4, 4, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
-	else if (a.cols <= 8192 && second) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 16, 1, true>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
-	else if (a.cols <= 8192) hipLaunchKernelGGL((norm_bwd_twice_kernel<512, 16, 1, false>), dim3((unsigned) nslabs), dim3(512), 0, rt().stream, a);
-	else if (second) hipLaunchKernelGGL(norm_bwd_wide_kernel<true>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
-	else hipLaunchKernelGGL(norm_bwd_wide_kernel<false>, dim3((unsigned) nslabs), dim3(TPB), 0, rt().stream, a);
+	else if (a.cols <= 8192) launch_bwd_twice(a, second, vec, nslabs);
+	else if (second) hipLaunchKernelGGL(norm_bwd_wide_kernel<true>, dim3((unsigned) nslabs), dim3(WIDE), 0, rt().stream, a);
+	else hipLaunchKernelGGL(norm_bwd_wide_kernel<false>, dim3((unsigned) nslabs), dim3(WIDE), 0, rt().stream, a);
 	CNET_LAUNCH_CHECK();
 	return a.planes ? norm_sum(a.partial, nslabs, a.planes, a.cols, shared ? dv : dw, dw, a.accumulate_w) : CNET_OK;
 }

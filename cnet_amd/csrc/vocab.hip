@@ -148,9 +148,9 @@ __device__ __forceinline__ void entry_gradients(const DistillArgs &a, const Entr
 }
 
 // The row in registers: T threads hold V x NIT columns each, so z is read once and the gradient written once, 16 bytes per element
-// each way (24 with dz*).  The entries and their values are fetched while the row is on its way.  T = 64: four rows to a workgroup.
-// 
-// LONG: the columns that the registers do not hold are read once more for the gradient (4096 x 50257: 36 of 100).
+// each way (24 with dz*), which is what bounds it: 8192 x 32768 takes 802 us, 5.4 TB/s (a copy of 1 GiB: 5.1).  The entries and their
+// values are fetched while the row is on its way.  T = 64: four rows to a workgroup (96 x 512: 4.9 us, a launch).
+// LONG: the columns that the registers do not hold are read once more for the gradient (4096 x 50257, 36 of 100 columns: 786 us).
 template <int T, int NIT, int V, bool LONG>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const DistillArgs a, const int policy) {
 	constexpr int G = T / 64, ROWS = T < TPB ? TPB / T : 1;
@@ -259,7 +259,8 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 	if (live) entry_gradients<T>(a, e, row, S, total, t, 0, a.cols);
 }
 
-// Few long rows: a row is dealt out to workgroups of SLAB columns each, in two launches (its sum, in parts; its gradient).
+// Few long rows: a row is dealt out to workgroups of SLAB columns each, in two launches (its sum, in parts; its gradient).  Bound by
+// the two launches: 3 x 100003 takes 8.5 us (116 with one workgroup per row).
 constexpr int SLAB_COLS = 8;           // of one thread
 constexpr int SLAB = TPB * SLAB_COLS;
 __global__ __launch_bounds__(TPB) void distill_slab_sum_kernel(const DistillArgs a, double *__restrict__ part) {
@@ -335,7 +336,8 @@ struct RowState {   // one entry per row of x, carried from launch to launch
 	float *c_re, *c_im;  // conj(z_label) / m, the label's share of the gradient
 };
 
-// sum |z|^2 and the largest |z|^2 over the columns of one piece of the logits, added to what the earlier pieces left
+// sum |z|^2 and the largest |z|^2 over the columns of one piece of the logits, added to what the earlier pieces left.  Reads the
+// logits from the memory-side cache, where the product has left them (4096 rows of 6144 columns, 201 MB: 34 us, beside 1400 for the product)
 __global__ __launch_bounds__(TPB) void head_piece_kernel(const float *__restrict__ zr, const float *__restrict__ zi, long ldz, int cols, int first_col,
 		RowState st) {
 	__shared__ double lds_d[WAVES];
@@ -382,7 +384,7 @@ constexpr double TO_DO = -1.0;
 
 // The rows that head_finish_kernel has marked, from w: part[row][slab] = sum |z|^2 over the slab of the vocabulary blockIdx.y.
 // The workgroup lists the marked ones of its HEAD_ROWS rows (in order; usually there are none) and takes them four at a time;
-// a wavefront forms four logits of four rows together, its lanes sharing K.
+// a wavefront forms four logits of four rows together, its lanes sharing K.  5 us where nothing is marked.
 __global__ __launch_bounds__(TPB) void head_direct_norm_kernel(const float *__restrict__ xr, const float *__restrict__ xi, long ldx,
 		const float *__restrict__ wr, const float *__restrict__ wi, long ldw, int B, int K, int N, RowState st) {
 	__shared__ int list[HEAD_ROWS];
@@ -560,6 +562,7 @@ __device__ __forceinline__ void finish_row(const HeadArgs &a, const RowState &st
 // T threads per row (64: four rows to a workgroup).  GRAM: the sum is formed here, from x and y; a row whose terms cancel (or that
 // holds a NaN or an overflow) is marked and left to the two kernels behind this one.  Rows beyond B, which fill up the last
 // chunk of the weights' product, become zero.
+// Bound by memory: x, y and the labels' rows of w are read, dx and xs written; 8192 x 1024, 335 MB, takes 74 us, 4.5 TB/s.
 template <int T, int V, bool BWD, bool GRAM>
 __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st, const float *__restrict__ diag_at, long diag_step, int rows) {
 	constexpr int G = T / 64, ROWS = TPB / T;
@@ -599,7 +602,7 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 	finish_row<G, V, BWD>(a, st, row, sum, lds_d + slot * G, t, lane, wave);
 }
 
-// the marked rows among HEAD_ROWS, once their sums are in st.part
+// the marked rows among HEAD_ROWS, once their sums are in st.part (a launch, 5 us, where there are none)
 template <int V, bool BWD>
 __global__ __launch_bounds__(TPB) void head_finish_marked_kernel(const HeadArgs a, RowState st) {
 	__shared__ double lds_d[WAVES];
@@ -616,7 +619,8 @@ __global__ __launch_bounds__(TPB) void head_finish_marked_kernel(const HeadArgs 
 }
 
 // The logits of one row as a whole (two planes of leading dimension ldz, a multiple of four): S, the largest, the label's logit,
-// loss; and, BWD, the logits overwritten with their gradient.  T threads per row.
+// loss; and, BWD, the logits overwritten with their gradient.  T threads per row.  The logits are few enough to be in the caches still:
+// a launch (96 rows of 512: 5 us).
 // st.c_re != NULL: the label's term is kept out of them, and goes to dx here and to dw behind the products.
 template <int T, bool BWD>
 __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, RowState st, float *__restrict__ z_re, float *__restrict__ z_im, long ldz) {
@@ -721,7 +725,9 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, RowState 
 // that every line of w is fetched whole by one lane quarter after the other, and step j of the chunk multiplies the lanes' j-th
 // values (the four k of a matrix instruction are 16 apart; x is laid out in LDS to match).  The next chunk of w is on its way in
 // registers, and that of x for all four wavefronts, while the present one is multiplied.
-// Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one).
+// Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one): 32768 entries of 1024 take 69 us
+// for one row, 3.9 TB/s (a sum over 1 GiB: 3.9), and 121 us for 48, 107 TFLOP/s; two wavefronts per SIMD is what the accumulators and
+// the chunk ahead leave room for, so waits show.
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 struct ScoreTile {   // what a workgroup leaves for every row
@@ -855,7 +861,7 @@ __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B
 	}
 }
 
-// One workgroup per row: its tiles, then its label
+// One workgroup per row: its tiles, then its label (32768 entries: 5 us, a launch)
 __global__ __launch_bounds__(TPB) void head_score_finish_kernel(const HeadArgs a, const ScoreTile *__restrict__ part, int tiles) {
 	__shared__ double lds_d[WAVES];
 	__shared__ ArgMax lds_a[WAVES];
@@ -973,6 +979,7 @@ struct LabelRow {
 // Workgroup (x, y): the ordered rows [CHUNK x, CHUNK x + CHUNK) of the block that starts at `first`, V columns per thread.  A run of
 // one label that lies inside the chunk is subtracted at once; the part of a run that reaches over the chunk's ends goes to
 // part[x][0] (it began before) or part[x][1] (it begins here).
+// Reads x and what it changes of dw: 8192 rows of 1024, 36 us; 1000 of 333, 8 us.
 template <int V>
 __global__ __launch_bounds__(TPB) void head_label_kernel(const ScatterArgs a, int first) {
 	__shared__ int label_at[CHUNK + 2], row_at[CHUNK];  // label_at[k + 1]: ordered row k of the chunk, and its neighbours
@@ -1034,7 +1041,7 @@ __global__ __launch_bounds__(TPB) void head_label_kernel(const ScatterArgs a, in
 	}
 }
 
-// The runs that reach over chunks: the chunk that such a run begins in adds up its parts in order
+// The runs that reach over chunks: the chunk that such a run begins in adds up its parts in order (8192 rows: 15 us)
 template <int V>
 __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs a, int first) {
 	const int c = (blockIdx.y * TPB + threadIdx.x) * V;
@@ -1068,7 +1075,7 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 
 // Fills what lies below the diagonal of a Hermitian matrix from what lies above it: C[j][i] = conj(C[i][j]).
 // Tiles of 32 x 32 turned over in LDS; blockIdx (x, y) = tile (column, row) of the part that is there.  diag (or NULL) receives the
-// diagonal, which a pass over the rows of x would otherwise gather line by line.
+// diagonal, which a pass over the rows of x would otherwise gather line by line.  1024 x 1024: 6 us, a launch and two misses.
 __global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K,
 		float *__restrict__ diag) {
 	__shared__ float tile[2][32][33];
@@ -1090,7 +1097,7 @@ __global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_
 }
 
 // Copies of both operands: dst[plane][r][c] = src_plane[r][c] inside rows x cols, zero outside.  The first blocks x copy x, the
-// others w; blockIdx.y = plane.  One thread per four columns of dst.
+// others w; blockIdx.y = plane.  One thread per four columns of dst.  1000 + 5003 rows of 333: 8 us.
 struct PackArgs {
 	const float *re[2], *im[2];
 	long lds[2];
