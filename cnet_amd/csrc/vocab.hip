@@ -726,8 +726,8 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, RowState 
 // values (the four k of a matrix instruction are 16 apart; x is laid out in LDS to match).  The next chunk of w is on its way in
 // registers, and that of x for all four wavefronts, while the present one is multiplied.
 // Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one): 32768 entries of 1024 take 69 us
-// for one row, 3.9 TB/s (a sum over 1 GiB: 3.9), and 121 us for 48, 107 TFLOP/s; two wavefronts per SIMD is what the accumulators and
-// the chunk ahead leave room for, so waits show.
+// for one row, 3.9 TB/s (a sum over 1 GiB: 3.9), and 121 us for 48, 107 TFLOP/s (the tiles are two wavefronts
+// per SIMD, so waits show).
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 struct ScoreTile {   // what a workgroup leaves for every row
