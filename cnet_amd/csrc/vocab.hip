@@ -1206,12 +1206,19 @@ static bool half_product(int K, int L, const float *re, const float *im, long ld
 	return half_product(K, L) && ld % 4 == 0 && ld < (1L << 22) && aligned16(re) && aligned16(im);
 }
 
+// Whether the label's terms go to dx and dw by themselves where the logits lie whole: three launches, 15 us, for digits.  dx off by,
+// among the others / apart: 300 x 1500 x 40000 1.6e-6 / 6e-8 (3761 -> 3784 us), 531 x 1000 x 4000 8e-7 / 5e-8; what
+// is left among the others (sums of 1024, or calls of less than about 130 us, whose sums the wavefronts share) stays within 5e-7
+// (1000 x 600 x 900, 89 x 1063 x 2620 4e-7, 300 x 128 x 4000 3e-7).
+static bool label_apart(int B, int K, int N) {
+	const int longest = std::max(B, N);
+	return longest > 4096 || (longest > 1024 && (double) B * N * K > (double) (1 << 28));
+}
+
 // Which way the call goes, by what its launches take: a product of m complex multiplications about 4 us + 8 m flop at 130 TFLOP/s,
 // any other kernel about 3 us, plus its bytes.
 //   whole   the logits in one piece, turned into their gradient where they lie; dx and dw from it: three products, one kernel.  The
-//           label's large entry among them would cost the products' sums digits as they get long (dx over 40000 entries:
-//           1.6e-6 off, 6e-8 without it), so beyond 4096 terms (2.5e-7) its terms go by themselves here too (300 x 1500 x 40000:
-//           3761 -> 3784 us)
+//           label's large entry among them costs the products' sums digits as they get long (label_apart)
 //   pieces  the logits piece by piece, and a second time for dw; the label's term by itself
 //   gram    T over N, y over K, P = x^H (x / S) over B, dw from it over K; the label's term by itself.  The argmax needs the logits
 //           all the same.
@@ -1231,12 +1238,12 @@ static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	const double label = bwd ? 20 + bytes(60 * b * k) : 0;
 	const double scan = pieces * (product(b * n * k / pieces) + bytes(8 * b * n / pieces));
 	double direct, gram = (half_product(K, N) ? 0.6 : 1.0) * product(n * k * k) + product(b * k * k) + (argmax ? scan : bytes(16 * b * k) + 3) + bytes(24 * b * k);
-	if (pieces == 1) direct = scan + (bwd ? bytes(16 * b * n) + 2 * product(b * n * k) + (std::max(B, N) > 4096 ? label : 0) : 0);
+	if (pieces == 1) direct = scan + (bwd ? bytes(16 * b * n) + 2 * product(b * n * k) + (label_apart(B, K, N) ? label : 0) : 0);
 	else direct = scan + bytes(24 * b * k) + (bwd ? pieces * 3 * product(b * n * k / pieces) + label : 0);
 	if (bwd) gram += (half_product(K, B) ? 0.6 : 1.0) * product(b * k * k) + product(n * k * k) + label;
 	p.gram = (bwd || !argmax) && (forced >= 0 ? forced != 0 : gram < direct);
 	p.whole = !p.gram && pieces == 1;
-	p.label = bwd && (!p.whole || std::max(B, N) > 4096);
+	p.label = bwd && (!p.whole || label_apart(B, K, N));
 	p.pieces = !p.whole && (argmax || !p.gram);
 	return p;
 }
