@@ -330,7 +330,8 @@ __global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, 
 // ------------------------------------------------------------------------------------------------ vocabulary head
 struct RowState {   // one entry per row of x, carried from launch to launch
 	double *sum;    // sum |z|^2 so far; below zero: still to be added up from `part`
-	double *part;   // [row][HEAD_SLABS]
+	double *part;   // [row][slabs]
+	int slabs;
 	float *best;    // largest |z|^2 so far, and its first index
 	int *index;
 	float *c_re, *c_im;  // conj(z_label) / m, the label's share of the gradient
@@ -378,73 +379,8 @@ __global__ __launch_bounds__(TPB) void head_piece_kernel(const float *__restrict
 // (the sum's size if the columns of w were orthogonal), a row with S < D / 64 is computed again from w itself, so that at most
 // six of the 24 bits are lost to the cancellation.
 constexpr float GRAM_LEAST = 1.0f / 64;
-constexpr int HEAD_SLABS = 32;      // parts of the vocabulary that such a row's logits are dealt out in
-constexpr int HEAD_ROWS = 64;       // rows whose marks one workgroup looks at
+constexpr int HEAD_ROWS = 64;       // rows whose marks one workgroup of head_finish_marked_kernel looks at
 constexpr double TO_DO = -1.0;
-
-// The rows that head_finish_kernel has marked, from w: part[row][slab] = sum |z|^2 over the slab of the vocabulary blockIdx.y.
-// The workgroup lists the marked ones of its HEAD_ROWS rows (in order; usually there are none) and takes them four at a time;
-// a wavefront forms four logits of four rows together, its lanes sharing K.  5 us where nothing is marked.
-__global__ __launch_bounds__(TPB) void head_direct_norm_kernel(const float *__restrict__ xr, const float *__restrict__ xi, long ldx,
-		const float *__restrict__ wr, const float *__restrict__ wi, long ldw, int B, int K, int N, RowState st) {
-	__shared__ int list[HEAD_ROWS];
-	__shared__ double lds_d[WAVES];
-	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-	const int mine = blockIdx.x * HEAD_ROWS + lane;
-	const bool marked = mine < B && st.sum[min(mine, B - 1)] < 0.0;
-	const unsigned long long set = __ballot(marked);
-	const int count = __popcll(set);
-	if (!count) return;
-	if (wave == 0 && marked) list[__popcll(set & ((1ull << lane) - 1))] = mine;
-	__syncthreads();
-	const int per = (N + HEAD_SLABS - 1) / HEAD_SLABS, k0 = min(N, (int) blockIdx.y * per), k1 = min(N, k0 + per);
-	for (int first = 0; first < count; first += 4) {
-		long xo[4];
-#pragma unroll
-		for (int r = 0; r < 4; ++r) xo[r] = (long) list[min(first + r, count - 1)] * ldx;
-		double sum[4] = {0.0, 0.0, 0.0, 0.0};
-		for (int k = k0 + 4 * wave; k < k1; k += 4 * WAVES) {
-			float re[4][4] = {}, im[4][4] = {};
-			for (int c = lane; c < K; c += 64) {
-				float a[4], b[4];
-#pragma unroll
-				for (int r = 0; r < 4; ++r) {
-					a[r] = xr[xo[r] + c];
-					b[r] = xi[xo[r] + c];
-				}
-#pragma unroll
-				for (int q = 0; q < 4; ++q) {
-					const long o = (long) min(k + q, N - 1) * ldw + c;
-					const float d = wr[o], e = wi[o];
-#pragma unroll
-					for (int r = 0; r < 4; ++r) {
-						re[r][q] = fmaf(a[r], d, fmaf(-b[r], e, re[r][q]));
-						im[r][q] = fmaf(a[r], e, fmaf(b[r], d, im[r][q]));
-					}
-				}
-			}
-#pragma unroll
-			for (int r = 0; r < 4; ++r)
-#pragma unroll
-				for (int q = 0; q < 4; ++q) {
-					const float u = wave_reduce(re[r][q], SumF()), v = wave_reduce(im[r][q], SumF());
-					if (k + q < k1) sum[r] += (double) u * u + (double) v * v;
-				}
-		}
-#pragma unroll
-		for (int r = 0; r < 4; ++r) {
-			// (every lane of a wavefront holds the same sum: one lane of each speaks for it)
-			if (lane == 0) lds_d[wave] = sum[r];
-			__syncthreads();
-			if (t == 0 && first + r < count) {
-				double total = lds_d[0];
-				for (int w = 1; w < WAVES; ++w) total += lds_d[w];
-				st.part[(long) list[first + r] * HEAD_SLABS + blockIdx.y] = total;
-			}
-			__syncthreads();
-		}
-	}
-}
 
 struct HeadArgs {
 	const float *x_re, *x_im, *w_re, *w_im;
@@ -613,7 +549,8 @@ __global__ __launch_bounds__(TPB) void head_finish_marked_kernel(const HeadArgs 
 		const long row = first + __ffsll((long long) set) - 1;
 		set &= set - 1;
 		double sum = 0.0;
-		for (int k = 0; k < HEAD_SLABS; ++k) sum += st.part[row * HEAD_SLABS + k];
+		for (int k = lane; k < st.slabs; k += 64) sum += st.part[row * st.slabs + k];
+		sum = wave_reduce(sum, SumD());
 		finish_row<WAVES, V, BWD>(a, st, row, sum, lds_d, t, lane, wave);
 	}
 }
@@ -725,9 +662,8 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, RowState 
 // that every line of w is fetched whole by one lane quarter after the other, and step j of the chunk multiplies the lanes' j-th
 // values (the four k of a matrix instruction are 16 apart; x is laid out in LDS to match).  The next chunk of w is on its way in
 // registers, and that of x for all four wavefronts, while the present one is multiplied.
-// Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one): 32768 entries of 1024 take 69 us
-// for one row, 3.9 TB/s (a sum over 1 GiB: 3.9), and 121 us for 48, 107 TFLOP/s (the tiles are two wavefronts
-// per SIMD, so waits show).
+// Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one): 32768 entries of 1024 take 56 us
+// for one row, 4.8 TB/s (a copy of 1 GiB: 5.1), and 120 us for 48, 107 TFLOP/s (the tiles are two wavefronts per SIMD, so waits show).
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 struct ScoreTile {   // what a workgroup leaves for every row
@@ -749,17 +685,19 @@ __device__ __forceinline__ floatx4 load_quad(const float *p, int k, int K) {
 	return floatx4{p[k], p[k + 1], p[k + 2], p[k + 3]};
 }
 
+constexpr int CHUNK_K = 64;
+// rows of x in LDS: [buffer][plane][four k][row] (an odd pitch: the 16 k groups of a row go to different banks)
+template <int MT>
+struct ScoreRows {
+	floatx4 v[2][2][CHUNK_K / 4][16 * MT + 1];
+};
+
+// The logits of 16 MT rows at the lanes' entries: rr sums xr wr, ii xi wi, ri xr wi + xi wr.  w_re, w_im: the lane's entry; x_at[i]: offset
+// of the row of x that the thread lays out as number (t + TPB i) / 16.
 template <int MT, bool V4>
-__global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B, ScoreTile *__restrict__ part) {
-	constexpr int CHUNK_K = 64, ROWS = 16 * MT, PITCH = ROWS + 1;  // (an odd pitch: the 16 k groups of a row go to different banks)
-	__shared__ floatx4 xs[2][2][CHUNK_K / 4][PITCH];               // [buffer][plane][four k][row]
-	__shared__ ScoreTile met[WAVES][ROWS];
-	const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, q = lane >> 4;
-	const int n0 = (blockIdx.x * WAVES + wave) * 16;
-	// lanes beyond the last entry or row read the last one again; their results are masked
-	const long entry = (long) min(n0 + r, a.N - 1) * a.ldw;
-	const float *w_re = a.w_re + entry, *w_im = a.w_im + entry;
-	floatx4 rr[MT], ii[MT], ri[MT];  // sums of xr wr, xi wi, and xr wi + xi wr
+__device__ __forceinline__ void score_tile(const HeadArgs &a, const float *w_re, const float *w_im, const long (&x_at)[MT], ScoreRows<MT> &xs,
+		floatx4 (&rr)[MT], floatx4 (&ii)[MT], floatx4 (&ri)[MT]) {
+	const int t = threadIdx.x, lane = t & 63, r = lane & 15, q = lane >> 4;
 #pragma unroll
 	for (int m = 0; m < MT; ++m) rr[m] = ii[m] = ri[m] = floatx4{0.f, 0.f, 0.f, 0.f};
 	floatx4 w[2][4], w_next[2][4], x_next[2 * MT];
@@ -773,10 +711,7 @@ __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B
 				w_next[1][j] = load_quad<V4, false>(w_im, k0 + 16 * q + 4 * j, a.K);
 			}
 #pragma unroll
-			for (int i = 0; i < 2 * MT; ++i) {
-				const int at = t + TPB * (i % MT), row = min(at / 16, B - 1);
-				x_next[i] = load_quad<V4, false>((i < MT ? a.x_re : a.x_im) + row * a.ldx, k0 + 4 * (at % 16), a.K);
-			}
+			for (int i = 0; i < 2 * MT; ++i) x_next[i] = load_quad<V4, false>((i < MT ? a.x_re : a.x_im) + x_at[i % MT], k0 + 4 * (t % 16), a.K);
 		} else {
 #pragma unroll
 			for (int j = 0; j < 4; ++j) {
@@ -784,10 +719,7 @@ __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B
 				w_next[1][j] = load_quad<V4, true>(w_im, k0 + 16 * q + 4 * j, a.K);
 			}
 #pragma unroll
-			for (int i = 0; i < 2 * MT; ++i) {
-				const int at = t + TPB * (i % MT), row = min(at / 16, B - 1);
-				x_next[i] = load_quad<V4, true>((i < MT ? a.x_re : a.x_im) + row * a.ldx, k0 + 4 * (at % 16), a.K);
-			}
+			for (int i = 0; i < 2 * MT; ++i) x_next[i] = load_quad<V4, true>((i < MT ? a.x_re : a.x_im) + x_at[i % MT], k0 + 4 * (t % 16), a.K);
 		}
 	};
 	fetch(0);
@@ -798,10 +730,7 @@ __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B
 			for (int j = 0; j < 4; ++j) w[p][j] = w_next[p][j];
 		// (the buffer was last read two chunks ago, before the barrier of the chunk between)
 #pragma unroll
-		for (int i = 0; i < 2 * MT; ++i) {
-			const int at = t + TPB * (i % MT);
-			xs[c & 1][i / MT][at % 16][at / 16] = x_next[i];
-		}
+		for (int i = 0; i < 2 * MT; ++i) xs.v[c & 1][i / MT][t % 16][(t + TPB * (i % MT)) / 16] = x_next[i];
 		__syncthreads();
 		if (c + 1 < chunks) fetch(c + 1);
 		__builtin_amdgcn_sched_barrier(0);  // (the loads go out before the products, not after them)
@@ -810,8 +739,8 @@ __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B
 			floatx4 xr[MT], xi[MT];
 #pragma unroll
 			for (int m = 0; m < MT; ++m) {
-				xr[m] = xs[c & 1][0][4 * q + j][16 * m + r];
-				xi[m] = xs[c & 1][1][4 * q + j][16 * m + r];
+				xr[m] = xs.v[c & 1][0][4 * q + j][16 * m + r];
+				xi[m] = xs.v[c & 1][1][4 * q + j][16 * m + r];
 			}
 #pragma unroll
 			for (int e = 0; e < 4; ++e) {
@@ -826,6 +755,22 @@ __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B
 			}
 		}
 	}
+}
+
+template <int MT, bool V4>
+__global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B, ScoreTile *__restrict__ part) {
+	constexpr int ROWS = 16 * MT;
+	__shared__ ScoreRows<MT> xs;
+	__shared__ ScoreTile met[WAVES][ROWS];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, q = lane >> 4;
+	const int n0 = (blockIdx.x * WAVES + wave) * 16;
+	// lanes beyond the last entry or row read the last one again; their results are masked
+	const long entry = (long) min(n0 + r, a.N - 1) * a.ldw;
+	long x_at[MT];
+#pragma unroll
+	for (int i = 0; i < MT; ++i) x_at[i] = min((t + TPB * i) / 16, B - 1) * a.ldx;
+	floatx4 rr[MT], ii[MT], ri[MT];
+	score_tile<MT, V4>(a, a.w_re + entry, a.w_im + entry, x_at, xs, rr, ii, ri);
 	// element i of a lane: entry n0 + r, row 16 m + 4 q + i; the 16 lanes of a quarter are combined in a fixed order
 	const bool in = n0 + r < a.N;
 #pragma unroll
@@ -896,6 +841,92 @@ struct ScatterArgs {
 	long ldk;
 	int B, K, N;
 };
+
+// ---- The rows that head_finish_kernel has marked, from w: part[row][slab] = sum |z|^2 over the slab blockIdx.x of the vocabulary, `per`
+// tiles of 64 entries.  A workgroup lists the marked ones of the DIRECT_BLOCK rows blockIdx.z (usually there are none: 5 us for the
+// launch) and takes them 32 at a time, every gridDim.y-th such group, in the way of the kernel above; what it finds for a row does
+// not depend on the rows beside it.  Of 8192 rows of 1024 -> 32768 entries, with none, a hundredth, a tenth and all of them marked, a
+// training step takes 4.4, 5.1, 6.9 and 22.8 ms (with four rows at a time on the vector unit 7.1, 23, 26 and 56).
+constexpr int DIRECT_BLOCK = 4096, DIRECT_MT = 2;
+template <bool V4>
+__global__ __launch_bounds__(TPB) void head_direct_kernel(const HeadArgs a, RowState st, int per) {
+	constexpr int MT = DIRECT_MT, ROWS = 16 * MT, EACH = DIRECT_BLOCK / TPB;
+	__shared__ ScoreRows<MT> xs;
+	__shared__ double met[WAVES][ROWS];
+	__shared__ unsigned short list[DIRECT_BLOCK];
+	__shared__ int found[WAVES];
+	const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, q = lane >> 4;
+	const long base = (long) blockIdx.z * DIRECT_BLOCK;
+	unsigned marks = 0;
+#pragma unroll
+	for (int i = 0; i < EACH; ++i) {
+		const long row = base + i * TPB + t;
+		marks |= (row < a.B && st.sum[min(row, (long) a.B - 1)] < 0.0 ? 1u : 0u) << i;
+	}
+	int mine = 0;
+#pragma unroll
+	for (int i = 0; i < EACH; ++i) mine += __popcll(__ballot(marks >> i & 1));
+	if (lane == 0) found[wave] = mine;
+	__syncthreads();
+	int at = 0, count = 0;
+#pragma unroll
+	for (int w = 0; w < WAVES; ++w) {
+		if (w < wave) at += found[w];
+		count += found[w];
+	}
+	if (!count) return;
+	for (int i = 0; i < EACH; ++i) {
+		const unsigned long long set = __ballot(marks >> i & 1);
+		if (marks >> i & 1) list[at + __popcll(set & ((1ull << lane) - 1))] = (unsigned short) (i * TPB + t);
+		at += __popcll(set);
+	}
+	__syncthreads();
+	const int tiles = (a.N + 16 * WAVES - 1) / (16 * WAVES), tile0 = blockIdx.x * per, tile1 = min(tiles, tile0 + per);
+	for (int first = blockIdx.y * ROWS; first < count; first += gridDim.y * ROWS) {
+		long x_at[MT];
+#pragma unroll
+		for (int i = 0; i < MT; ++i) x_at[i] = (base + list[min(first + (t + TPB * i) / 16, count - 1)]) * a.ldx;
+		double sum[MT][4];
+#pragma unroll
+		for (int m = 0; m < MT; ++m)
+#pragma unroll
+			for (int i = 0; i < 4; ++i) sum[m][i] = 0.0;
+		for (int tile = tile0; tile < tile1; ++tile) {
+			const int n = (tile * WAVES + wave) * 16 + r;
+			const long entry = (long) min(n, a.N - 1) * a.ldw;
+			floatx4 rr[MT], ii[MT], ri[MT];
+			__syncthreads();  // (the buffers' last readers)
+			score_tile<MT, V4>(a, a.w_re + entry, a.w_im + entry, x_at, xs, rr, ii, ri);
+			if (n < a.N) {
+#pragma unroll
+				for (int m = 0; m < MT; ++m)
+#pragma unroll
+					for (int i = 0; i < 4; ++i) {
+						const float z_r = rr[m][i] - ii[m][i], z_i = ri[m][i];
+						sum[m][i] = fma((double) z_i, (double) z_i, fma((double) z_r, (double) z_r, sum[m][i]));
+					}
+			}
+		}
+#pragma unroll
+		for (int m = 0; m < MT; ++m)
+#pragma unroll
+			for (int i = 0; i < 4; ++i) {
+				double v = sum[m][i];
+				v += exchange<double, 0>(v);
+				v += exchange<double, 1>(v);
+				v += exchange<double, 2>(v);
+				v += exchange<double, 3>(v);
+				if (r == 0) met[wave][16 * m + 4 * q + i] = v;
+			}
+		__syncthreads();
+		if (t < ROWS && first + t < count) {
+			double v = met[0][t];
+			for (int w = 1; w < WAVES; ++w) v += met[w][t];
+			st.part[(base + list[first + t]) * st.slabs + blockIdx.x] = v;
+		}
+		// (met is written again behind the barriers of the next group's tiles)
+	}
+}
 
 // ---- The label's term of the weights' gradient: dw[label[r]] -= c_r x_r for every row r.  Labels of a text repeat (the most
 // frequent token of a batch of 8192 names hundreds of rows), so the rows are put in order of their labels first and then worked
@@ -1179,6 +1210,7 @@ struct HeadBuffers {
 	int *row_of, *label_of;
 	float *label_part;
 	int piece_cols;                // columns of one piece, also its leading dimension
+	int per;                       // tiles of head_direct_kernel to a slab
 	long ldk;                      // leading dimension of y, xs and gram
 };
 
@@ -1276,7 +1308,11 @@ static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b
 	const size_t rows = ((size_t) pad.B + 63) / 64 * 64;
 	const size_t piece = plan.pieces || plan.whole ? 2 * (size_t) pad.B * b.piece_cols : 0;
 	const size_t wide = plan.bwd || plan.gram ? 2 * (size_t) pad.B * b.ldk : 0, square = plan.gram ? 2 * (size_t) pad.K * b.ldk : 0;
-	const size_t part = plan.gram && !plan.pieces ? 2 * HEAD_SLABS * rows : 0;
+	// the parts of the vocabulary that a marked row is dealt out in: at most an eighth of what y takes for the row, or 32
+	const int tiles = (pad.N + 16 * WAVES - 1) / (16 * WAVES), most = std::min(128, std::max(32, pad.K / 8));
+	b.per = (tiles + most - 1) / most;
+	b.st.slabs = (tiles + b.per - 1) / b.per;
+	const size_t part = plan.gram && !plan.pieces ? 2 * (size_t) b.st.slabs * rows : 0;
 	const bool label = plan.label;
 	const size_t order = label ? rows : 0, label_part = label ? (size_t) (std::min(pad.B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
 	const size_t copy_x = pad.copy ? 2 * (size_t) pad.B * b.ldk : 0, copy_w = pad.copy ? 2 * (size_t) pad.N * b.ldk : 0;
@@ -1392,7 +1428,7 @@ static void launch_finish(const HeadArgs &a, const RowState &st, bool bwd, bool 
 }
 
 // the pass over the rows behind the products that give y; gram: the sums come from it, with the diagonal of T, one element every diag_step
-static int head_finish(const HeadArgs &a, const RowState &st, bool bwd, bool gram, const float *diag_at, long diag_step, int rows) {
+static int head_finish(const HeadArgs &a, const RowState &st, int per, bool bwd, bool gram, const float *diag_at, long diag_step, int rows) {
 	auto m4 = [](long v) { return v % 4 == 0; };
 	const bool vec = m4(a.K) && m4(a.ldx) && m4(a.ldw) && (!bwd || m4(a.lddx)) && aligned16(a.x_re) && aligned16(a.x_im) && aligned16(a.w_re) &&
 			aligned16(a.w_im) && aligned16(a.dx_re) && aligned16(a.dx_im) && aligned16(a.dxs_re) && aligned16(a.dxs_im);
@@ -1404,8 +1440,13 @@ static int head_finish(const HeadArgs &a, const RowState &st, bool bwd, bool gra
 	CNET_LAUNCH_CHECK();
 	if (!gram) return CNET_OK;
 	const unsigned groups = (unsigned) ((a.B + HEAD_ROWS - 1) / HEAD_ROWS);
-	hipLaunchKernelGGL(head_direct_norm_kernel, dim3(groups, HEAD_SLABS), dim3(TPB), 0, rt().stream, a.x_re, a.x_im, a.ldx, a.w_re, a.w_im, a.ldw, a.B, a.K,
-			a.N, st);
+	// (as many workgroups as fill the device twice share the groups of marked rows, should there be many)
+	const unsigned blocks = (unsigned) ((a.B + DIRECT_BLOCK - 1) / DIRECT_BLOCK);
+	const unsigned share = (unsigned) std::max(1, std::min(DIRECT_BLOCK / (16 * DIRECT_MT), 2 * rt().prop.multiProcessorCount / (int) (st.slabs * blocks)));
+	const dim3 grid((unsigned) st.slabs, share, blocks);
+	if (m4(a.ldx) && m4(a.ldw) && aligned16(a.x_re) && aligned16(a.x_im) && aligned16(a.w_re) && aligned16(a.w_im))
+		hipLaunchKernelGGL(head_direct_kernel<true>, grid, dim3(TPB), 0, rt().stream, a, st, per);
+	else hipLaunchKernelGGL(head_direct_kernel<false>, grid, dim3(TPB), 0, rt().stream, a, st, per);
 	CNET_LAUNCH_CHECK();
 	if (vec && bwd) hipLaunchKernelGGL((head_finish_marked_kernel<4, true>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
 	else if (vec) hipLaunchKernelGGL((head_finish_marked_kernel<4, false>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
@@ -1490,7 +1531,7 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 		if (rc) return rc;
 	}
 	const bool apart = half_product(Kp, pad.N, a.w_re, a.w_im, a.ldw);  // the diagonal of T lies by itself
-	rc = head_finish(a, b.st, bwd, plan.gram && !plan.pieces, apart ? b.diag : g_re, apart ? 1 : ldk + 1, bwd ? pad.B : B);
+	rc = head_finish(a, b.st, b.per, bwd, plan.gram && !plan.pieces, apart ? b.diag : g_re, apart ? 1 : ldk + 1, bwd ? pad.B : B);
 	if (rc) return rc;
 	if (!bwd) return CNET_OK;
 	if (plan.gram) {

@@ -5,7 +5,7 @@ import sys
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from cnet_amd import capi  # noqa: E402
-from tests.test_gpu_vocab import head_check  # noqa: E402
+from tests.test_gpu_vocab import head_check, weak_data  # noqa: E402
 
 
 def main():
@@ -15,6 +15,10 @@ def main():
         for argmax in (True, False):
             print(B, K, N, argmax, flush=True)
             head_check(B, K, N, pad, off, argmax)
+    # rows whose sum is formed again from w: in two blocks of rows, all of them, a few beside the end, unaligned
+    for B, K, N, pad, off, every in ((4300, 24, 100, 0, 0, 3), (150, 200, 400, 0, 0, 1), (129, 72, 65, 4, 0, 128), (500, 61, 900, 2, 1, 2), (40, 130, 9000, 0, 0, 1)):
+        print(B, K, N, "weak", flush=True)
+        head_check(B, K, N, pad, off, False, weak_data(B, K, N, 1e-3, every))
 
 
 if __name__ == "__main__":

@@ -277,19 +277,23 @@ def test_vocab_head_half_of_a_gram_matrix(gpu, B, K, N, pad, off):
     head_check(B, K, N, pad, off, argmax=False)
 
 
-@pytest.mark.parametrize("B,K,N", [(600, 64, 1000), (300, 160, 16000)])
-@pytest.mark.parametrize("weak", [1e-1, 1e-3, 1e-6])
-def test_vocab_head_rows_in_directions_that_the_weights_hardly_have(gpu, weak, B, K, N):
-    """Every row of w is one strong direction plus a little noise, and a third of the rows of x is orthogonal to it: there the Gram
-    matrix gives sum |z|^2 as a difference of large terms, and the rows are computed again from w."""
+def weak_data(B, K, N, weak, every=3):
+    """rows of w that are one strong direction plus a little noise; every third row of x is orthogonal to that"""
     rng = np.random.default_rng(15)
     x, w, labels = head_data(rng, B, K, N)
     axis = np.ones(K) / np.sqrt(K)
     w = rnd(rng, N, 1) * axis + weak * w
-    x[::3] -= (x[::3] @ axis)[:, None] * axis
+    x[::every] -= (x[::every] @ axis)[:, None] * axis
     x, w = (z.real.astype(np.float32).astype(np.float64) + 1j * z.imag.astype(np.float32) for z in (x, w))
     labels[7] = 1
-    head_check(B, K, N, argmax=False, data=(x, w, labels))
+    return x, w, labels
+
+
+@pytest.mark.parametrize("B,K,N", [(600, 64, 1000), (300, 160, 16000)])
+@pytest.mark.parametrize("weak", [1e-1, 1e-3, 1e-6])
+def test_vocab_head_rows_in_directions_that_the_weights_hardly_have(gpu, weak, B, K, N):
+    """There the Gram matrix gives sum |z|^2 as a difference of large terms, and the rows are computed again from w."""
+    head_check(B, K, N, argmax=False, data=weak_data(B, K, N, weak))
 
 
 @pytest.mark.parametrize("B,K,N", [(70, 8, 9000), (200, 6, 30000), (5000, 4, 9), (101, 700, 4000)])
