@@ -419,7 +419,7 @@ def test_vocab_head_a_row_of_nan_stays_in_its_row(gpu):
     assert 0 <= am.download()[4] < N
 
 
-@pytest.mark.parametrize("B,K,N", [(20, 48, 300), (300, 40, 260), (100, 300, 1001), (700, 333, 1100)])
+@pytest.mark.parametrize("B,K,N", [(20, 48, 300), (300, 40, 260), (100, 300, 1001), (700, 333, 1100), (60, 7, 5000), (200, 300, 4500), (700, 333, 4001)])
 def test_vocab_head_rows_left_out_may_hold_anything(gpu, B, K, N):
     """NaN and infinities in rows without a label touch neither the other rows nor the gradient of the weights"""
     rng = np.random.default_rng(16)
@@ -440,18 +440,21 @@ def test_vocab_head_rows_left_out_may_hold_anything(gpu, B, K, N):
     assert not loss.download()[labels < 0].any()
 
 
-def test_vocab_head_in_a_graph(gpu):
+@pytest.mark.parametrize("B,K,N,argmax", [(260, 64, 1000, True), (700, 333, 4001, False), (60, 7, 5000, False), (17, 33, 9001, True)])
+def test_vocab_head_in_a_graph(gpu, B, K, N, argmax):
     rng = np.random.default_rng(14)
-    B, K, N = 260, 64, 1000
     x, w, labels = head_data(rng, B, K, N)
     X, W, L = cmat(x, K), cmat(w, K), ops.ints(labels)
     s, loss, am, dX, dW = capi.empty(B), capi.empty(B), capi.empty(B, np.int32), grad(x.shape, K), grad(w.shape, K)
 
+    best = capi.empty(B)
+
     def step():
-        ops.vocab_head_fwd_bwd_sym(X, W, L, s, loss, am, dX, dW)
+        ops.vocab_head_fwd_bwd_sym(X, W, L, s, loss, am if argmax else None, dX, dW)
+        ops.vocab_head_fwd(X, W, None, s, best, am)
 
     def results():
-        return [s.download(), loss.download(), am.download(), dz_of(dX), dz_of(dW)]
+        return [s.download(), loss.download(), best.download(), am.download(), dz_of(dX), dz_of(dW)]
     step()
     want = results()
     exes = []
