@@ -1264,6 +1264,15 @@ __global__ __launch_bounds__(64 * W) void cgemm_skinny_two_kernel(const CgemmArg
 	else skinny_tile<W, A_V4, B_V4>(args1, st1, blockIdx.x - tiles0, red);
 }
 
+// The same for the two backward products of a Linear of any width, dx = g w and dw = g^T x, whose operands are laid out differently.
+template <int W, bool A_V4>
+__global__ __launch_bounds__(64 * W) void cgemm_skinny_bwd_kernel(const CgemmArgs args0, const SkinnyStrides st0, const int tiles0,
+		const CgemmArgs args1, const SkinnyStrides st1) {
+	__shared__ float red[W * 2 * 4 * 64];
+	if ((int) blockIdx.x < tiles0) skinny_tile<W, A_V4, false>(args0, st0, blockIdx.x, red);
+	else skinny_tile<W, false, false>(args1, st1, blockIdx.x - tiles0, red);
+}
+
 // The two backward products of a narrow Linear (args0: dx = g w, all rows of the batch, K <= 16; args1: dw = g^T x) and, behind
 // them, the backward pass of the Hadamard gate with a shared row of weights whose CGelu produced x.  Workgroup n < tiles_n of
 // dx forms columns 16 n .. 16 n + 15 of dx (a row tile per wavefront), keeps them in LDS, takes them through the CGelu and
@@ -1562,6 +1571,24 @@ bool try_skinny_two(bool a_mcontig0, bool b_ncontig0, const CgemmArgs &proto0, b
 	if (!plan_skinny_two(a_mcontig0, b_ncontig0, proto0, a_mcontig1, b_ncontig1, proto1, nprob, args0, args1, v0)) return false;
 	const SkinnyStrides st0 = skinny_strides(args0, a_mcontig0, b_ncontig0), st1 = skinny_strides(args1, a_mcontig1, b_ncontig1);
 	*rc = CNET_SKINNY_PICK(v0, launch_skinny_two, (args0, st0, args1, st1, nprob));
+	return true;
+}
+
+// dx = g w and dw = g^T x as one launch where both are small and whole: true and *rc set.  A product of its own would take 8 or 4
+// wavefronts per tile and 128-bit loads by its own sizes; here the longer one decides for both (96 x 64 x 512: 7.6 us, apart 7.2 + 4.3).
+bool try_skinny_bwd(const CgemmArgs &to_input, const CgemmArgs &to_weight, int *rc) {
+	CgemmArgs args0, args1;
+	if (!plan_skinny(false, true, to_input, 1, 1, args0) || !plan_skinny(true, true, to_weight, 1, 1, args1)) return false;
+	const int tiles0 = args0.tiles_m * args0.tiles_n, tiles = tiles0 + args1.tiles_m * args1.tiles_n;
+	const int cus = cnet::rt().prop.multiProcessorCount;
+	if (args0.splits != 1 || args1.splits != 1 || tiles > 4 * cus) return false;
+	const SkinnyVariant v = skinny_variant(false, true, args0, 1, 1);
+	const SkinnyStrides st0 = skinny_strides(args0, false, true), st1 = skinny_strides(args1, true, true);
+	const bool wide = 2 * tiles <= 3 * cus && std::max(args0.K, args1.K) >= 256;
+	auto kern = wide ? (v.a_v4 ? cgemm_skinny_bwd_kernel<8, true> : cgemm_skinny_bwd_kernel<8, false>)
+			: (v.a_v4 ? cgemm_skinny_bwd_kernel<4, true> : cgemm_skinny_bwd_kernel<4, false>);
+	hipLaunchKernelGGL(kern, dim3((unsigned) tiles), dim3(wide ? 512 : 256), 0, cnet::rt().stream, args0, st0, tiles0, args1, st1);
+	*rc = hipGetLastError() == hipSuccess ? CNET_OK : cnet::fail(CNET_ERR_HIP, "cgemm: launch of the two backward products failed");
 	return true;
 }
 
@@ -2354,6 +2381,32 @@ static CgemmArgs pair_args(int nprob, int M, int N, int K, const float *const a_
 	return a;
 }
 
+// one_launch: small products of different layouts share a launch too, in an order of their sums that may differ from that of
+// a launch each
+int clinear_bwd_sym(bool one_launch, const float *g_dz_re, const float *g_dz_im, int64_t ldg, const float *x_re, const float *x_im, int64_t ldx,
+		const float *w_re, const float *w_im, int64_t ldw, float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx,
+		int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B,
+		int K, int N) {
+	CNET_REQUIRE_INIT();
+	CNET_CHECK_ARG(B > 0 && K > 0 && N > 0);
+	CNET_CHECK_ARG(g_dz_re && g_dz_im && x_re && x_im && w_re && w_im);
+	CNET_CHECK_ARG(dx_dz_re && dx_dz_im && ((dx_dzs_re == nullptr) == (dx_dzs_im == nullptr)));
+	CNET_CHECK_ARG(dw_dz_re && dw_dz_im && ((dw_dzs_re == nullptr) == (dw_dzs_im == nullptr)));
+	CNET_CHECK_ARG(ldg >= N && ldx >= K && ldw >= K && lddx >= K && lddw >= K);
+	// the two products as cnet_clinear_bwd_input_sym and cnet_clinear_bwd_weight_sym set them up
+	const float *gr[2] = {g_dz_re, g_dz_re}, *gi[2] = {g_dz_im, g_dz_im};
+	const float *wr[2] = {w_re, w_re}, *wi[2] = {w_im, w_im}, *xr[2] = {x_re, x_re}, *xi[2] = {x_im, x_im};
+	float *dxr[2] = {dx_dz_re, dx_dzs_re}, *dxi[2] = {dx_dz_im, dx_dzs_im}, *dwr[2] = {dw_dz_re, dw_dzs_re}, *dwi[2] = {dw_dz_im, dw_dzs_im};
+	const bool cj[2] = {false, false};
+	CgemmArgs to_input = pair_args(1, B, K, N, gr, gi, ldg, wr, wi, ldw, cj, dxr, dxi, lddx, accumulate_dx, 0, dx_dzs_re ? MIRROR_CONJ : 0);
+	CgemmArgs to_weight = pair_args(1, N, K, B, gr, gi, ldg, xr, xi, ldx, cj, dwr, dwi, lddw, accumulate_dw, 0, dw_dzs_re ? MIRROR_CONJ : 0);
+	int rc = CNET_OK;
+	if (try_skinny_two(false, true, to_input, true, true, to_weight, 1, &rc)) return rc;
+	if (one_launch && try_skinny_bwd(to_input, to_weight, &rc)) return rc;
+	rc = cgemm_dispatch(false, true, to_input, 1, 1);
+	return rc != CNET_OK ? rc : cgemm_dispatch(true, true, to_weight, 1, 1);
+}
+
 }  // namespace cnet
 
 using namespace cnet;
@@ -2549,23 +2602,8 @@ int cnet_clinear_bwd_sym(const float *g_dz_re, const float *g_dz_im, int64_t ldg
 		const float *w_re, const float *w_im, int64_t ldw, float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx,
 		int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B,
 		int K, int N) {
-	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(B > 0 && K > 0 && N > 0);
-	CNET_CHECK_ARG(g_dz_re && g_dz_im && x_re && x_im && w_re && w_im);
-	CNET_CHECK_ARG(dx_dz_re && dx_dz_im && ((dx_dzs_re == nullptr) == (dx_dzs_im == nullptr)));
-	CNET_CHECK_ARG(dw_dz_re && dw_dz_im && ((dw_dzs_re == nullptr) == (dw_dzs_im == nullptr)));
-	CNET_CHECK_ARG(ldg >= N && ldx >= K && ldw >= K && lddx >= K && lddw >= K);
-	// the two products as cnet_clinear_bwd_input_sym and cnet_clinear_bwd_weight_sym set them up
-	const float *gr[2] = {g_dz_re, g_dz_re}, *gi[2] = {g_dz_im, g_dz_im};
-	const float *wr[2] = {w_re, w_re}, *wi[2] = {w_im, w_im}, *xr[2] = {x_re, x_re}, *xi[2] = {x_im, x_im};
-	float *dxr[2] = {dx_dz_re, dx_dzs_re}, *dxi[2] = {dx_dz_im, dx_dzs_im}, *dwr[2] = {dw_dz_re, dw_dzs_re}, *dwi[2] = {dw_dz_im, dw_dzs_im};
-	const bool cj[2] = {false, false};
-	CgemmArgs to_input = pair_args(1, B, K, N, gr, gi, ldg, wr, wi, ldw, cj, dxr, dxi, lddx, accumulate_dx, 0, dx_dzs_re ? MIRROR_CONJ : 0);
-	CgemmArgs to_weight = pair_args(1, N, K, B, gr, gi, ldg, xr, xi, ldx, cj, dwr, dwi, lddw, accumulate_dw, 0, dw_dzs_re ? MIRROR_CONJ : 0);
-	int rc = CNET_OK;
-	if (try_skinny_two(false, true, to_input, true, true, to_weight, 1, &rc)) return rc;
-	rc = cgemm_dispatch(false, true, to_input, 1, 1);
-	return rc != CNET_OK ? rc : cgemm_dispatch(true, true, to_weight, 1, 1);
+	return clinear_bwd_sym(false, g_dz_re, g_dz_im, ldg, x_re, x_im, ldx, w_re, w_im, ldw, dx_dz_re, dx_dz_im, dx_dzs_re, dx_dzs_im, lddx, accumulate_dx,
+			dw_dz_re, dw_dz_im, dw_dzs_re, dw_dzs_im, lddw, accumulate_dw, B, K, N);
 }
 
 }  // extern "C"

@@ -15,6 +15,9 @@ namespace cnet {
 int cgemm_pair(bool a_mcontig, bool b_ncontig, int nprob, int M, int N, int K, const float *const a_re[2], const float *const a_im[2], long lda,
 		const float *const b_re[2], const float *const b_im[2], long ldb, const bool conj_b[2], float *const c_re[2], float *const c_im[2],
 		long ldc, int accumulate, int tri, int mirror);
+int clinear_bwd_sym(bool one_launch, const float *g_dz_re, const float *g_dz_im, int64_t ldg, const float *x_re, const float *x_im, int64_t ldx,
+		const float *w_re, const float *w_im, int64_t ldw, float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx,
+		int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B, int K, int N);
 int cgemm_gram(int K, int L, const float *a_re, const float *a_im, long lda, float *c_re, float *c_im, long ldc);
 }  // namespace cnet
 
@@ -1505,7 +1508,7 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 		CNET_LAUNCH_CHECK();
 		if (!bwd) return CNET_OK;
 		if (pad.B == B && !plan.label)  // both in one launch where they are small
-			return cnet_clinear_bwd_sym(z_re, z_im, np, a.xs_re, a.xs_im, ldk, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx,
+			return clinear_bwd_sym(true, z_re, z_im, np, a.xs_re, a.xs_im, ldk, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx,
 					a.accumulate_dx, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw, B, K, N);
 		rc = cnet_clinear_bwd_input_sym(z_re, z_im, np, a.w_re, a.w_im, a.ldw, a.dx_re, a.dx_im, a.dxs_re, a.dxs_im, a.lddx, B, K, N,
 				a.accumulate_dx || plan.label);
