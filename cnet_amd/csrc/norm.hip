@@ -199,7 +199,7 @@ struct Sum3Op {
 // SECOND: the next block's norm takes part (the join with a gradient at y).
 // KEEP: the weights stay in registers, and the next row's operands are requested before the exchange of this one.
 // Bound by memory: the join at 8192 x 1024 moves 403 MB in 81 us, 5.0 TB/s, 5 us of it norm_sum_kernel (one exchange after the other,
-// with the rows read twice, took 255 us); 515 x 1001 with a gate per row, 25 MB, 8.4 us.
+// with the rows read twice, took 255 us); 515 x 1001 with a gate per row, 25 MB, 6.5 us.
 template <int T, int NIT, int V, bool SECOND, bool KEEP>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdArgs a, const int policy) {
 	constexpr int G = T / 64, R = T < TPB ? TPB / T : 1, NP = SECOND ? 4 : 2;
@@ -729,7 +729,10 @@ static int norm_bwd(BwdArgs &a, const Out4 &dv, const Out4 &dw) {
 	// Two workgroups to a compute unit, one of the wide ones, all with as many rows: a workgroup's sums are written and read again, which more of them
 	// would do more often (8192 x 1024: 81 us with 512 workgroups, 89 with 768, 93 with 1024; 1024 x 8192: 139 with 256, 154 with 512).
 	const int groups = a.cols <= 256 ? 4 : a.cols <= 512 ? 2 : 1;  // rows that a workgroup works on at a time
-	const int want = std::max(1, std::min((a.rows + groups - 1) / groups, (a.cols > 1024 ? 1 : 2) * rt().prop.multiProcessorCount));
+	// Without such sums (a gate per row) four to a unit: 515 x 1001 6.4 against 8.3 us, 3000 x 130 5.7 against 7.4, 8192 x 1024 the same;
+	// the wide ones stay at one (1000 x 4000: 35 against 37).
+	const int per_unit = a.cols > 1024 ? 1 : a.planes ? 2 : 4;
+	const int want = std::max(1, std::min((a.rows + groups - 1) / groups, per_unit * rt().prop.multiProcessorCount));
 	a.rows_per_slab = (a.rows + want - 1) / want;
 	const int nslabs = (a.rows + a.rows_per_slab - 1) / a.rows_per_slab;
 	if (a.planes) {
