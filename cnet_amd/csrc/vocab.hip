@@ -665,8 +665,9 @@ __global__ __launch_bounds__(T) void head_row_kernel(const HeadArgs a, RowState 
 // that every line of w is fetched whole by one lane quarter after the other, and step j of the chunk multiplies the lanes' j-th
 // values (the four k of a matrix instruction are 16 apart; x is laid out in LDS to match).  The next chunk of w is on its way in
 // registers, and that of x for all four wavefronts, while the present one is multiplied.
-// Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one): 32768 entries of 1024 take 56 us
-// for one row, 4.8 TB/s (a copy of 1 GiB: 5.1), and 120 us for 48, 107 TFLOP/s (the tiles are two wavefronts per SIMD, so waits show).
+// Bound by reading w up to 16 rows, by the matrix pipe beyond (four real products per complex one): 32768 entries of 1024 take 68 us
+// for one row, 3.9 TB/s (a sum over 1 GiB: 3.9; 56 us where calls follow each other closely and find part of w in the memory-side
+// cache), and 120 us for 48, 107 TFLOP/s (the tiles are two wavefronts per SIMD, so waits show).
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 struct ScoreTile {   // what a workgroup leaves for every row
