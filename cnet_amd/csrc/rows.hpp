@@ -42,7 +42,9 @@ __device__ __forceinline__ T exchange(T v) {
 	return b.t;
 }
 
-// After the six steps lane 0 (in fact every lane) holds op over all 64 lanes, combined in a fixed order.
+// After the six steps lane 0 (in fact every lane) holds op over all 64 lanes, combined in a fixed order.  The order is not the same in
+// every lane (the quads of a row of 16 meet in two different pairings): where op rounds, lanes may differ in the last bits, and a branch that
+// the whole row has to take alike goes by lane 0.
 template <class T, class Op>
 __device__ __forceinline__ T wave_reduce(T v, Op op) {
 	v = op(v, exchange<T, 0>(v));

@@ -532,6 +532,10 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 		}
 		sum = group_reduce<double, G>(sum, SumD(), lds_d, slot, wave, lane);
 		diag = group_reduce<float, G>(diag, SumF(), lds_f, slot, wave, lane);
+		if (G == 1) {  // the lanes' totals may differ in their last bits (wave_reduce): lane 0 decides for the row
+			sum = __shfl(sum, 0);
+			diag = __shfl(diag, 0);
+		}
 		const bool good = sum >= (double) (GRAM_LEAST * diag) && diag < 3.0e38f;
 		if (t == 0) st.sum[row] = good ? sum : TO_DO;
 		if (!good) return;
