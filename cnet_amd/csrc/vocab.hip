@@ -788,6 +788,7 @@ __global__ __launch_bounds__(TPB) void head_score_kernel(const HeadArgs a, int B
 			const float z_r = rr[m][i] - ii[m][i], z_i = ri[m][i];
 			double sum = in ? fma((double) z_i, (double) z_i, (double) z_r * z_r) : 0.0;
 			ArgMax best = {in ? fmaf(z_r, z_r, z_i * z_i) : -1.f, n0 + r};
+			if (!(best.v >= 0.f)) best.v = -1.f;  // a NaN is no entry's largest, and would be kept by whoever compares with it
 			sum += exchange<double, 0>(sum);
 			sum += exchange<double, 1>(sum);
 			sum += exchange<double, 2>(sum);
