@@ -205,7 +205,15 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 	}
 	if (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the entries are this wavefront's own
 	else if (!a.loss) __syncthreads();                                   // (the exchange of the sum has had its barriers)
-	const float total = total_weight(e, lane), share = total / S;
+	const float total = total_weight(e, lane);
+	const bool none = total == 0.f;  // nothing to learn from (a row of padding): gradient 0 whatever the row holds, NaN and infinities too
+	const float share = none ? 0.f : total / S;
+	if (none) {
+#pragma unroll
+		for (int k = 0; k < NIT; ++k)
+#pragma unroll
+			for (int q = 0; q < V; ++q) re[k][q] = im[k][q] = 0.f;
+	}
 	// the gradient first, the loss while it is on its way to memory
 	if (live && a.dz_re) {
 #pragma unroll
@@ -236,8 +244,8 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 				load_v<V>(v, zi + c);
 #pragma unroll
 				for (int q = 0; q < V; ++q) {
-					u[q] *= share;
-					v[q] *= share;
+					u[q] = none ? 0.f : u[q] * share;
+					v[q] = none ? 0.f : v[q] * share;
 					n[q] = -v[q];
 				}
 				store_v<V>(a.dz_re + o, u);
@@ -259,7 +267,7 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void distill_kernel(const Distil
 	if (!a.dz_re) return;
 	if (G == 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 	else __syncthreads();
-	if (live) entry_gradients<T>(a, e, row, S, total, t, 0, a.cols);
+	if (live && !none) entry_gradients<T>(a, e, row, S, total, t, 0, a.cols);
 }
 
 // Few long rows: a row is dealt out to workgroups of SLAB columns each, in two launches (its sum, in parts; its gradient).  Bound by
@@ -310,12 +318,13 @@ __global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, 
 	sum = group_reduce<double, WAVES>(sum, SumD(), lds_d, 0, wave, lane);  // (its barriers are the entries' as well)
 	const float S = a.loss ? clamped((float) sum) : a.s[row];
 	const float total = total_weight(e, lane);
+	const bool none = total == 0.f;  // as in distill_kernel
 	if (a.dz_re) {
 		const float share = total / S;
 #pragma unroll
 		for (int k = 0; k < SLAB_COLS; ++k) {
 			const int c = c0 + k * TPB + t;
-			if (c < a.cols) distill_store(a, row, c, re[k] * share, -(im[k] * share));
+			if (c < a.cols) distill_store(a, row, c, none ? 0.f : re[k] * share, none ? 0.f : -(im[k] * share));
 		}
 	}
 	if (a.loss && blockIdx.x == 0) {
@@ -326,6 +335,7 @@ __global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, 
 		}
 	}
 	if (!a.dz_re) return;
+	if (none) return;
 	__syncthreads();
 	entry_gradients<TPB>(a, e, row, S, total, t, c0, c1);
 }

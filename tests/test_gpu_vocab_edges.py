@@ -34,3 +34,35 @@ def test_vocab_head_argmax_beside_a_logit_of_nan(gpu, B, N, at):
     sure = gap[:, -1] > gap[:, -2] * (1 + 1e-4)            # (two logits as large to within their roundings: either)
     assert sure.sum() >= 0.9 * B and np.array_equal(got[sure], want[sure])
     assert np.all(np.isnan(s.download())) and np.all(np.isnan(loss.download()))
+
+
+# every way a row can go: a wavefront's, a workgroup's of each width, longer than its registers, dealt out to several workgroups
+DISTIL_WAYS = [(6, 300, 5), (6, 513, 5), (6, 1200, 70), (6, 4000, 5), (6, 8191, 5), (70, 9001, 5), (70, 20000, 3), (66, 33000, 9), (6, 9001, 5), (3, 100003, 64)]
+
+
+@pytest.mark.parametrize("rows,cols,top", DISTIL_WAYS)
+@pytest.mark.parametrize("pad", [0, 1])
+def test_distill_rows_of_padding_may_hold_anything(gpu, rows, cols, top, pad):
+    """A row without an entry has loss 0 and gradient 0, with NaN and infinities in it as well; the rows beside it are what they were."""
+    rng = np.random.default_rng(cols + top)
+    z = rnd(rng, rows, cols)
+    ids = np.stack([rng.permutation(cols)[:top] for _ in range(rows)]).astype(np.int32)
+    q = rng.random((rows, top)).astype(np.float32) + np.float32(0.1)
+    ids[1:3] = -1
+    q[1] = 0
+    q[2] = np.nan                                          # (the weight of no entry at all)
+    I, Q = ops.ints(ids), capi.to_device(q)
+
+    def run(z):
+        with np.errstate(invalid="ignore"):
+            Z = cmat(z, cols + pad)
+        s, loss, dz, dz2 = capi.empty(rows), capi.empty(rows), grad(z.shape, cols + pad, fill=5.0), grad(z.shape, cols + pad, fill=5.0)
+        ops.distill_fwd_bwd_sym(Z, I, Q, top, s, loss, dz)
+        ops.distill_bwd_sym(Z, s, I, Q, top, dz2)
+        assert np.array_equal(dz_of(dz), dz_of(dz2)) and np.array_equal(dzs_of(dz2), dz_of(dz2).conj())
+        return loss.download(), dz_of(dz)
+    good = run(z)
+    z[1], z[2, ::7], z[2, 1] = np.nan, np.inf, -np.inf
+    loss, dz = run(z)
+    assert np.all(loss[1:3] == 0) and np.all(dz[1:3] == 0)
+    assert np.array_equal(loss, good[0]) and np.array_equal(dz, good[1])
