@@ -35,6 +35,7 @@ struct FwdArgs {
 	long ldy, ldh;
 	float *s, *s2;
 	float scale, eps;
+	double inv_cols;
 	int rows, cols;
 };
 
@@ -48,9 +49,16 @@ struct BwdArgs {
 	int rows, cols, accumulate, accumulate_w;
 };
 
+// |z|^2 added to a sum in double: a square of single precision leaves its range at 1.8e19, and a finite row would come out as zeros
+__device__ __forceinline__ double add_power(double sum, float re, float im) {
+	return fma((double) im, (double) im, fma((double) re, (double) re, sum));
+}
+
 // (the clamp lets a NaN through, which fmaxf would not: the whole row is then NaN)
-__device__ __forceinline__ float inv_rms(float sum, int cols, float eps) {
-	const float rms = sqrtf(sum / (float) cols + eps);
+__device__ __forceinline__ float inv_rms(double sum, double inv_cols, float eps) {
+	const double mean = sum * inv_cols + (double) eps;
+	if (!(mean < 1.0e37)) return (float) (1.0 / sqrt(mean));  // beyond single precision: few rows ever, so the long way
+	const float rms = sqrtf((float) mean);
 	return 1.0f / (rms <= 1.0e-15f ? 1.0e-15f : rms);
 }
 
@@ -106,7 +114,7 @@ __device__ __forceinline__ void store_grad(const Out4 &o, long row, float *re, f
 template <int T, int NIT, int V, bool JOIN>
 __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdArgs a, const int policy) {
 	constexpr int G = T / 64, ROWS = T < TPB ? TPB / T : 1;
-	__shared__ float lds[ROWS * G];
+	__shared__ double lds[ROWS * G];
 	const int slot = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
 	const bool live = (long) blockIdx.x * ROWS + slot < a.rows;
 	const long row = live ? (long) blockIdx.x * ROWS + slot : a.rows - 1;
@@ -125,20 +133,17 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdAr
 			load_cols<V>(u_i[k], a.u.im + row * a.u.ld, c, a.cols, policy);
 		}
 	}
-	float sum = 0.f;
+	double sum = 0.0;
 #pragma unroll
 	for (int k = 0; k < NIT; ++k) {
 		const bool in = (k * T + t) * V < a.cols;
 #pragma unroll
-		for (int q = 0; q < V; ++q) {
-			const float d = x_r[k][q] * x_r[k][q] + x_i[k][q] * x_i[k][q];
-			sum += in ? d : 0.f;
-		}
+		for (int q = 0; q < V; ++q) sum = in ? add_power(sum, x_r[k][q], x_i[k][q]) : sum;
 	}
-	sum = group_reduce<float, G>(sum, SumF(), lds, slot, wave, lane);
-	const float s = inv_rms(sum, a.cols, a.eps);
+	sum = group_reduce<double, G>(sum, SumD(), lds, slot, wave, lane);
+	const float s = inv_rms(sum, a.inv_cols, a.eps);
 	if (t == 0 && live && a.s) a.s[row] = s;
-	float sum2 = 0.f;
+	double sum2 = 0.0;
 #pragma unroll
 	for (int k = 0; k < NIT; ++k) {
 		const int c = (k * T + t) * V;
@@ -152,8 +157,7 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdAr
 			if (JOIN) {
 				y_r = u_r[k][q] + a.scale * y_r;
 				y_i = u_i[k][q] + a.scale * y_i;
-				const float d = y_r * y_r + y_i * y_i;
-				sum2 += c < a.cols ? d : 0.f;
+				sum2 = c < a.cols ? add_power(sum2, y_r, y_i) : sum2;
 			}
 			x_r[k][q] = y_r;
 			x_i[k][q] = y_i;
@@ -164,8 +168,8 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_fwd_kernel(const FwdAr
 		}
 	}
 	if (!JOIN || !a.y_re) return;
-	sum2 = group_reduce<float, G>(sum2, SumF(), lds, slot, wave, lane);
-	const float s2 = inv_rms(sum2, a.cols, a.eps);
+	sum2 = group_reduce<double, G>(sum2, SumD(), lds, slot, wave, lane);
+	const float s2 = inv_rms(sum2, a.inv_cols, a.eps);
 	if (!live) return;
 	if (t == 0 && a.s2) a.s2[row] = s2;
 #pragma unroll
@@ -488,15 +492,15 @@ constexpr int WIDE = 1024;  // threads of the two kernels for wide rows
 // 4.3 TB/s (105 with 256 threads).
 template <bool JOIN>
 __global__ __launch_bounds__(WIDE) void norm_fwd_wide_kernel(const FwdArgs a) {
-	__shared__ float lds[WIDE / 64];
+	__shared__ double lds[WIDE / 64];
 	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
 	const long row = blockIdx.x;
 	const float *xr = a.x.re + row * a.x.ld, *xi = a.x.im + row * a.x.ld;
 	const float *vr = a.v.re + row * a.v.ld, *vi = a.v.im + row * a.v.ld;
-	float sum = 0.f;
-	for (int c = t; c < a.cols; c += WIDE) sum += xr[c] * xr[c] + xi[c] * xi[c];
-	sum = group_reduce<float, WIDE / 64>(sum, SumF(), lds, 0, wave, lane);
-	const float s = inv_rms(sum, a.cols, a.eps);
+	double sum = 0.0;
+	for (int c = t; c < a.cols; c += WIDE) sum = add_power(sum, xr[c], xi[c]);
+	sum = group_reduce<double, WIDE / 64>(sum, SumD(), lds, 0, wave, lane);
+	const float s = inv_rms(sum, a.inv_cols, a.eps);
 	if (t == 0 && a.s) a.s[row] = s;
 	if (!JOIN) {
 		for (int c = t; c < a.cols; c += WIDE) {
@@ -506,18 +510,18 @@ __global__ __launch_bounds__(WIDE) void norm_fwd_wide_kernel(const FwdArgs a) {
 		}
 		return;
 	}
-	float sum2 = 0.f;
+	double sum2 = 0.0;
 	for (int c = t; c < a.cols; c += WIDE) {
 		const float n_r = xr[c] * s, n_i = xi[c] * s;
 		const float h_r = a.u.re[row * a.u.ld + c] + a.scale * (vr[c] * n_r - vi[c] * n_i);
 		const float h_i = a.u.im[row * a.u.ld + c] + a.scale * (vr[c] * n_i + vi[c] * n_r);
 		a.h_re[row * a.ldh + c] = h_r;
 		a.h_im[row * a.ldh + c] = h_i;
-		sum2 += h_r * h_r + h_i * h_i;
+		sum2 = add_power(sum2, h_r, h_i);
 	}
 	if (!a.y_re) return;
-	sum2 = group_reduce<float, WIDE / 64>(sum2, SumF(), lds, 0, wave, lane);
-	const float s2 = inv_rms(sum2, a.cols, a.eps);
+	sum2 = group_reduce<double, WIDE / 64>(sum2, SumD(), lds, 0, wave, lane);
+	const float s2 = inv_rms(sum2, a.inv_cols, a.eps);
 	if (t == 0 && a.s2) a.s2[row] = s2;
 	const float *wr = a.w.re + row * a.w.ld, *wi = a.w.im + row * a.w.ld;
 	for (int c = t; c < a.cols; c += WIDE) {
@@ -684,7 +688,8 @@ static void launch_fwd(const FwdArgs &a, bool join, bool vec, int policy) {
 static bool vec_ok(const Planes &p) { return p.ld % 4 == 0 && aligned16(p.re) && aligned16(p.im); }
 static bool vec_ok(const Out4 &o) { return o.ld % 4 == 0 && aligned16(o.re) && aligned16(o.im) && aligned16(o.sre) && aligned16(o.sim); }
 
-static int norm_fwd(const FwdArgs &a, bool join) {
+static int norm_fwd(FwdArgs &a, bool join) {
+	a.inv_cols = 1.0 / a.cols;
 	const bool vec = a.cols % 4 == 0 && vec_ok(a.x) && vec_ok(a.v) && vec_ok(a.u) && vec_ok(a.w) && vec_ok(Planes{a.y_re, a.y_im, a.ldy}) &&
 			vec_ok(Planes{a.h_re, a.h_im, a.ldh});
 	const int policy = stream_policy(ST_STORES, join ? 8 : 4, (long) a.rows * a.cols);

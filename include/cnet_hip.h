@@ -527,7 +527,8 @@ int cnet_embedding_bwd(const int32_t *tokens, const float *g_dzs_re, const float
  * cnet_norm_join_fwd, behind a block and in front of the next: h = u + scale v .* f s1 (u: the residual path, f: what the block
  *      computed, s1 as above from f) and y = w .* h s2 (s2 from h; w one shared row).  w and y NULL: the last block, h alone.
  *      s, s2: as above.
- * All sums in fp32 over a fixed tree; an infinity or NaN of a row stays in that row (the weights' gradients sum over the rows).
+ * Sums of |x|^2 are formed in double, so that no finite row is beyond them, all others in fp32, each over a fixed tree; an infinity or
+ * NaN of a row stays in that row (the weights' gradients sum over the rows).
  * Fewer than 2^22 rows; results must not overlap operands. */
 int cnet_norm_gate_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *v_re, const float *v_im, int64_t ldv,
                        float *y_re, float *y_im, int64_t ldy, float *s, int rows, int cols, float eps);
