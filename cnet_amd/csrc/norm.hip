@@ -6,6 +6,7 @@
 //
 // Backward, for a conjugate gradient pair, all as dL/dz: with g = dL/dy and p = g v (= dL/dn),
 //   dx = s (p - conj(n) t),  t = mean Re(p n),     dv = g n  (summed over the rows when they share v);
+// where the clamp holds, s does not depend on x, and t is zero.
 // the join adds what the next norm hands back to the gradient of h, dh = gh + back(g), gives it to u as it is, and goes on with
 // f under the gradient scale dh.
 #include "common.hpp"
@@ -54,12 +55,16 @@ __device__ __forceinline__ double add_power(double sum, float re, float im) {
 	return fma((double) im, (double) im, fma((double) re, (double) re, sum));
 }
 
+constexpr float LEAST = 1.0e-15f;  // of a row's rms
+// whether this s is the clamp's, and so the same for every x nearby
+__device__ __forceinline__ bool at_clamp(float s) { return s >= 1.0f / LEAST; }
+
 // (the clamp lets a NaN through, which fmaxf would not: the whole row is then NaN)
 __device__ __forceinline__ float inv_rms(double sum, double inv_cols, float eps) {
 	const double mean = sum * inv_cols + (double) eps;
 	if (!(mean < 1.0e37)) return (float) (1.0 / sqrt(mean));  // beyond single precision: few rows ever, so the long way
 	const float rms = sqrtf((float) mean);
-	return 1.0f / (rms <= 1.0e-15f ? 1.0e-15f : rms);
+	return 1.0f / (rms <= LEAST ? LEAST : rms);
 }
 
 __device__ __forceinline__ void put(float *p, float v, int accumulate) { *p = accumulate ? *p + v : v; }
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(T < TPB ? TPB : T) void norm_bwd_kernel(const BwdAr
 		const float s2_row = s2;
 		if (KEEP && base + R < r1) fetch(min(base + R + group, r1 - 1));
 		m = group_reduce<Sum3, G>(m, Sum3Op(), lds, group, wave, lane);
-		const float t2 = m.b * inv_n * s2_row, t1 = a.scale * (m.a - t2 * m.c) * inv_n;
+		const float t2 = at_clamp(s2_row) ? 0.f : m.b * inv_n * s2_row, t1 = at_clamp(s_row) ? 0.f : a.scale * (m.a - t2 * m.c) * inv_n;
 		if (!live) continue;
 #pragma unroll
 		for (int k = 0; k < NIT; ++k) {
@@ -437,7 +442,8 @@ __global__ __launch_bounds__(T) void norm_bwd_twice_kernel(const BwdArgs a) {
 			}
 		}
 		m = group_reduce<Sum3, G>(m, Sum3Op(), lds, 0, wave, lane);
-		const float inv_n = 1.0f / (float) a.cols, t2 = m.b * inv_n * s2, t1 = a.scale * (m.a - t2 * m.c) * inv_n;
+		const float inv_n = 1.0f / (float) a.cols, t2 = at_clamp(s2) ? 0.f : m.b * inv_n * s2;
+		const float t1 = at_clamp(s) ? 0.f : a.scale * (m.a - t2 * m.c) * inv_n;
 #pragma unroll
 		for (int k = 0; k < NIT; ++k) {
 			if (k * T * V >= a.cols) break;
@@ -561,6 +567,7 @@ __global__ __launch_bounds__(WIDE) void norm_bwd_wide_kernel(const BwdArgs a) {
 				t2 += p_r * n_r - p_i * n_i;
 			}
 			t2 = group_reduce<float, WIDE / 64>(t2, SumF(), lds, 0, wave, lane) * inv_n;
+			if (at_clamp(s2)) t2 = 0.f;
 		}
 		// the gradient at the result of the (first) norm and its weights: scale dh, or g
 		auto at = [&](int c, float &d_r, float &d_i) {
@@ -585,6 +592,7 @@ __global__ __launch_bounds__(WIDE) void norm_bwd_wide_kernel(const BwdArgs a) {
 			t1 += (d_r * v_r - d_i * v_i) * n_r - (d_r * v_i + d_i * v_r) * n_i;
 		}
 		t1 = group_reduce<float, WIDE / 64>(t1, SumF(), lds, 0, wave, lane) * inv_n;
+		if (at_clamp(s)) t1 = 0.f;
 		for (int c = t; c < a.cols; c += WIDE) {
 			float d_r, d_i;
 			at(c, d_r, d_i);

@@ -45,3 +45,45 @@ def test_norm_rows_whose_squares_leave_single_precision(gpu, cols, pad):
     close(s2.download()[:, None], want2, want2, rr, "s2")
     close(cval(Y2), w * h * want2, np.abs(w) * np.abs(h) * want2, rr + 12, "y2")
     assert np.abs(cval(Y2)).max(1).min() > 0.1
+
+
+@pytest.mark.parametrize("cols,pad", WIDTHS)
+def test_norm_gradient_of_rows_at_the_clamp(gpu, cols, pad):
+    """A row whose rms is below 1e-15 (eps = 0) is scaled by 1e15 whatever it is: y is linear in it, and so is what comes back."""
+    rng = np.random.default_rng(cols + 1)
+    rows = 5
+    size = np.array([6e-16, 3e-16, 0.7, 0.0, 2e-15])[:, None]           # clamped, clamped, not, a row of zeros, not
+    x = rounded(rnd(rng, rows, cols, 0.7) * size)
+    s_w = inv_rms(x, 0.0)
+    held = (s_w >= 0.9999e15)[:, 0]
+    assert list(held) == [True, True, False, True, False]
+    v, w, g = rnd(rng, 1, cols, 0.3, 1.0), rnd(rng, 1, cols, 0.2, 1.0), rnd(rng, rows, cols)
+    ld, rr = cols + pad, row_roundings(cols)
+    X, V, Y, s = cmat(x, ld), cmat(v, ld), cmat(0 * x, ld), capi.empty(rows)
+    ops.norm_gate_fwd(X, V, Y, s, 0.0)
+    close(s.download()[:, None], s_w, s_w, rr, "s")
+    dX, dV = grad(x.shape, ld), grad(v.shape, ld)
+    ops.norm_gate_bwd_sym(X, s, V, cmat(g, ld), dX, dV)
+    dx, dv, bound, size_v = back(x, s_w, v, g)
+    dx = np.where(held[:, None], s_w * v * g, dx)                       # dL/dx of y = v x 1e15
+    close(dz_of(dX), dx, bound, 3 * rr + 16, "dx")
+    close(dz_of(dV), dv.sum(0, keepdims=True), size_v.sum(0, keepdims=True), rr + 16 + rows, "dv")
+    # the join's second norm: h = u + scale v f s1 below the clamp in some rows
+    scale = 2.0 ** -52
+    f, u, gh = rnd(rng, rows, cols, 0.7), rounded(rnd(rng, rows, cols) * np.array([1e-16, 0.0, 1.0, 4e-16, 1e-3])[:, None]), rnd(rng, rows, cols)
+    H, Y2, s1, s2 = cmat(0 * u, ld), cmat(0 * u, ld), capi.empty(rows), capi.empty(rows)
+    F, W = cmat(f, ld), cmat(w, ld)
+    ops.norm_join_fwd(cmat(u, ld), F, V, scale, H, s1, W, Y2, s2, 0.0)
+    h = cval(H)
+    s1_w, s2_w = inv_rms(f, 0.0), inv_rms(h, 0.0)
+    held = (s2_w >= 0.9999e15)[:, 0]
+    assert list(held) == [True, True, False, True, False]
+    dU, dF, dV, dW = grad(u.shape, ld), grad(u.shape, ld), grad(v.shape, ld), grad(w.shape, ld)
+    ops.norm_join_bwd_sym(F, s1, V, scale, H, s2, W, cmat(gh, ld), cmat(g, ld), dU, dF, dV, dW)
+    dh, _, bound, _ = back(h, s2_w, w, g)
+    dh = np.where(held[:, None], s2_w * w * g, dh) + gh
+    bound = bound + np.abs(gh)
+    close(dz_of(dU), dh, bound, 3 * rr + 20, "du")
+    df, _, _, _ = back(f, s1_w, scale * v, dh)
+    _, _, bound, _ = back(np.abs(f), s1_w, scale * np.abs(v), bound)
+    close(dz_of(dF), df, bound, 8 * rr + 40, "df")
