@@ -1484,6 +1484,24 @@ double skinny_us(const CgemmArgs &args, int nprob, int batch) {
 	return (3.0 + 0.0075 * k_slice) * std::max(1.0, wgs / (2.0 * cus)) + (args.splits > 1 ? 6.0 : 0.0);
 }
 
+// tuning overrides: 4, 8 or 16 wavefronts per tile of the small-C kernel (0: by its own rule), and 0 for two small products of a call as
+// launches of their own
+int skinny_forced_w() {
+	static const int forced = [] {
+		const char *e = getenv("CNET_CGEMM_SKINNY_W");
+		const int w = e ? atoi(e) : 0;
+		return w == 4 || w == 8 || w == 16 ? w : 0;
+	}();
+	return forced;
+}
+bool skinny_two_enabled() {
+	static const bool enabled = [] {
+		const char *e = getenv("CNET_CGEMM_SKINNY_TWO");
+		return !e || atoi(e) != 0;
+	}();
+	return enabled;
+}
+
 // which instantiation of cgemm_skinny_kernel a planned product takes: float4 loads along K per operand, wavefronts per tile
 struct SkinnyVariant {
 	bool a_v4, b_v4;
@@ -1502,12 +1520,9 @@ SkinnyVariant skinny_variant(bool a_mcontig, bool b_ncontig, const CgemmArgs &ar
 	// Four wavefronts per tile, which leaves room for several tiles on a compute unit; eight (two per SIMD, each other's
 	// latency cover) when there are so few tiles that most units hold one at most (64 x 784 x 784: 9.0 -> 8.5 us; with
 	// three tiles per unit, 256 x 784 x 784: 19.8 -> 21.6 us, so not there).
-	static const int forced_w = [] {
-		const char *e = getenv("CNET_CGEMM_SKINNY_W");  // tuning override: 4, 8 or 16 wavefronts per tile
-		return e ? atoi(e) : 0;
-	}();
+	const int forced_w = skinny_forced_w();
 	const long wgs = (long) args.tiles_m * args.tiles_n * nprob * batch * args.splits;
-	v.w = forced_w == 4 || forced_w == 8 || forced_w == 16 ? forced_w
+	v.w = forced_w ? forced_w
 			: (args.splits == 1 && 2 * wgs <= 3 * cnet::rt().prop.multiProcessorCount && args.K >= 256) ? 8 : 4;
 	return v;
 }
@@ -1548,11 +1563,7 @@ int launch_skinny_two(const CgemmArgs &args0, const SkinnyStrides &st0, const Cg
 // instantiation `v` of it, so that they can go out as one launch.
 bool plan_skinny_two(bool a_mcontig0, bool b_ncontig0, const CgemmArgs &proto0, bool a_mcontig1, bool b_ncontig1, const CgemmArgs &proto1,
 		int nprob, CgemmArgs &args0, CgemmArgs &args1, SkinnyVariant &v) {
-	static const bool enabled = [] {
-		const char *e = getenv("CNET_CGEMM_SKINNY_TWO");  // tuning override: 0 launches the two products one after the other
-		return !e || atoi(e) != 0;
-	}();
-	if (!enabled || proto0.M <= 0 || proto0.N <= 0 || proto0.K <= 0 || proto1.M <= 0 || proto1.N <= 0 || proto1.K <= 0) return false;
+	if (!skinny_two_enabled() || proto0.M <= 0 || proto0.N <= 0 || proto0.K <= 0 || proto1.M <= 0 || proto1.N <= 0 || proto1.K <= 0) return false;
 	if (!plan_skinny(a_mcontig0, b_ncontig0, proto0, nprob, 1, args0) || !plan_skinny(a_mcontig1, b_ncontig1, proto1, nprob, 1, args1))
 		return false;
 	if (args0.splits != 1 || args1.splits != 1) return false;
@@ -1578,16 +1589,18 @@ bool try_skinny_two(bool a_mcontig0, bool b_ncontig0, const CgemmArgs &proto0, b
 // wavefronts per tile and 128-bit loads by its own sizes; here the longer one decides for both (96 x 64 x 512: 7.6 us, apart 7.2 + 4.3).
 bool try_skinny_bwd(const CgemmArgs &to_input, const CgemmArgs &to_weight, int *rc) {
 	CgemmArgs args0, args1;
+	if (!skinny_two_enabled()) return false;
 	if (!plan_skinny(false, true, to_input, 1, 1, args0) || !plan_skinny(true, true, to_weight, 1, 1, args1)) return false;
 	const int tiles0 = args0.tiles_m * args0.tiles_n, tiles = tiles0 + args1.tiles_m * args1.tiles_n;
 	const int cus = cnet::rt().prop.multiProcessorCount;
 	if (args0.splits != 1 || args1.splits != 1 || tiles > 4 * cus) return false;
 	const SkinnyVariant v = skinny_variant(false, true, args0, 1, 1);
 	const SkinnyStrides st0 = skinny_strides(args0, false, true), st1 = skinny_strides(args1, true, true);
-	const bool wide = 2 * tiles <= 3 * cus && std::max(args0.K, args1.K) >= 256;
-	auto kern = wide ? (v.a_v4 ? cgemm_skinny_bwd_kernel<8, true> : cgemm_skinny_bwd_kernel<8, false>)
+	const int w = skinny_forced_w() ? skinny_forced_w() : 2 * tiles <= 3 * cus && std::max(args0.K, args1.K) >= 256 ? 8 : 4;
+	auto kern = w == 16 ? (v.a_v4 ? cgemm_skinny_bwd_kernel<16, true> : cgemm_skinny_bwd_kernel<16, false>)
+			: w == 8 ? (v.a_v4 ? cgemm_skinny_bwd_kernel<8, true> : cgemm_skinny_bwd_kernel<8, false>)
 			: (v.a_v4 ? cgemm_skinny_bwd_kernel<4, true> : cgemm_skinny_bwd_kernel<4, false>);
-	hipLaunchKernelGGL(kern, dim3((unsigned) tiles), dim3(wide ? 512 : 256), 0, cnet::rt().stream, args0, st0, tiles0, args1, st1);
+	hipLaunchKernelGGL(kern, dim3((unsigned) tiles), dim3((unsigned) (64 * w)), 0, cnet::rt().stream, args0, st0, tiles0, args1, st1);
 	*rc = hipGetLastError() == hipSuccess ? CNET_OK : cnet::fail(CNET_ERR_HIP, "cgemm: launch of the two backward products failed");
 	return true;
 }
