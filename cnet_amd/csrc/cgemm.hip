@@ -2394,18 +2394,12 @@ static CgemmArgs pair_args(int nprob, int M, int N, int K, const float *const a_
 	return a;
 }
 
-// one_launch: small products of different layouts share a launch too, in an order of their sums that may differ from that of
-// a launch each
+// What cnet_clinear_bwd_sym does once it has checked its arguments.  one_launch: small products of different layouts share a launch too, in an
+// order of their sums that may differ from that of a launch each
 int clinear_bwd_sym(bool one_launch, const float *g_dz_re, const float *g_dz_im, int64_t ldg, const float *x_re, const float *x_im, int64_t ldx,
 		const float *w_re, const float *w_im, int64_t ldw, float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx,
 		int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B,
 		int K, int N) {
-	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(B > 0 && K > 0 && N > 0);
-	CNET_CHECK_ARG(g_dz_re && g_dz_im && x_re && x_im && w_re && w_im);
-	CNET_CHECK_ARG(dx_dz_re && dx_dz_im && ((dx_dzs_re == nullptr) == (dx_dzs_im == nullptr)));
-	CNET_CHECK_ARG(dw_dz_re && dw_dz_im && ((dw_dzs_re == nullptr) == (dw_dzs_im == nullptr)));
-	CNET_CHECK_ARG(ldg >= N && ldx >= K && ldw >= K && lddx >= K && lddw >= K);
 	// the two products as cnet_clinear_bwd_input_sym and cnet_clinear_bwd_weight_sym set them up
 	const float *gr[2] = {g_dz_re, g_dz_re}, *gi[2] = {g_dz_im, g_dz_im};
 	const float *wr[2] = {w_re, w_re}, *wi[2] = {w_im, w_im}, *xr[2] = {x_re, x_re}, *xi[2] = {x_im, x_im};
@@ -2615,6 +2609,12 @@ int cnet_clinear_bwd_sym(const float *g_dz_re, const float *g_dz_im, int64_t ldg
 		const float *w_re, const float *w_im, int64_t ldw, float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx,
 		int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B,
 		int K, int N) {
+	CNET_REQUIRE_INIT();
+	CNET_CHECK_ARG(B > 0 && K > 0 && N > 0);
+	CNET_CHECK_ARG(g_dz_re && g_dz_im && x_re && x_im && w_re && w_im);
+	CNET_CHECK_ARG(dx_dz_re && dx_dz_im && ((dx_dzs_re == nullptr) == (dx_dzs_im == nullptr)));
+	CNET_CHECK_ARG(dw_dz_re && dw_dz_im && ((dw_dzs_re == nullptr) == (dw_dzs_im == nullptr)));
+	CNET_CHECK_ARG(ldg >= N && ldx >= K && ldw >= K && lddx >= K && lddw >= K);
 	return clinear_bwd_sym(false, g_dz_re, g_dz_im, ldg, x_re, x_im, ldx, w_re, w_im, ldw, dx_dz_re, dx_dz_im, dx_dzs_re, dx_dzs_im, lddx, accumulate_dx,
 			dw_dz_re, dw_dz_im, dw_dzs_re, dw_dzs_im, lddw, accumulate_dw, B, K, N);
 }
