@@ -773,7 +773,7 @@ extern "C" {
 int cnet_norm_gate_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *v_re, const float *v_im, int64_t ldv, float *y_re,
 		float *y_im, int64_t ldy, float *s, int rows, int cols, float eps) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && cols < (1 << 30));
 	CNET_CHECK_ARG(eps >= 0.0f && std::isfinite(eps));
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(x_re && x_im && v_re && v_im && y_re && y_im);
@@ -796,7 +796,7 @@ int cnet_norm_gate_bwd_sym(const float *x_re, const float *x_im, int64_t ldx, co
 		int64_t lddx, float *dv_dz_re, float *dv_dz_im, float *dv_dzs_re, float *dv_dzs_im, int64_t lddv, int rows, int cols, int accumulate,
 		int accumulate_w) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && cols < (1 << 30));
 	if (!rows && (ldv || accumulate_w)) return CNET_OK;
 	CNET_CHECK_ARG(dv_dz_re && dv_dz_im && ((dv_dzs_re == nullptr) == (dv_dzs_im == nullptr)) && lddv >= cols);
 	const Out4 dv = {dv_dz_re, dv_dz_im, dv_dzs_re, dv_dzs_im, (long) lddv};
@@ -823,7 +823,7 @@ int cnet_norm_join_fwd(const float *u_re, const float *u_im, int64_t ldu, const 
 		const float *v_im, int64_t ldv, float scale, float *h_re, float *h_im, int64_t ldh, float *s, const float *w_re, const float *w_im,
 		float *y_re, float *y_im, int64_t ldy, float *s2, int rows, int cols, float eps) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && cols < (1 << 30));
 	CNET_CHECK_ARG(eps >= 0.0f && std::isfinite(eps));
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(u_re && u_im && f_re && f_im && v_re && v_im && h_re && h_im);
@@ -857,7 +857,7 @@ int cnet_norm_join_bwd_sym(const float *f_re, const float *f_im, int64_t ldf, co
 		int64_t lddf, float *dv_dz_re, float *dv_dz_im, float *dv_dzs_re, float *dv_dzs_im, int64_t lddv, float *dw_dz_re, float *dw_dz_im,
 		float *dw_dzs_re, float *dw_dzs_im, int rows, int cols, int accumulate, int accumulate_w) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && cols < (1 << 30));
 	CNET_CHECK_ARG((gh_dz_re == nullptr) == (gh_dz_im == nullptr) && (gy_dz_re == nullptr) == (gy_dz_im == nullptr));
 	const bool second = gy_dz_re != nullptr || (!rows && dw_dz_re != nullptr);
 	if (!rows && accumulate_w) return CNET_OK;

@@ -1576,7 +1576,7 @@ extern "C" {
 int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top, float *s, float *loss,
 		int rows, int cols) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && cols < (1 << 30) && top > 0 && top <= CNET_DISTILL_MAX_TOP);
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && loss && ldz >= cols);
 	return distill(DistillArgs{z_re, z_im, (long) ldz, ids, probs, top, s, loss, nullptr, nullptr, nullptr, nullptr, 0, rows, cols});
@@ -1585,7 +1585,7 @@ int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const in
 int cnet_distill_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, const float *s, const int32_t *ids, const float *probs, int top,
 		float *dz_dz_re, float *dz_dz_im, float *dz_dzs_re, float *dz_dzs_im, int64_t lddz, int rows, int cols) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && cols < (1 << 30) && top > 0 && top <= CNET_DISTILL_MAX_TOP);
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && ldz >= cols);
 	CNET_CHECK_ARG(dz_dz_re && dz_dz_im && ((dz_dzs_re == nullptr) == (dz_dzs_im == nullptr)) && lddz >= cols);
@@ -1596,7 +1596,7 @@ int cnet_distill_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, cons
 int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top, float *s, float *loss,
 		float *dz_dz_re, float *dz_dz_im, float *dz_dzs_re, float *dz_dzs_im, int64_t lddz, int rows, int cols) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && top > 0 && top <= CNET_DISTILL_MAX_TOP);
+	CNET_CHECK_ARG(rows >= 0 && rows < (1 << 22) && cols > 0 && cols < (1 << 30) && top > 0 && top <= CNET_DISTILL_MAX_TOP);
 	if (!rows) return CNET_OK;
 	CNET_CHECK_ARG(z_re && z_im && ids && probs && s && loss && ldz >= cols);
 	CNET_CHECK_ARG(dz_dz_re && dz_dz_im && ((dz_dzs_re == nullptr) == (dz_dzs_im == nullptr)) && lddz >= cols);
@@ -1607,7 +1607,7 @@ int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, 
 int cnet_vocab_head_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw, const int32_t *labels,
 		float *s, float *loss, int32_t *argmax, int B, int K, int N) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && N > 0 && N < (1 << 28));
+	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && K < (1 << 30) && N > 0 && N < (1 << 28));
 	if (!B) return CNET_OK;
 	CNET_CHECK_ARG(x_re && x_im && w_re && w_im && s && (loss || argmax));
 	CNET_CHECK_ARG(ldx >= K && ldw >= K);
@@ -1632,7 +1632,7 @@ int cnet_vocab_head_fwd_bwd_sym(const float *x_re, const float *x_im, int64_t ld
 		int64_t lddx, int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B,
 		int K, int N) {
 	CNET_REQUIRE_INIT();
-	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && N > 0 && N < (1 << 28));
+	CNET_CHECK_ARG(B >= 0 && B < (1 << 24) && K > 0 && K < (1 << 30) && N > 0 && N < (1 << 28));
 	CNET_CHECK_ARG(dw_dz_re && dw_dz_im && ((dw_dzs_re == nullptr) == (dw_dzs_im == nullptr)) && lddw >= K);
 	if (!B) {
 		if (accumulate_dw) return CNET_OK;

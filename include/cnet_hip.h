@@ -529,7 +529,7 @@ int cnet_embedding_bwd(const int32_t *tokens, const float *g_dzs_re, const float
  *      s, s2: as above.
  * Sums of |x|^2 are formed in double, so that no finite row is beyond them, all others in fp32, each over a fixed tree; an infinity or
  * NaN of a row stays in that row (the weights' gradients sum over the rows).
- * Fewer than 2^22 rows; results must not overlap operands. */
+ * Fewer than 2^22 rows and 2^30 columns; results must not overlap operands. */
 int cnet_norm_gate_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *v_re, const float *v_im, int64_t ldv,
                        float *y_re, float *y_im, int64_t ldy, float *s, int rows, int cols, float eps);
 int cnet_norm_join_fwd(const float *u_re, const float *u_im, int64_t ldu, const float *f_re, const float *f_im, int64_t ldf,
@@ -565,7 +565,7 @@ int cnet_norm_join_bwd_sym(const float *f_re, const float *f_im, int64_t ldf, co
  * a NaN loss and counts in Q alone, as a label outside the row does in CrossEntropy.  One entry of weight 1 is CrossEntropy.
  * The gradient is assigned; its dz* half may be NULL.  cnet_distill_fwd_bwd_sym gives the results of the other two in one
  * call, with z read once where a row fits a workgroup's registers (32768 columns).  `loss` may point into memory from
- * cnet_host_alloc.  Fewer than 2^22 rows; results must not overlap operands. */
+ * cnet_host_alloc.  Fewer than 2^22 rows and 2^30 columns; results must not overlap operands. */
 #define CNET_DISTILL_MAX_TOP 1024
 int cnet_distill_fwd(const float *z_re, const float *z_im, int64_t ldz, const int32_t *ids, const float *probs, int top,
                      float *s, float *loss, int rows, int cols);
@@ -593,7 +593,7 @@ int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, 
  * x / sqrt(s), are formed in single precision and have to stay within its range.
  * The buffer holds a few planes of [B x K] and [K x K] or at most about 192 MiB of logits (more only where 64 columns of B rows
  * are), with one aligned copy of w (up to 2 GiB) where K is not a multiple of 16 or a plane not aligned to 16 bytes.
- * B < 2^24, N < 2^28; results must not overlap operands. */
+ * B < 2^24, K < 2^30, N < 2^28; results must not overlap operands. */
 int cnet_vocab_head_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw,
                         const int32_t *labels, float *s, float *loss, int32_t *argmax, int B, int K, int N);
 int cnet_vocab_head_fwd_bwd_sym(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw,

@@ -87,3 +87,21 @@ def test_norm_gradient_of_rows_at_the_clamp(gpu, cols, pad):
     df, _, _, _ = back(f, s1_w, scale * v, dh)
     _, _, bound, _ = back(np.abs(f), s1_w, scale * np.abs(v), bound)
     close(dz_of(dF), df, bound, 8 * rr + 40, "df")
+
+
+def test_norm_and_vocabulary_refuse_rows_that_32_bit_columns_cannot_walk(gpu):
+    """A thread's next column has to stay within 32 bits behind the row's end: 2^30 columns and more are refused before anything is read."""
+    lib, wide, p, invalid = capi.load(), 1 << 30, capi.zeros(4).ptr, -2
+    for cols in (wide, (1 << 31) - 1):
+        ld = 1 << 31
+        assert lib.cnet_norm_gate_fwd(p, p, ld, p, p, 0, p, p, ld, None, 1, cols, EPS) == invalid
+        assert lib.cnet_norm_gate_bwd_sym(p, p, ld, p, p, p, 0, p, p, ld, p, p, None, None, ld, p, p, None, None, ld, 1, cols, 0, 0) == invalid
+        assert lib.cnet_norm_join_fwd(p, p, ld, p, p, ld, p, p, 0, 1.0, p, p, ld, None, None, None, None, None, 0, None, 1, cols, EPS) == invalid
+        assert lib.cnet_norm_join_bwd_sym(p, p, ld, p, p, p, 0, 1.0, None, None, 0, None, None, None, p, p, ld, None, None, 0, p, p, None, None, ld,
+                                          p, p, None, None, ld, p, p, None, None, ld, None, None, None, None, 1, cols, 0, 0) == invalid
+        assert lib.cnet_distill_fwd(p, p, ld, p, p, 1, p, p, 1, cols) == invalid
+        assert lib.cnet_distill_bwd_sym(p, p, ld, p, p, p, 1, p, p, None, None, ld, 1, cols) == invalid
+        assert lib.cnet_distill_fwd_bwd_sym(p, p, ld, p, p, 1, p, p, p, p, None, None, ld, 1, cols) == invalid
+        assert lib.cnet_vocab_head_fwd(p, p, ld, p, p, ld, p, p, p, p, 1, cols, 1) == invalid
+        assert lib.cnet_vocab_head_fwd_bwd_sym(p, p, ld, p, p, ld, p, p, p, None, p, p, None, None, ld, 0, p, p, None, None, ld, 0, 1, cols, 1) == invalid
+        assert b"cols < (1 << 30)" in lib.cnet_last_error() or b"K < (1 << 30)" in lib.cnet_last_error()
