@@ -16,7 +16,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "lib", "libcnet_hip.so")
-SOURCES = ["runtime.hip", "cgemm.hip", "cdft.hip", "elementwise.hip", "reduce.hip", "embedding.hip", "norm.hip", "vocab.hip"]
+SOURCES = ["runtime.hip", "cgemm.hip", "cdft.hip", "elementwise.hip", "reduce.hip", "embedding.hip", "norm.hip", "gram.hip", "vocab.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
          # no fused multiply-add contraction: the elementwise kernels then round like the CPU path

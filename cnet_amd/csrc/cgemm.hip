@@ -104,10 +104,6 @@ struct CgemmArgs {
 	float *ce_dz_re = nullptr, *ce_dz_im = nullptr, *ce_dzs_re = nullptr, *ce_dzs_im = nullptr;
 	long ce_ldo = 0, ce_lddz = 0;
 	int ce_vec = 0;  // the 128-bit instantiation of the row routine (what the separate launch would pick for these operands)
-	// C = A^H A is Hermitian and the caller fills what lies below the diagonal from what lies above: only the blocks that reach the
-	// diagonal or lie above it are computed, (t + 1) / 2t of the work for t blocks a side.  Square blocks, one problem.  C below the
-	// diagonal is left undefined.
-	int upper = 0;
 };
 constexpr int MIRROR_CONJ = 1, MIRROR_GELU = 2, MIRROR_HERM = 3, MIRROR_HGELU = 4, MIRROR_CE = 5;
 
@@ -145,16 +141,8 @@ __device__ __forceinline__ void gelu_store(const CgemmArgs &args, long off, floa
 // Which block of C (per problem) a linear block number stands for: walks groups of 8 block rows column by column, after
 // spreading consecutive workgroup numbers (which the hardware deals round-robin to the XCDs) over contiguous strips.
 __device__ __forceinline__ void map_block(const CgemmArgs &args, int pid, int grid_n, int &tile_m, int &tile_n) {
-	const int total = args.upper ? args.tiles_m * (args.tiles_m + 1) / 2 : args.tiles_m * grid_n;
+	const int total = args.tiles_m * grid_n;
 	if (total % NUM_XCD == 0) pid = (pid % NUM_XCD) * (total / NUM_XCD) + pid / NUM_XCD;
-	if (args.upper) {  // column by column: block column j starts at number j (j + 1) / 2
-		int j = (int) ((sqrtf(8.0f * (float) pid + 1.0f) - 1.0f) * 0.5f);
-		while (j * (j + 1) / 2 > pid) --j;
-		while ((j + 1) * (j + 2) / 2 <= pid) ++j;
-		tile_n = j;
-		tile_m = pid - j * (j + 1) / 2;
-		return;
-	}
 	constexpr int GROUP = 8;
 	const int width = GROUP * grid_n;
 	const int first_m = (pid / width) * GROUP;
@@ -958,7 +946,6 @@ __global__ __launch_bounds__(256) void splitk_reduce_kernel(CgemmArgs args, int 
 	const int part = idx >= plane;  // 0: re, 1: im
 	const long e = idx - part * plane;
 	const long row = e / args.N, col = e - row * args.N;
-	if (args.upper && col < row) return;  // (not wanted, and not computed below the diagonal blocks)
 	const float *first = args.partial + (((long) prob * nbatch + b) * 2 + part) * plane + e;
 	float v = cnet::ordered_sum(first, (long) nprob * nbatch * 2 * plane, args.splits);
 	float *c = (part ? args.p[prob].c_im : args.p[prob].c_re) + (long) b * args.stride_c + row * args.ldc + col;
@@ -1694,7 +1681,7 @@ int launch(const CgemmArgs &proto, int nprob, int batch, int tail_splits = 0, in
 	args.chunks_per_split = 0;
 	args.partial = nullptr;
 	{
-		const long blocks = args.upper ? (long) args.tiles_m * (args.tiles_m + 1) / 2 : (long) args.tiles_m * args.tiles_n * nprob * batch;
+		const long blocks = (long) args.tiles_m * args.tiles_n * nprob * batch;
 		const long cus = cnet::rt().prop.multiProcessorCount;
 		const int nchunks = (args.K + KC - 1) / KC;
 		int splits = k_cuts;  // from the cost model; -1: the rule for the kernels it does not cover
@@ -1711,7 +1698,7 @@ int launch(const CgemmArgs &proto, int nprob, int batch, int tail_splits = 0, in
 			if (!args.partial) return CNET_ERR_OUT_OF_MEMORY;
 		}
 	}
-	dim3 grid(args.upper ? args.tiles_m * (args.tiles_m + 1) / 2 : args.tiles_m * grid_tiles_n(args), nprob, batch * args.splits);
+	dim3 grid(args.tiles_m * grid_tiles_n(args), nprob, batch * args.splits);
 	// The fast kernel addresses a lane's 16 bytes inside the operand tile of a chunk with an unsigned 32-bit byte offset:
 	// (row * ld + k) * 4 for rows < min(block edge, rows of the operand), or (k * ld + row) * 4 for k < KC.  A leading
 	// dimension beyond that (8.4 M floats for a K-contiguous operand under a 128-row block) goes to cgemm_kernel, whose
@@ -1722,7 +1709,7 @@ int launch(const CgemmArgs &proto, int nprob, int batch, int tail_splits = 0, in
 	};
 	const bool fast_ok = VEC == 4 && args.K % KC == 0 && offsets_fit(args.lda, A_MCONTIG, BM, args.M) &&
 			offsets_fit(args.ldb, B_NCONTIG, BN, args.N);
-	if (tail_splits >= 2 && fast_ok && !args.tri && !args.upper && batch == 1 && args.splits == 1) {
+	if (tail_splits >= 2 && fast_ok && !args.tri && batch == 1 && args.splits == 1) {
 		const long cus = cnet::rt().prop.multiProcessorCount;
 		const long all = (long) args.tiles_m * args.tiles_n * nprob;
 		const int nchunks = args.K / KC;
@@ -1830,7 +1817,6 @@ double plan_blocks(const CgemmArgs &a, int nprob, int batch, int layout, int *sh
 	const long cus = cnet::rt().prop.multiProcessorCount;
 	auto blocks = [&](int bm, int bn) {
 		long tn = (a.N + bn - 1) / bn;
-		if (a.upper) return tn * (tn + 1) / 2;
 		if (a.tri) tn = (tn + 1) / 2;  // one workgroup per mirrored pair of column blocks
 		return (long) ((a.M + bm - 1) / bm) * tn * nprob * batch;
 	};
@@ -1945,11 +1931,11 @@ double plan_blocks(const CgemmArgs &a, int nprob, int batch, int layout, int *sh
 	const int khz = cnet::rt().prop.clockRate;
 	const double flop_per_us_per_unit = 256.0 * (khz > 0 ? khz * 1e-3 : 2.4e3);
 	const int nchunks = (a.K + KC - 1) / KC;
-	const bool tail_possible = forced_tail != 0 && a.K % KC == 0 && !a.tri && !a.upper && batch == 1;
+	const bool tail_possible = forced_tail != 0 && a.K % KC == 0 && !a.tri && batch == 1;
 	int best = 3, best_tail = 0, best_cuts = 1;
 	double best_us = 1e30;
 	for (int k = 0; k < 5; ++k) {
-		if (a.upper ? k == 1 || k == 2 : forced >= 0 && forced != k) continue;  // (square blocks)
+		if (forced >= 0 && forced != k) continue;
 		if (k == 4 && (forced != 4 && a.K % KC != 0)) continue;  // only the fast kernel has the two-stage form: shape 3 there
 		// beyond seven blocks per unit the two-stage form is erratic on a long K (8192 x 1024 of C: .95 at K = 2048, .83 - .97
 		// from 4096 on, layout by layout)
@@ -1987,7 +1973,7 @@ double plan_blocks(const CgemmArgs &a, int nprob, int batch, int layout, int *sh
 		}();
 		if (!a.tri && nb < 2 * cus && nchunks >= 8 && (plan_cuts || nb * 2 <= cus)) {
 			const long few = nb * 2 <= cus ? std::min<long>(cus / nb, nchunks / 4) : 0;  // one slice-workgroup per unit
-			for (long s : {2L, 3L, 4L, 6L, 8L, few, a.upper ? 2 * few : 0L}) {
+			for (long s : {2L, 3L, 4L, 6L, 8L, few}) {
 				if (s < 2 || nchunks / s < 4 || (long) batch * s > 65535) continue;
 				const int k_slice = (int) ((nchunks + s - 1) / s) * KC;
 				const long p = (nb * s + cus - 1) / cus;
@@ -2336,27 +2322,6 @@ int cgemm_real_a(int M, int N, int K, const float *a_re, const float *a_im, long
 		a.herm_hi = herm_n - N;
 	}
 	return cgemm_dispatch(false, true, a, 1, 1);
-}
-
-// Used by vocab.hip.  C [K][K] = A^H A for an A of L rows, its part on and above the diagonal; what lies below is undefined.  Planes of
-// A on 16 bytes with a leading dimension that is a multiple of four, or CNET_ERR_UNSUPPORTED.
-int cgemm_gram(int K, int L, const float *a_re, const float *a_im, long lda, float *c_re, float *c_im, long ldc) {
-	if (!aligned16(a_re) || !aligned16(a_im) || lda % 4 != 0 || lda >= (1L << 22))
-		return fail(CNET_ERR_UNSUPPORTED, "cgemm: a Gram matrix takes aligned planes with a leading dimension below 2^22");
-	const float *ar[2] = {a_re, a_re}, *ai[2] = {a_im, a_im};
-	float *cr[2] = {c_re, c_re}, *ci[2] = {c_im, c_im};
-	const bool cj[2] = {false, false};
-	const int whole = L - L % KC;  // (the rest of the rows as a short product of its own)
-	CgemmArgs a = pair_args(1, K, K, whole, ar, ai, lda, ar, ai, lda, cj, cr, ci, ldc, 0, 0, 0);
-	a.p[0].a_im_sign = -1.0f;
-	a.upper = 1;
-	int rc = whole > 0 ? pick_tile<true, true, 4>(a, 1, 1) : CNET_OK;
-	if (rc != CNET_OK || whole == L) return rc;
-	a.upper = 0;
-	a.K = L - whole;
-	a.accumulate = whole > 0;
-	for (const float **q : {&a.p[0].a_re, &a.p[0].a_im, &a.p[0].b_re, &a.p[0].b_im}) *q += (long) whole * lda;
-	return cgemm_dispatch(true, true, a, 1, 1);
 }
 
 static CgemmArgs pair_args(int nprob, int M, int N, int K, const float *const a_re[2], const float *const a_im[2], long lda,

@@ -5,6 +5,7 @@
 //   dL/dz_k = conj(z_k) Q / S - q_k conj(z_k) / max(|z_k|^2, 1e-15)
 // for targets q_k with the sum Q: one label (q = Q = 1), or the teacher's entries.
 #include "common.hpp"
+#include "gram.hpp"
 #include "rows.hpp"
 
 #include <algorithm>
@@ -18,7 +19,6 @@ int cgemm_pair(bool a_mcontig, bool b_ncontig, int nprob, int M, int N, int K, c
 int clinear_bwd_sym(bool one_launch, const float *g_dz_re, const float *g_dz_im, int64_t ldg, const float *x_re, const float *x_im, int64_t ldx,
 		const float *w_re, const float *w_im, int64_t ldw, float *dx_dz_re, float *dx_dz_im, float *dx_dzs_re, float *dx_dzs_im, int64_t lddx,
 		int accumulate_dx, float *dw_dz_re, float *dw_dz_im, float *dw_dzs_re, float *dw_dzs_im, int64_t lddw, int accumulate_dw, int B, int K, int N);
-int cgemm_gram(int K, int L, const float *a_re, const float *a_im, long lda, float *c_re, float *c_im, long ldc);
 }  // namespace cnet
 
 namespace {
@@ -342,9 +342,10 @@ __global__ __launch_bounds__(TPB) void distill_slab_kernel(const DistillArgs a, 
 
 // ------------------------------------------------------------------------------------------------ vocabulary head
 struct RowState {   // one entry per row of x, carried from launch to launch
-	double *sum;    // sum |z|^2 so far; below zero: still to be added up from `part`
-	double *part;   // [row][slabs]
+	double *sum;    // sum |z|^2 so far
+	double *part;   // [row][slabs]: what it is added up from, through a Gram matrix
 	int slabs;
+	double *weight; // 1 / S, or 0 where the row is left out: what x^H x is weighted with
 	float *best;    // largest |z|^2 so far, and its first index
 	int *index;
 	float *c_re, *c_im;  // conj(z_label) / m, the label's share of the gradient
@@ -387,14 +388,12 @@ __global__ __launch_bounds__(TPB) void head_piece_kernel(const float *__restrict
 
 // ---- The loss through the Gram matrix of w.  The loss knows the logits z = x w^T through sum |z|^2 alone, a quadratic form of x:
 // with T = w^H w (K x K), y = conj(x) T is what the logits' gradient hands back to x (before its division by S and without the
-// label's term) and S = sum_j y_j x_j.  So neither S nor either gradient needs the logits: N K^2 + B K^2 products stand for
-// B N K.  What it costs is accuracy where x lies in directions that w hardly has: the terms of S cancel.  With D = sum |x_i|^2 T_ii
-// (the sum's size if the columns of w were orthogonal), a row with S < D / 64 is computed again from w itself, so that at most
-// six of the 24 bits are lost to the cancellation.
-constexpr float GRAM_LEAST = 1.0f / 64;
-constexpr int HEAD_ROWS = 64;       // rows whose marks one workgroup of head_finish_marked_kernel looks at
-constexpr double TO_DO = -1.0;
-
+// label's term) and S = sum_j y_j x_j; and dw is conj(w) P with P = x^H diag(1 / S) x (again without the label's term).  So neither S
+// nor either gradient needs the logits: N K^2 + B K^2 products stand for B N K.
+// Where x lies in directions that w hardly has (or a row of w in directions that the batch hardly has) these sums are small and
+// their terms are not.  With D = sum |x_i|^2 T_ii, what their terms amount to, a sum of rounded terms is off by D / S roundings, where the sum
+// over the logits is off by about sqrt(D / S).  T, y, S and P are therefore formed and kept in double (gram.hip), which is
+// closer than logits in single precision down to D / S = 1e17, where these have no digit left.
 struct HeadArgs {
 	const float *x_re, *x_im, *w_re, *w_im;
 	long ldx, ldw;
@@ -402,7 +401,7 @@ struct HeadArgs {
 	float *s, *loss;
 	int *argmax;
 	const float *y_re, *y_im;  // conj(z) w, not yet divided by S
-	float *xs_re, *xs_im;      // the rows that are trained on, as the weights' gradient reads them; zeros elsewhere
+	float *xs_re, *xs_im;      // without a Gram matrix: the rows that are trained on, as the weights' gradient reads them; zeros elsewhere
 	long ldy;                  // leading dimension of y and xs
 	float *dx_re, *dx_im, *dxs_re, *dxs_im;
 	long lddx;
@@ -445,9 +444,9 @@ __device__ __forceinline__ LabelTerm label_term(const HeadArgs &a, long row, int
 }
 
 // What is left to do for a row once its sum |z|^2 is known, by G wavefronts: S, the label's logit, loss, and the gradient at x: y / S
-// minus the label's row of w times conj(z_label) / m.  xs = x / sqrt(S), so that both operands of the weights' gradient come
-// from it: a row that is left out is zero in either, whatever it holds (padding may hold anything).
-template <int G, int V, bool BWD>
+// minus the label's row of w times conj(z_label) / m.  For the weights' gradient, GRAM: the row's weight; otherwise xs = x / sqrt(S), so
+// that both of its operands come from it: a row that is left out is zero in either, whatever it holds (padding may hold anything).
+template <int G, int V, bool BWD, bool GRAM>
 __device__ __forceinline__ void finish_row(const HeadArgs &a, const RowState &st, long row, double sum, double *lds, int t, int lane, int wave) {
 	const float S = clamped((float) sum);
 	int best = a.labels && !a.argmax ? 0 : st.index[row];
@@ -462,6 +461,7 @@ __device__ __forceinline__ void finish_row(const HeadArgs &a, const RowState &st
 	if (t == 0) {
 		st.c_re[row] = l.c_re;
 		st.c_im[row] = l.c_im;
+		if (GRAM) st.weight[row] = l.live ? 1.0 / (double) S : 0.0;
 	}
 	const float *xr = a.x_re + row * a.ldx, *xi = a.x_im + row * a.ldx;
 	const long label_row = (l.label < 0 ? 0 : l.label) * a.ldw;
@@ -477,8 +477,10 @@ __device__ __forceinline__ void finish_row(const HeadArgs &a, const RowState &st
 				load_v<V>(g_i, a.y_im + o);
 				load_v<V>(w_r, a.w_re + label_row + c);
 				load_v<V>(w_i, a.w_im + label_row + c);
-				load_v<V>(s_r, xr + c);
-				load_v<V>(s_i, xi + c);
+				if (!GRAM) {
+					load_v<V>(s_r, xr + c);
+					load_v<V>(s_i, xi + c);
+				}
 #pragma unroll
 				for (int k = 0; k < V; ++k) {
 					g_r[k] = g_r[k] * inv - (l.c_re * w_r[k] - l.c_im * w_i[k]);
@@ -503,20 +505,20 @@ __device__ __forceinline__ void finish_row(const HeadArgs &a, const RowState &st
 				give(a.dxs_im, g_i, -1.f);
 			}
 		}
-		store_v<V>(a.xs_re + o, s_r);
-		store_v<V>(a.xs_im + o, s_i);
+		if (!GRAM) {
+			store_v<V>(a.xs_re + o, s_r);
+			store_v<V>(a.xs_im + o, s_i);
+		}
 	}
 }
 
-// T threads per row (64: four rows to a workgroup).  GRAM: the sum is formed here, from x and y; a row whose terms cancel (or that
-// holds a NaN or an overflow) is marked and left to the two kernels behind this one.  Rows beyond B, which fill up the last
-// chunk of the weights' product, become zero.
-// Bound by memory: x, y and the labels' rows of w are read, dx and xs written; 8192 x 1024, 335 MB, takes 74 us, 4.5 TB/s.
+// T threads per row (64: four rows to a workgroup).  GRAM: the sum is added up from its parts.  Rows beyond B, which fill up the last
+// chunk of the weights' product, become zero in xs.
+// Bound by memory: y and the labels' rows of w are read, dx written; 8192 x 1024, 201 MB, takes @@ us.
 template <int T, int V, bool BWD, bool GRAM>
-__global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st, const float *__restrict__ diag_at, long diag_step, int rows) {
+__global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st, int rows) {
 	constexpr int G = T / 64, ROWS = TPB / T;
 	__shared__ double lds_d[WAVES];
-	__shared__ float lds_f[WAVES];
 	const int slot = threadIdx.x / T, t = threadIdx.x % T, lane = threadIdx.x & 63, wave = t >> 6;
 	const long row = (long) blockIdx.x * ROWS + slot;
 	if (row >= rows) return;
@@ -525,51 +527,14 @@ __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowS
 		return;
 	}
 	double sum;
-	if (GRAM) {
+	if (GRAM) {  // (every wavefront for itself, and lane 0's for all of them)
 		sum = 0.0;
-		float diag = 0.f;
-		for (int c = t * V; c < a.K; c += T * V) {
-			float x_r[V], x_i[V], y_r[V], y_i[V];
-			load_v<V>(x_r, a.x_re + row * a.ldx + c);
-			load_v<V>(x_i, a.x_im + row * a.ldx + c);
-			load_v<V>(y_r, a.y_re + row * a.ldy + c);
-			load_v<V>(y_i, a.y_im + row * a.ldy + c);
-#pragma unroll
-			for (int k = 0; k < V; ++k) {
-				sum += (double) x_r[k] * y_r[k] - (double) x_i[k] * y_i[k];
-				diag += (x_r[k] * x_r[k] + x_i[k] * x_i[k]) * diag_at[(c + k) * diag_step];
-			}
-		}
-		sum = group_reduce<double, G>(sum, SumD(), lds_d, slot, wave, lane);
-		diag = group_reduce<float, G>(diag, SumF(), lds_f, slot, wave, lane);
-		if (G == 1) {  // the lanes' totals may differ in their last bits (wave_reduce): lane 0 decides for the row
-			sum = __shfl(sum, 0);
-			diag = __shfl(diag, 0);
-		}
-		const bool good = sum >= (double) (GRAM_LEAST * diag) && diag < 3.0e38f;
-		if (t == 0) st.sum[row] = good ? sum : TO_DO;
-		if (!good) return;
+		for (int k = lane; k < st.slabs; k += 64) sum += st.part[row * st.slabs + k];
+		sum = __shfl(wave_reduce(sum, SumD()), 0);
 	} else {
 		sum = st.sum[row];
 	}
-	finish_row<G, V, BWD>(a, st, row, sum, lds_d + slot * G, t, lane, wave);
-}
-
-// the marked rows among HEAD_ROWS, once their sums are in st.part (a launch, 5 us, where there are none)
-template <int V, bool BWD>
-__global__ __launch_bounds__(TPB) void head_finish_marked_kernel(const HeadArgs a, RowState st) {
-	__shared__ double lds_d[WAVES];
-	const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-	const int first = blockIdx.x * HEAD_ROWS;
-	unsigned long long set = __ballot(first + lane < a.B && st.sum[min(first + lane, a.B - 1)] < 0.0);
-	while (set) {
-		const long row = first + __ffsll((long long) set) - 1;
-		set &= set - 1;
-		double sum = 0.0;
-		for (int k = lane; k < st.slabs; k += 64) sum += st.part[row * st.slabs + k];
-		sum = wave_reduce(sum, SumD());
-		finish_row<WAVES, V, BWD>(a, st, row, sum, lds_d, t, lane, wave);
-	}
+	finish_row<G, V, BWD, GRAM>(a, st, row, sum, lds_d + slot * G, t, lane, wave);
 }
 
 // The logits of one row as a whole (two planes of leading dimension ldz, a multiple of four): S, the largest, the label's logit,
@@ -861,92 +826,6 @@ struct ScatterArgs {
 	int B, K, N;
 };
 
-// ---- The rows that head_finish_kernel has marked, from w: part[row][slab] = sum |z|^2 over the slab blockIdx.x of the vocabulary, `per`
-// tiles of 64 entries.  A workgroup lists the marked ones of the DIRECT_BLOCK rows blockIdx.z (usually there are none: 5 us for the
-// launch) and takes them 32 at a time, every gridDim.y-th such group, in the way of the kernel above; what it finds for a row does
-// not depend on the rows beside it.  Of 8192 rows of 1024 -> 32768 entries, with none, a hundredth, a tenth and all of them marked, a
-// training step takes 4.4, 5.1, 6.9 and 22.8 ms (with four rows at a time on the vector unit 7.1, 23, 26 and 56).
-constexpr int DIRECT_BLOCK = 4096, DIRECT_MT = 2;
-template <bool V4>
-__global__ __launch_bounds__(TPB) void head_direct_kernel(const HeadArgs a, RowState st, int per) {
-	constexpr int MT = DIRECT_MT, ROWS = 16 * MT, EACH = DIRECT_BLOCK / TPB;
-	__shared__ ScoreRows<MT> xs;
-	__shared__ double met[WAVES][ROWS];
-	__shared__ unsigned short list[DIRECT_BLOCK];
-	__shared__ int found[WAVES];
-	const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r = lane & 15, q = lane >> 4;
-	const long base = (long) blockIdx.z * DIRECT_BLOCK;
-	unsigned marks = 0;
-#pragma unroll
-	for (int i = 0; i < EACH; ++i) {
-		const long row = base + i * TPB + t;
-		marks |= (row < a.B && st.sum[min(row, (long) a.B - 1)] < 0.0 ? 1u : 0u) << i;
-	}
-	int mine = 0;
-#pragma unroll
-	for (int i = 0; i < EACH; ++i) mine += __popcll(__ballot(marks >> i & 1));
-	if (lane == 0) found[wave] = mine;
-	__syncthreads();
-	int at = 0, count = 0;
-#pragma unroll
-	for (int w = 0; w < WAVES; ++w) {
-		if (w < wave) at += found[w];
-		count += found[w];
-	}
-	if (!count) return;
-	for (int i = 0; i < EACH; ++i) {
-		const unsigned long long set = __ballot(marks >> i & 1);
-		if (marks >> i & 1) list[at + __popcll(set & ((1ull << lane) - 1))] = (unsigned short) (i * TPB + t);
-		at += __popcll(set);
-	}
-	__syncthreads();
-	const int tiles = (a.N + 16 * WAVES - 1) / (16 * WAVES), tile0 = blockIdx.x * per, tile1 = min(tiles, tile0 + per);
-	for (int first = blockIdx.y * ROWS; first < count; first += gridDim.y * ROWS) {
-		long x_at[MT];
-#pragma unroll
-		for (int i = 0; i < MT; ++i) x_at[i] = (base + list[min(first + (t + TPB * i) / 16, count - 1)]) * a.ldx;
-		double sum[MT][4];
-#pragma unroll
-		for (int m = 0; m < MT; ++m)
-#pragma unroll
-			for (int i = 0; i < 4; ++i) sum[m][i] = 0.0;
-		for (int tile = tile0; tile < tile1; ++tile) {
-			const int n = (tile * WAVES + wave) * 16 + r;
-			const long entry = (long) min(n, a.N - 1) * a.ldw;
-			floatx4 rr[MT], ii[MT], ri[MT];
-			__syncthreads();  // (the buffers' last readers)
-			score_tile<MT, V4>(a, a.w_re + entry, a.w_im + entry, x_at, xs, rr, ii, ri);
-			if (n < a.N) {
-#pragma unroll
-				for (int m = 0; m < MT; ++m)
-#pragma unroll
-					for (int i = 0; i < 4; ++i) {
-						const float z_r = rr[m][i] - ii[m][i], z_i = ri[m][i];
-						sum[m][i] = fma((double) z_i, (double) z_i, fma((double) z_r, (double) z_r, sum[m][i]));
-					}
-			}
-		}
-#pragma unroll
-		for (int m = 0; m < MT; ++m)
-#pragma unroll
-			for (int i = 0; i < 4; ++i) {
-				double v = sum[m][i];
-				v += exchange<double, 0>(v);
-				v += exchange<double, 1>(v);
-				v += exchange<double, 2>(v);
-				v += exchange<double, 3>(v);
-				if (r == 0) met[wave][16 * m + 4 * q + i] = v;
-			}
-		__syncthreads();
-		if (t < ROWS && first + t < count) {
-			double v = met[0][t];
-			for (int w = 1; w < WAVES; ++w) v += met[w][t];
-			st.part[(base + list[first + t]) * st.slabs + blockIdx.x] = v;
-		}
-		// (met is written again behind the barriers of the next group's tiles)
-	}
-}
-
 // ---- The label's term of the weights' gradient: dw[label[r]] -= c_r x_r for every row r.  Labels of a text repeat (the most
 // frequent token of a batch of 8192 names hundreds of rows), so the rows are put in order of their labels first and then worked
 // off in chunks of equal length, whatever the labels.  The order is the stable one, so a label's rows are added in order.
@@ -1123,29 +1002,6 @@ __global__ __launch_bounds__(TPB) void head_label_join_kernel(const ScatterArgs 
 	dst.subtract(a, label, c, re, im);
 }
 
-// Fills what lies below the diagonal of a Hermitian matrix from what lies above it: C[j][i] = conj(C[i][j]).
-// Tiles of 32 x 32 turned over in LDS; blockIdx (x, y) = tile (column, row) of the part that is there.  diag (or NULL) receives the
-// diagonal, which a pass over the rows of x would otherwise gather line by line.  1024 x 1024: 6 us, a launch and two misses.
-__global__ __launch_bounds__(TPB) void head_mirror_kernel(float *__restrict__ c_re, float *__restrict__ c_im, long ldc, int K,
-		float *__restrict__ diag) {
-	__shared__ float tile[2][32][33];
-	const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
-	if (r0 == c0 && diag && threadIdx.x < 32 && r0 + (int) threadIdx.x < K) diag[r0 + threadIdx.x] = c_re[(r0 + threadIdx.x) * (ldc + 1)];
-	if (c0 < r0) return;
-	const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-	for (int k = ty; k < 32; k += 8)
-		if (r0 + k < K && c0 + tx < K) {
-			tile[0][k][tx] = c_re[(long) (r0 + k) * ldc + c0 + tx];
-			tile[1][k][tx] = c_im[(long) (r0 + k) * ldc + c0 + tx];
-		}
-	__syncthreads();
-	for (int k = ty; k < 32; k += 8)
-		if (c0 + k < K && r0 + tx < K && c0 + k > r0 + tx) {
-			c_re[(long) (c0 + k) * ldc + r0 + tx] = tile[0][tx][k];
-			c_im[(long) (c0 + k) * ldc + r0 + tx] = -tile[1][tx][k];
-		}
-}
-
 // Copies of both operands: dst[plane][r][c] = src_plane[r][c] inside rows x cols, zero outside.  The first blocks x copy x, the
 // others w; blockIdx.y = plane.  One thread per four columns of dst.  1000 + 5003 rows of 333: 8 us.
 struct PackArgs {
@@ -1223,14 +1079,13 @@ static int distill(const DistillArgs &a) {
 // what the calls of the head keep between their launches, carved out of one buffer of the library
 struct HeadBuffers {
 	RowState st;
-	float *piece, *y, *xs, *gram;  // planes re, im
-	float *diag;
+	float *piece, *y, *xs;         // planes re, im
+	Gram64 gram;                   // T, then P
 	float *x, *w;                  // copies of the operands (HeadPad)
 	int *row_of, *label_of;
 	float *label_part;
 	int piece_cols;                // columns of one piece, also its leading dimension
-	int per;                       // tiles of head_direct_kernel to a slab
-	long ldk;                      // leading dimension of y, xs and gram
+	long ldk;                      // leading dimension of y and xs
 };
 
 struct HeadPlan {
@@ -1249,14 +1104,6 @@ static long piece_bytes() {
 	return mb << 20;
 }
 
-// A Gram matrix (K x K, over L rows): the product leaves out the blocks below the diagonal and a pass of 5 us fills them in, if that
-// is less than what they would take.  A whole call, all blocks / half of them: 8192 rows x 1024 -> 32768 entries 5141 / 3933 us,
-// 2048 x 336 -> 8192 243 / 212, 4000 x 128 -> 30000 170 / 155; but 2000 x 192 -> 8000 128 / 129 and 1000 x 256 -> 4096 106 / 113.
-static bool half_product(int K, int L) { return K > 64 && (double) K * K * L >= 4.0e8; }
-static bool half_product(int K, int L, const float *re, const float *im, long ld) {
-	return half_product(K, L) && ld % 4 == 0 && ld < (1L << 22) && aligned16(re) && aligned16(im);
-}
-
 // Whether the label's terms go to dx and dw by themselves where the logits lie whole: three launches, 15 us, for digits.  dx off by,
 // among the others / apart: 300 x 1500 x 40000 1.6e-6 / 6e-8 (3761 -> 3784 us), 531 x 1000 x 4000 8e-7 / 5e-8; what
 // is left among the others (sums of 1024, or calls of less than about 130 us, whose sums the wavefronts share) stays within 5e-7
@@ -1266,13 +1113,13 @@ static bool label_apart(int B, int K, int N) {
 	return longest > 4096 || (longest > 1024 && (double) B * N * K > (double) (1 << 28));
 }
 
-// Which way the call goes, by what its launches take: a product of m complex multiplications about 4 us + 8 m flop at 130 TFLOP/s,
-// any other kernel about 3 us, plus its bytes.
+// Which way the call goes, by what its launches take: an fp32 product of m complex multiplications about 4 us + 8 m flop at 130
+// TFLOP/s, the products in double by their matrix instructions, any other kernel about 3 us, plus its bytes.
 //   whole   the logits in one piece, turned into their gradient where they lie; dx and dw from it: three products, one kernel.  The
 //           label's large entry among them costs the products' sums digits as they get long (label_apart)
 //   pieces  the logits piece by piece, and a second time for dw; the label's term by itself
-//   gram    T over N, y over K, P = x^H (x / S) over B, dw from it over K; the label's term by itself.  The argmax needs the logits
-//           all the same.
+//   gram    T over N, y over K, P = x^H (x / S) over B, dw from it over K, all in double; the label's term by itself.  The argmax needs
+//           the logits all the same.
 static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	static const int forced = [] {
 		const char *e = getenv("CNET_HEAD_GRAM");  // tuning override: 0 / 1 never / always through the Gram matrix
@@ -1288,10 +1135,10 @@ static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	auto bytes = [](double v) { return 3.0 + v / 4e6; };
 	const double label = bwd ? 20 + bytes(60 * b * k) : 0;
 	const double scan = pieces * (product(b * n * k / pieces) + bytes(8 * b * n / pieces));
-	double direct, gram = (half_product(K, N) ? 0.6 : 1.0) * product(n * k * k) + product(b * k * k) + (argmax ? scan : bytes(16 * b * k) + 3) + bytes(24 * b * k);
+	double direct, gram = gram64_us(K, N) + times_gram_us(B, K) + (argmax ? scan : 0.0) + bytes(bwd ? 24 * b * k : 0.0);
 	if (pieces == 1) direct = scan + (bwd ? bytes(16 * b * n) + 2 * product(b * n * k) + (label_apart(B, K, N) ? label : 0) : 0);
 	else direct = scan + bytes(24 * b * k) + (bwd ? pieces * 3 * product(b * n * k / pieces) + label : 0);
-	if (bwd) gram += (half_product(K, B) ? 0.6 : 1.0) * product(b * k * k) + product(n * k * k) + label;
+	if (bwd) gram += gram64_us(K, B) + times_gram_us(N, K) + label;
 	p.gram = (bwd || !argmax) && (forced >= 0 ? forced != 0 : gram < direct);
 	p.whole = !p.gram && pieces == 1;
 	p.label = bwd && (!p.whole || label_apart(B, K, N));
@@ -1310,8 +1157,8 @@ struct HeadPad {
 static HeadPad head_pad(const HeadArgs &a, int B, const HeadPlan &plan) {
 	auto up = [](int v) { return (v + 15) / 16 * 16; };
 	HeadPad p = {false, B, a.K, a.N};
-	if ((double) a.N * a.K < (double) (1 << 18)) return p;
-	if (plan.bwd) p.B = up(B);
+	if ((double) a.N * a.K < (double) (1 << 18) || (plan.gram && !plan.pieces)) return p;  // (the products in double take any layout)
+	if (plan.bwd && !plan.gram) p.B = up(B);
 	const bool odd = a.K % 16 || a.ldx % 4 || a.ldw % 4 || !aligned16(a.x_re) || !aligned16(a.x_im) || !aligned16(a.w_re) || !aligned16(a.w_im);
 	if (odd && 8.0 * up(a.N) * up(a.K) <= (double) (1L << 31)) {
 		p.copy = true;
@@ -1321,21 +1168,19 @@ static HeadPad head_pad(const HeadArgs &a, int B, const HeadPlan &plan) {
 	return p;
 }
 
-static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b) {
+static int head_buffers(const HeadPad &pad, const HeadPlan &plan, int K, HeadBuffers &b) {
 	b.piece_cols = plan.piece_cols;
 	b.ldk = ((long) pad.K + 3) / 4 * 4;
 	const size_t rows = ((size_t) pad.B + 63) / 64 * 64;
 	const size_t piece = plan.pieces || plan.whole ? 2 * (size_t) pad.B * b.piece_cols : 0;
-	const size_t wide = plan.bwd || plan.gram ? 2 * (size_t) pad.B * b.ldk : 0, square = plan.gram ? 2 * (size_t) pad.K * b.ldk : 0;
-	// the parts of the vocabulary that a marked row is dealt out in: at most an eighth of what y takes for the row, or 32
-	const int tiles = (pad.N + 16 * WAVES - 1) / (16 * WAVES), most = std::min(128, std::max(32, pad.K / 8));
-	b.per = (tiles + most - 1) / most;
-	b.st.slabs = (tiles + b.per - 1) / b.per;
-	const size_t part = plan.gram && !plan.pieces ? 2 * (size_t) b.st.slabs * rows : 0;
+	const size_t wide = plan.bwd ? 2 * (size_t) pad.B * b.ldk : 0, xs = plan.gram ? 0 : wide;
+	b.gram.ld = K;
+	b.st.slabs = (K + GRAM_TILE - 1) / GRAM_TILE;
+	const size_t square = plan.gram ? 4 * (size_t) K * K : 0, part = plan.gram ? 2 * (size_t) b.st.slabs * rows : 0, weight = plan.gram ? 2 * rows : 0;
 	const bool label = plan.label;
 	const size_t order = label ? rows : 0, label_part = label ? (size_t) (std::min(pad.B, ORDER_ROWS) + CHUNK - 1) / CHUNK * 4 * b.ldk : 0;
 	const size_t copy_x = pad.copy ? 2 * (size_t) pad.B * b.ldk : 0, copy_w = pad.copy ? 2 * (size_t) pad.N * b.ldk : 0;
-	float *p = (float *) vocab_workspace((6 * rows + part + piece + 2 * wide + square + 2 * order + label_part + copy_x + copy_w + (plan.gram ? b.ldk : 0)) * sizeof(float));
+	float *p = (float *) vocab_workspace((6 * rows + square + part + weight + piece + wide + xs + 2 * order + label_part + copy_x + copy_w) * sizeof(float));
 	if (!p) return rt().capturing ? CNET_ERR_UNSUPPORTED : CNET_ERR_OUT_OF_MEMORY;
 	auto take = [&](size_t floats) {
 		float *q = p;
@@ -1343,16 +1188,16 @@ static int head_buffers(const HeadPad &pad, const HeadPlan &plan, HeadBuffers &b
 		return q;
 	};
 	b.st.sum = (double *) take(2 * rows);
+	b.gram.re = (double *) take(square);
 	b.st.part = (double *) take(part);
+	b.st.weight = (double *) take(weight);
 	b.st.best = take(rows);
 	b.st.index = (int *) take(rows);
 	b.st.c_re = take(rows);
 	b.st.c_im = take(rows);
 	b.piece = take(piece);
 	b.y = take(wide);
-	b.xs = take(wide);
-	b.gram = take(square);
-	b.diag = take(plan.gram ? b.ldk : 0);
+	b.xs = take(xs);
 	b.label_part = take(label_part);
 	b.row_of = (int *) take(order);
 	b.label_of = (int *) take(order);
@@ -1376,17 +1221,6 @@ static int conj_product_pair(bool a_kmajor, int M, int N, int K, const float *a_
 	float *cr[2] = {cs_re, c_re}, *ci[2] = {cs_im, c_im};
 	const bool cj[2] = {true, true};
 	return cgemm_pair(a_kmajor, true, 1, M, N, K, ar, ai, lda, br, bi, ldb, cj, cr, ci, ldc, accumulate, 0, 1);
-}
-
-// C = A^H A [K][K] for an A of L rows; half of it by the product where that pays, its diagonal then to diag (or NULL) as well
-static int gram_product(int K, int L, const float *a_re, const float *a_im, long lda, float *c_re, float *c_im, long ldc, float *diag) {
-	if (!half_product(K, L, a_re, a_im, lda)) return conj_product(1, K, K, L, a_re, a_im, lda, a_re, a_im, lda, c_re, c_im, ldc, 0);
-	const int rc = cgemm_gram(K, L, a_re, a_im, lda, c_re, c_im, ldc);
-	if (rc) return rc;
-	const unsigned tiles = (unsigned) ((K + 31) / 32);
-	hipLaunchKernelGGL(head_mirror_kernel, dim3(tiles, tiles), dim3(TPB), 0, rt().stream, c_re, c_im, ldc, K, diag);
-	CNET_LAUNCH_CHECK();
-	return CNET_OK;
 }
 
 static int head_labels(const HeadArgs &a, const HeadBuffers &b, int B, float *dw_re, float *dw_im, float *dws_re, float *dws_im, long lddw) {
@@ -1438,39 +1272,24 @@ static int head_score(const HeadArgs &a, int B) {
 }
 
 template <int T, int V>
-static void launch_finish(const HeadArgs &a, const RowState &st, bool bwd, bool gram, const float *diag_at, long diag_step, int rows) {
+static void launch_finish(const HeadArgs &a, const RowState &st, bool bwd, bool gram, int rows) {
 	const dim3 grid((unsigned) ((rows + TPB / T - 1) / (TPB / T)));
-	if (bwd && gram) hipLaunchKernelGGL((head_finish_kernel<T, V, true, true>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
-	else if (bwd) hipLaunchKernelGGL((head_finish_kernel<T, V, true, false>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
-	else if (gram) hipLaunchKernelGGL((head_finish_kernel<T, V, false, true>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
-	else hipLaunchKernelGGL((head_finish_kernel<T, V, false, false>), grid, dim3(TPB), 0, rt().stream, a, st, diag_at, diag_step, rows);
+	if (bwd && gram) hipLaunchKernelGGL((head_finish_kernel<T, V, true, true>), grid, dim3(TPB), 0, rt().stream, a, st, rows);
+	else if (bwd) hipLaunchKernelGGL((head_finish_kernel<T, V, true, false>), grid, dim3(TPB), 0, rt().stream, a, st, rows);
+	else if (gram) hipLaunchKernelGGL((head_finish_kernel<T, V, false, true>), grid, dim3(TPB), 0, rt().stream, a, st, rows);
+	else hipLaunchKernelGGL((head_finish_kernel<T, V, false, false>), grid, dim3(TPB), 0, rt().stream, a, st, rows);
 }
 
-// the pass over the rows behind the products that give y; gram: the sums come from it, with the diagonal of T, one element every diag_step
-static int head_finish(const HeadArgs &a, const RowState &st, int per, bool bwd, bool gram, const float *diag_at, long diag_step, int rows) {
+// the pass over the rows behind the products that give y
+static int head_finish(const HeadArgs &a, const RowState &st, bool bwd, bool gram, int rows) {
 	auto m4 = [](long v) { return v % 4 == 0; };
 	const bool vec = m4(a.K) && m4(a.ldx) && m4(a.ldw) && (!bwd || m4(a.lddx)) && aligned16(a.x_re) && aligned16(a.x_im) && aligned16(a.w_re) &&
 			aligned16(a.w_im) && aligned16(a.dx_re) && aligned16(a.dx_im) && aligned16(a.dxs_re) && aligned16(a.dxs_im);
 	// a wavefront per row up to 512 columns (or what 128-bit accesses make of them), a workgroup beyond
-	if (vec && a.K <= 512) launch_finish<64, 4>(a, st, bwd, gram, diag_at, diag_step, rows);
-	else if (vec) launch_finish<256, 4>(a, st, bwd, gram, diag_at, diag_step, rows);
-	else if (a.K <= 256) launch_finish<64, 1>(a, st, bwd, gram, diag_at, diag_step, rows);
-	else launch_finish<256, 1>(a, st, bwd, gram, diag_at, diag_step, rows);
-	CNET_LAUNCH_CHECK();
-	if (!gram) return CNET_OK;
-	const unsigned groups = (unsigned) ((a.B + HEAD_ROWS - 1) / HEAD_ROWS);
-	// (as many workgroups as fill the device twice share the groups of marked rows, should there be many)
-	const unsigned blocks = (unsigned) ((a.B + DIRECT_BLOCK - 1) / DIRECT_BLOCK);
-	const unsigned share = (unsigned) std::max(1, std::min(DIRECT_BLOCK / (16 * DIRECT_MT), 2 * rt().prop.multiProcessorCount / (int) (st.slabs * blocks)));
-	const dim3 grid((unsigned) st.slabs, share, blocks);
-	if (m4(a.ldx) && m4(a.ldw) && aligned16(a.x_re) && aligned16(a.x_im) && aligned16(a.w_re) && aligned16(a.w_im))
-		hipLaunchKernelGGL(head_direct_kernel<true>, grid, dim3(TPB), 0, rt().stream, a, st, per);
-	else hipLaunchKernelGGL(head_direct_kernel<false>, grid, dim3(TPB), 0, rt().stream, a, st, per);
-	CNET_LAUNCH_CHECK();
-	if (vec && bwd) hipLaunchKernelGGL((head_finish_marked_kernel<4, true>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
-	else if (vec) hipLaunchKernelGGL((head_finish_marked_kernel<4, false>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
-	else if (bwd) hipLaunchKernelGGL((head_finish_marked_kernel<1, true>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
-	else hipLaunchKernelGGL((head_finish_marked_kernel<1, false>), dim3(groups), dim3(TPB), 0, rt().stream, a, st);
+	if (vec && a.K <= 512) launch_finish<64, 4>(a, st, bwd, gram, rows);
+	else if (vec) launch_finish<256, 4>(a, st, bwd, gram, rows);
+	else if (a.K <= 256) launch_finish<64, 1>(a, st, bwd, gram, rows);
+	else launch_finish<256, 1>(a, st, bwd, gram, rows);
 	CNET_LAUNCH_CHECK();
 	return CNET_OK;
 }
@@ -1483,7 +1302,7 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 	const HeadPlan plan = head_plan(B, K, N, bwd, a.argmax || !a.labels);
 	const HeadPad pad = head_pad(a, B, plan);
 	HeadBuffers b;
-	int rc = head_buffers(pad, plan, b);
+	int rc = head_buffers(pad, plan, K, b);
 	if (rc) return rc;
 	const int np = b.piece_cols, Kp = pad.K;  // Kp: K, or K filled up with zeros where the operands are copies
 	const long ldk = b.ldk;
@@ -1500,7 +1319,6 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 	}
 	float *z_re = b.piece, *z_im = b.piece + (size_t) pad.B * np;
 	float *y_re = b.y, *y_im = b.y + (size_t) pad.B * ldk;
-	float *g_re = b.gram, *g_im = b.gram + (size_t) Kp * ldk;
 	a.y_re = y_re;
 	a.y_im = y_im;
 	a.xs_re = b.xs;
@@ -1544,19 +1362,18 @@ static int head(const HeadArgs &proto, int B, float *dw_re, float *dw_im, float 
 		}
 	}
 	if (plan.gram) {
-		rc = gram_product(Kp, pad.N, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, b.diag);
+		rc = gram64(K, N, a.w_re, a.w_im, a.ldw, nullptr, b.gram);
 		if (rc) return rc;
-		rc = conj_product(0, B, K, Kp, a.x_re, a.x_im, a.ldx, g_re, g_im, ldk, y_re, y_im, ldk, 0);
+		rc = times_gram(B, K, a.x_re, a.x_im, a.ldx, b.gram, GramOut{bwd ? y_re : nullptr, bwd ? y_im : nullptr, nullptr, nullptr, ldk, 0, b.st.part});
 		if (rc) return rc;
 	}
-	const bool apart = half_product(Kp, pad.N, a.w_re, a.w_im, a.ldw);  // the diagonal of T lies by itself
-	rc = head_finish(a, b.st, b.per, bwd, plan.gram && !plan.pieces, apart ? b.diag : g_re, apart ? 1 : ldk + 1, bwd ? pad.B : B);
+	rc = head_finish(a, b.st, bwd, plan.gram, bwd ? pad.B : B);
 	if (rc) return rc;
 	if (!bwd) return CNET_OK;
 	if (plan.gram) {
-		rc = gram_product(Kp, pad.B, a.xs_re, a.xs_im, ldk, g_re, g_im, ldk, nullptr);
+		rc = gram64(K, B, a.x_re, a.x_im, a.ldx, b.st.weight, b.gram);
 		if (rc) return rc;
-		rc = conj_product_pair(false, N, K, Kp, a.w_re, a.w_im, a.ldw, g_re, g_im, ldk, dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw);
+		rc = times_gram(N, K, a.w_re, a.w_im, a.ldw, b.gram, GramOut{dw_re, dw_im, dws_re, dws_im, lddw, accumulate_dw, nullptr});
 		if (rc) return rc;
 	}
 	for (int n0 = 0; !plan.gram && n0 < N; n0 += np) {  // the logits again, over sqrt(S) and zero where a row is left out
