@@ -393,7 +393,7 @@ __global__ __launch_bounds__(TPB) void head_piece_kernel(const float *__restrict
 // Where x lies in directions that w hardly has (or a row of w in directions that the batch hardly has) these sums are small and
 // their terms are not.  With D = sum |x_i|^2 T_ii, what their terms amount to, a sum of rounded terms is off by D / S roundings, where the sum
 // over the logits is off by about sqrt(D / S).  T, y, S and P are therefore formed and kept in double (gram.hip), which is
-// closer than logits in single precision down to D / S = 1e17, where these have no digit left.
+// closer than logits in single precision wherever these have a digit left (D / S up to 1e14).
 struct HeadArgs {
 	const float *x_re, *x_im, *w_re, *w_im;
 	long ldx, ldw;
@@ -514,7 +514,7 @@ __device__ __forceinline__ void finish_row(const HeadArgs &a, const RowState &st
 
 // T threads per row (64: four rows to a workgroup).  GRAM: the sum is added up from its parts.  Rows beyond B, which fill up the last
 // chunk of the weights' product, become zero in xs.
-// Bound by memory: y and the labels' rows of w are read, dx written; 8192 x 1024, 201 MB, takes @@ us.
+// Bound by memory: y and the labels' rows of w are read, dx written; 8192 x 1024, 201 MB, takes 42 us, 4.8 TB/s.
 template <int T, int V, bool BWD, bool GRAM>
 __global__ __launch_bounds__(TPB) void head_finish_kernel(const HeadArgs a, RowState st, int rows) {
 	constexpr int G = T / 64, ROWS = TPB / T;

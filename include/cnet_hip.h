@@ -587,12 +587,13 @@ int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, 
  * the rows in an order that depends on the sizes alone, their dz* halves optional, each with its accumulate flag.  With B == 0 dw
  * is zero (or left).
  * How: the loss depends on the logits through a quadratic form of x, so with T = w^H w and P = x^H diag(1 / s) x neither s nor
- * either gradient needs them (N K^2 + B K^2 products for B N K); rows in directions that w hardly has are summed from w itself.
- * The smaller heads form the logits in a buffer of the library, whole or in pieces of the vocabulary; a few rows are scored in one
- * pass over w.  The argmax needs the logits: a step without it is the faster one.  Products of two weights, and of two entries of
- * x / sqrt(s), are formed in single precision and have to stay within its range.
- * The buffer holds a few planes of [B x K] and [K x K] or at most about 192 MiB of logits (more only where 64 columns of B rows
- * are), with one aligned copy of w (up to 2 GiB) where K is not a multiple of 16 or a plane not aligned to 16 bytes.
+ * either gradient needs them (N K^2 + B K^2 products for B N K).  T, P and the sums that come of them are double, so that rows in directions
+ * that w hardly has, and entries of w in directions that the batch hardly has, keep their digits.  The smaller heads form the logits in a
+ * buffer of the library, whole or in pieces of the vocabulary; a few rows are scored in one pass over w.  The argmax needs the logits: a
+ * step without it is the faster one.  s, and the sums conj(z) w over the vocabulary, have to stay within the range of single precision.
+ * The library's buffer holds a few planes of [B x K], two of [K x K] in double, or at most about 192 MiB of logits (more only where 64 columns
+ * of B rows are), with one aligned copy of w (up to 2 GiB) where logits are formed and K is not a multiple of 16 or a plane not aligned to
+ * 16 bytes; it and the workspace (up to 512 MiB for parts of T) are allocated half as large again.
  * B < 2^24, K < 2^30, N < 2^28; results must not overlap operands. */
 int cnet_vocab_head_fwd(const float *x_re, const float *x_im, int64_t ldx, const float *w_re, const float *w_im, int64_t ldw,
                         const int32_t *labels, float *s, float *loss, int32_t *argmax, int B, int K, int N);

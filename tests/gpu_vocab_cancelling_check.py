@@ -22,6 +22,10 @@ def main():
         for argmax in (False, True):
             print(B, K, N, argmax, flush=True)
             cancelling_check(rounded(x), rounded(w), labels, True, pad, off, argmax)
+    # leading dimensions whose offsets inside a block of 64 rows pass 32 bits
+    x, w, labels = head_data(np.random.default_rng(3), 2, 5, 3)
+    print("far", flush=True)
+    cancelling_check(rounded(x), rounded(w), labels, True, 1 << 23)
     for B, K, N, pad, off in CANCELLING + [(129, 72, 65, 4, 0), (40, 130, 9000, 0, 0)]:
         for weak in WEAK:
             print(B, K, N, weak, flush=True)
