@@ -151,7 +151,7 @@ __device__ __forceinline__ void entry_gradients(const DistillArgs &a, const Entr
 }
 
 // The row in registers: T threads hold V x NIT columns each, so z is read once and the gradient written once, 16 bytes per element
-// each way (24 with dz*), which is what bounds it: 8192 x 32768 takes 802 us, 5.4 TB/s (a copy of 1 GiB: 5.1).  The entries and their
+// each way (24 with dz*), which is what bounds it: 8192 x 32768 takes 802 us among other work, 5.4 TB/s (a copy of 1 GiB: 5.1).  The entries and their
 // values are fetched while the row is on its way.  T = 64: four rows to a workgroup (96 x 512: 4.9 us, a launch).
 // LONG: the columns that the registers do not hold are read once more for the gradient (4096 x 50257, 36 of 100 columns: 786 us).
 template <int T, int NIT, int V, bool LONG>
@@ -1055,7 +1055,7 @@ static int distill(const DistillArgs &a) {
 		CNET_LAUNCH_CHECK();
 		return CNET_OK;
 	}
-	// (8192 x 32768, read once and written once: 772 us with the streaming hint on both sides, 801 on the stores, 862 on the loads, 824
+	// (8192 x 32768, read once and written once, repeated on the same planes: 772 us with the streaming hint on both sides, 801 on the stores, 862 on the loads, 824
 	// with none; 5.6 TB/s)
 	const int policy = stream_policy(a.dz_re ? ST_BOTH : ST_LOADS, !a.dz_re ? 2 : a.dzs_re ? 6 : 4, (long) a.rows * a.cols);
 #define CNET_DISTILL(T, E, LONG)                                                                                                                     \

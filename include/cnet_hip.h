@@ -561,8 +561,8 @@ int cnet_norm_join_bwd_sym(const float *f_re, const float *f_im, int64_t ldf, co
  *        loss = sum_j q_j (log q_j - log max(p[id_j], 1e-15))        dz_k = conj(z_k) (Q / s - q(k) / max(|z_k|^2, 1e-15))
  * with Q the sum of a row's weights q_j and q(k) the sum of those whose id is k (the same id may come more than once).
  * ids[rows][top] int32, probs[rows][top] >= 0, 1 <= top <= CNET_DISTILL_MAX_TOP; they need not add up to 1.  An entry with a
- * negative id is padding and left out of everything; a row of padding has loss 0 and gradient 0.  An id >= cols gives its row
- * a NaN loss and counts in Q alone, as a label outside the row does in CrossEntropy.  One entry of weight 1 is CrossEntropy.
+ * negative id is padding and left out of everything; a row of padding has loss 0 and gradient 0, whatever it holds.  An id >= cols with
+ * a weight gives its row a NaN loss and counts in Q alone, as a label outside the row does in CrossEntropy.  One entry of weight 1 is CrossEntropy.
  * The gradient is assigned; its dz* half may be NULL.  cnet_distill_fwd_bwd_sym gives the results of the other two in one
  * call, with z read once where a row fits a workgroup's registers (32768 columns).  `loss` may point into memory from
  * cnet_host_alloc.  Fewer than 2^22 rows and 2^30 columns; results must not overlap operands. */
@@ -584,7 +584,7 @@ int cnet_distill_fwd_bwd_sym(const float *z_re, const float *z_im, int64_t ldz, 
  * as in cnet_cross_entropy_bwd (no entry is the label).  cnet_vocab_head_fwd: labels NULL takes each row's argmax for its label
  * (scoring: loss is then -log of the largest probability); loss or argmax may be NULL, not both.
  * cnet_vocab_head_fwd_bwd_sym: argmax may be NULL; dx and dw are the conjugate pairs of the gradients at x and w, summed over
- * the rows in an order that depends on the sizes alone, their dz* halves optional, each with its accumulate flag.  With B == 0 dw
+ * the rows in an order that sizes, strides and alignment decide, their dz* halves optional, each with its accumulate flag.  With B == 0 dw
  * is zero (or left).
  * How: the loss depends on the logits through a quadratic form of x, so with T = w^H w and P = x^H diag(1 / s) x neither s nor
  * either gradient needs them (N K^2 + B K^2 products for B N K).  T, P and the sums that come of them are double, so that rows in directions
@@ -617,10 +617,12 @@ int cnet_vocab_head_fwd_bwd_sym(const float *x_re, const float *x_im, int64_t ld
  *   CNET_CGEMM_SKINNY = 0        small products on the block kernels instead of the small-C kernel
  *   CNET_CGEMM_SKINNY_TILES = n  largest number of 16x16 tiles of C the small-C kernel takes (default 4 per compute unit)
  *   CNET_CGEMM_SKINNY_W = 4|8|16 wavefronts per tile of the small-C kernel
- *   CNET_CGEMM_SKINNY_TWO = 0    two small products of one call as two launches (and the gate behind them as launches of its own)
+ *   CNET_CGEMM_SKINNY_TWO = 0    two small products of one call as two launches (and the gate behind them as launches of its own),
+ *                                also in the vocabulary head
  *   CNET_CGEMM_3M = 0 | 1        initial value of cnet_cgemm_set_products (1: three real products per complex one)
  *   CNET_CGEMM_PACK = 0          large products of misaligned operands on the operands as they are (no aligned copies)
- *   CNET_HEAD_GRAM = 0 | 1       the vocabulary head never / always through w^H w (default: by what its products cost)
+ *   CNET_HEAD_GRAM = 0 | 1       the vocabulary head never / always through w^H w (default: by what its products cost; up to 64 rows
+ *                                are scored in one pass over w all the same)
  *   CNET_HEAD_PIECE_MB = n       size of the buffer for logits in cnet_vocab_head_* (default 192)
  *   CNET_DFT_FOLD = 0            the transform of real samples without folding them about n/2 first
  *   CNET_STREAM_MIN_MB = n       footprint (MiB) from which an elementwise / row launch counts as streaming (default 256)
