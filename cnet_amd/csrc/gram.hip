@@ -316,12 +316,12 @@ namespace cnet {
 double gram64_us(int K, int L) {
 	const int s = gram_splits(K, L), chunks = (L + KC - 1) / KC;
 	const double tiles = (K + BT - 1) / BT, cus = rt().prop.multiProcessorCount;
-	return 16.0 + 1.24 * std::ceil(tiles * (tiles + 1) / 2 * s / cus) * ((chunks + s - 1) / s) * chunk_us() + (s + 1) * 8.0 * K * K / 3e6;
+	return 11.0 + 1.24 * std::ceil(tiles * (tiles + 1) / 2 * s / cus) * ((chunks + s - 1) / s) * chunk_us() + (s + 1) * 8.0 * K * K / 3e6;
 }
 
 double times_gram_us(int M, int K) {
 	const double blocks = (double) ((M + BT - 1) / BT) * ((K + BT - 1) / BT);
-	return 14.0 + 1.24 * std::ceil(blocks / rt().prop.multiProcessorCount) * ((K + KC - 1) / KC) * chunk_us();
+	return 9.0 + 1.24 * std::ceil(blocks / rt().prop.multiProcessorCount) * ((K + KC - 1) / KC) * chunk_us();
 }
 
 int gram64(int K, int L, const float *a_re, const float *a_im, long lda, const double *weight, const Gram64 &c) {

@@ -1113,8 +1113,10 @@ static bool label_apart(int B, int K, int N) {
 	return longest > 4096 || (longest > 1024 && (double) B * N * K > (double) (1 << 28));
 }
 
-// Which way the call goes, by what its launches take: an fp32 product of m complex multiplications about 4 us + 8 m flop at 130
-// TFLOP/s, the products in double by their matrix instructions, any other kernel about 3 us, plus its bytes.
+// Which way the call goes, by what its launches take: an fp32 product of m complex multiplications about 8 us + 8 m flop at 115
+// TFLOP/s, the products in double by their matrix instructions, any other kernel about 3 us, plus its bytes.  Steps without the argmax, the
+// logits as a whole / through the Gram matrices, both measured: 1188 x 125 -> 1869 155 / 108 us, 1155 x 551 -> 862 202 / 243, 7365 x 490 -> 633
+// 601 / 524, 1624 x 1537 -> 305 269 / 1071, 2333 x 594 -> 5021 1471 / 636, 2183 x 1696 -> 8441 5689 / 4816, 331 x 675 -> 1215 138 / 280.
 //   whole   the logits in one piece, turned into their gradient where they lie; dx and dw from it: three products, one kernel.  The
 //           label's large entry among them costs the products' sums digits as they get long (label_apart)
 //   pieces  the logits piece by piece, and a second time for dw; the label's term by itself
@@ -1131,7 +1133,7 @@ static HeadPlan head_plan(int B, int K, int N, bool bwd, bool argmax) {
 	p.piece_cols = (int) std::min(all, std::max(64L, piece_bytes() / (8 * (long) B) / 64 * 64));
 	const int pieces = (N + p.piece_cols - 1) / p.piece_cols;
 	const double b = B, k = K, n = N;
-	auto product = [](double m) { return 4.0 + m * 8 / 130e6; };
+	auto product = [](double m) { return 8.0 + m * 8 / 115e6; };
 	auto bytes = [](double v) { return 3.0 + v / 4e6; };
 	const double label = bwd ? 20 + bytes(60 * b * k) : 0;
 	const double scan = pieces * (product(b * n * k / pieces) + bytes(8 * b * n / pieces));
