@@ -15,12 +15,11 @@
 // the operands' alignment); what is lost is lost at the barriers, hence eight wavefronts of 32 x 16, four to a SIMD with a second workgroup
 // beside (four of 32 x 32: 3.39 ms).
 #include "common.hpp"
+#include "gram.hpp"
 #include "rows.hpp"
 
 #include <algorithm>
 #include <cmath>
-
-#include "gram.hpp"
 
 namespace {
 
